@@ -10,11 +10,27 @@ after which ``DABSNModel``, ``DABSNSequenceLM``, ``train_step`` and the
 checkpoint code run unchanged on the B200 kernels.  The kernels themselves
 are a C-ABI shared library (``include/dabsn_b200.h``) loaded with ctypes;
 ``dabsn_b200.ops`` exposes them on torch tensors directly.
+
+``token_log_probs``, ``distillation_loss`` and ``embedding`` are differentiable
+functions of torch tensors that need neither the reference nor ``install``:
+scoring and distillation over a model's logits, and its token embedding.
 """
 
 from __future__ import annotations
 
+from .autograd import TokenLogProbs, distillation_loss, embedding, token_log_probs
 from .backend import b200_status, enable, enable_b200, install, native_available, status
 
-__all__ = ["b200_status", "enable", "enable_b200", "install", "native_available", "status"]
+__all__ = [
+    "TokenLogProbs",
+    "b200_status",
+    "distillation_loss",
+    "embedding",
+    "enable",
+    "enable_b200",
+    "install",
+    "native_available",
+    "status",
+    "token_log_probs",
+]
 __version__ = "0.1.0"

@@ -119,6 +119,25 @@ _SIGNATURES = {
     ),
     "dabsn_ce_logits_fwd": ([_i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp], _i32),
     "dabsn_ce_logits_bwd": ([_i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp], _i32),
+    "dabsn_token_scores_fwd": (
+        [_i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _i64] + [_vp] * 6, _i32),
+    "dabsn_token_scores_bwd": (
+        [_i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float] + [_vp] * 6, _i32),
+    "dabsn_distill_list_bytes": ([_i64, _i64], ctypes.c_size_t),
+    "dabsn_distill_prep": (
+        [_i32, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _i64, _vp, _vp], _i32),
+    "dabsn_distill_fwd": (
+        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float] + [_vp] * 3, _i32),
+    "dabsn_distill_bwd": (
+        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _i32, _vp, _i64, _vp, _vp],
+        _i32),
+    "dabsn_distill_reduce": ([_i64, _i64, _vp, _vp, _i32, _vp, _vp], _i32),
+    "dabsn_embedding_fwd": (
+        [_i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _vp], _i32),
+    "dabsn_embedding_bwd_workspace": ([_i64, _i64, _i64], ctypes.c_size_t),
+    "dabsn_embedding_bwd": (
+        [_i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _vp,
+         ctypes.c_size_t, _vp], _i32),
     "dabsn_input_proj_fwd": ([_i64, _i64, _i64, _vp, _i64] + [_vp] * 6, _i32),
     "dabsn_input_proj_bwd": ([_i64, _i64, _i64, _vp, _i64] + [_vp] * 8, _i32),
     "dabsn_rec_grad": ([_i64, _i64, _vp, _i64] + [_vp] * 5, _i32),
@@ -194,6 +213,7 @@ DEVICE_CODES = {
     4: "a bounded wait of the reverse scan timed out",
     6: "a bounded wait of the tensor-core GEMM timed out",
     7: "a cross-entropy target lies outside [0, V) and is not ignore_index",
+    8: "a token (to score, to look up, or of a teacher's list) lies outside [0, V)",
 }
 
 

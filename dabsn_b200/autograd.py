@@ -7,14 +7,19 @@
 * ``ThreeWayRead`` replaces the CUDA admitted read
   (``dabsn.kernels.triton.cuda_compact_three_way_read``).
 * ``LongScan`` replaces ``dabsn.kernels.long.fused_long_scan_from_state``.
+* ``token_log_probs``, ``distillation_loss`` and ``embedding`` are operators of
+  their own at the vocabulary ends of a model (the reference has no such
+  functions); they are exported as ``dabsn_b200.token_log_probs`` and so on.
 """
 
 from __future__ import annotations
 
 import os
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _native, ops
 
@@ -613,6 +618,194 @@ def make_ce_from_logits(original):
 
     chunked_cross_entropy_from_logits.__wrapped_reference__ = original
     return chunked_cross_entropy_from_logits
+
+
+class TokenLogProbs(NamedTuple):
+    """What :func:`token_log_probs` returns: FP32 numbers shaped like the
+    tokens, and the alternatives with one more axis (int64 ids)."""
+
+    log_prob: Tensor
+    entropy: Tensor
+    top_log_probs: Tensor
+    top_tokens: Tensor
+
+
+class _TokenScores(torch.autograd.Function):
+    """Log-probability and entropy of every row, differentiable in the logits;
+    saves the logits and two numbers a row."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
+        flat = logits.detach()
+        log_prob, entropy, top_values, top_ids, stats = ops.token_scores_forward(
+            flat, tokens, top_k, temperature, ignore_index, ctx.needs_input_grad[0])
+        ctx.mark_non_differentiable(top_values, top_ids)
+        ctx.set_materialize_grads(False)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, tokens, stats, entropy)
+        ctx.meta = (temperature, ignore_index)
+        return log_prob, entropy, top_values, top_ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, *_):
+        if g_log_prob is None and g_entropy is None:
+            return None, None, None, None, None
+        logits, tokens, stats, entropy = ctx.saved_tensors
+        temperature, ignore_index = ctx.meta
+        dl = ops.token_scores_backward(logits.detach(), tokens, temperature, ignore_index, stats,
+                                       entropy, g_log_prob, g_entropy)
+        return dl, None, None, None, None
+
+
+def _as_rows(logits: Tensor) -> Tensor:
+    """[..., V] as a matrix with contiguous rows; a view wherever the strides
+    allow one."""
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError("logits must have a vocabulary axis with at least one entry")
+    flat = logits.reshape(-1, logits.shape[-1])
+    rows_apart = flat.shape[0] <= 1 or flat.stride(0) >= flat.shape[1]
+    if (flat.stride(1) != 1 and flat.shape[1] > 1) or not rows_apart:
+        flat = flat.contiguous()
+    return flat
+
+
+def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperature: float = 1.0,
+                    ignore_index: int = -100) -> TokenLogProbs:
+    """Log-probabilities of given tokens under ``softmax(logits / temperature)``.
+
+    ``logits`` [..., V] (CUDA, FP32 or BF16; any row stride), ``tokens`` [...]
+    (int64 or int32).  Returns a :class:`TokenLogProbs`: ``log_prob`` and
+    ``entropy`` [...] in FP32, and the ``top_k`` (0 to 128) most likely tokens
+    of every row as ``top_log_probs`` / ``top_tokens`` [..., top_k], most
+    likely first, equal logits by the lower id.  ``log_prob`` and ``entropy``
+    are differentiable in the logits; the alternatives are not.
+
+    A row whose token is ``ignore_index`` is not read: log-probability and
+    entropy 0, alternatives -inf with id -1, no gradient.  A row whose logits
+    are all -inf has log-probability -inf, entropy 0, no gradient, and its
+    first ids as alternatives.  NaN or +inf among the logits makes the row's
+    numbers NaN (its alternatives' ids are then valid but unspecified).  A
+    token outside [0, V) makes its log-probability NaN and is raised at the
+    next synchronisation (device status 8)."""
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens has shape {tuple(tokens.shape)}, expected "
+                         f"{tuple(logits.shape[:-1])}")
+    shape = tokens.shape
+    with torch.autocast("cuda", enabled=False):
+        out = _TokenScores.apply(_as_rows(logits), tokens.reshape(-1), int(top_k),
+                                 float(temperature), int(ignore_index))
+    return TokenLogProbs(out[0].reshape(shape), out[1].reshape(shape),
+                         out[2].reshape(*shape, top_k), out[3].reshape(*shape, top_k))
+
+
+class _Distillation(torch.autograd.Function):
+    """Row losses (reduction "none"), their sum or their mean."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, ignore_index,
+                reduction):
+        entries = teacher_tokens.shape[1]
+        lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
+                                 ignore_index)
+        loss, stats = ops.distill_forward(logits.detach(), lists, entries, temperature)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, lists, stats)
+        ctx.meta = (entries, temperature, reduction)
+        if reduction == "none":
+            return loss
+        return ops.distill_reduce(loss, lists, entries, reduction == "mean")
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        logits, lists, stats = ctx.saved_tensors
+        entries, temperature, reduction = ctx.meta
+        dl = ops.distill_backward(logits.detach(), lists, entries, temperature, stats,
+                                  reduction == "mean", grad)
+        return dl, None, None, None, None, None
+
+
+def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor, *,
+                      temperature: float = 1.0, ignore_index: int = -100,
+                      reduction: str = "mean") -> Tensor:
+    """Distillation from a teacher's top logits:
+    ``temperature^2 * KL(q || softmax(logits / temperature))`` with ``q`` the
+    softmax of ``teacher_logits / temperature`` over the entries a row lists.
+
+    ``logits`` [..., V] (CUDA, FP32 or BF16; any row stride),
+    ``teacher_tokens`` [..., K] ids (int64 or int32, 1 to 256 a row) and
+    ``teacher_logits`` [..., K] (FP32 or BF16; logits or log-probabilities:
+    only their differences count).  Entries whose id is ``ignore_index`` are
+    absent; an id listed twice counts with both its entries.  ``reduction`` is
+    "mean" (over the rows that list anything; 0 if none does), "sum" or "none".
+    The loss is FP32; the gradient goes to ``logits`` alone, in their dtype.
+
+    A row that lists nothing, or whose teacher logits are all -inf, has loss 0
+    and no gradient, and its logits are not read.  A listed token whose logit
+    is -inf makes the loss +inf.  An id outside [0, V) makes the loss NaN and
+    is raised at the next synchronisation (device status 8)."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be mean, sum or none, got {reduction!r}")
+    shape = logits.shape[:-1]
+    for name, t in (("teacher_tokens", teacher_tokens), ("teacher_logits", teacher_logits)):
+        if t.dim() != logits.dim() or t.shape[:-1] != shape:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                             f"{(*shape, 'entries')}")
+    if teacher_tokens.shape != teacher_logits.shape:
+        raise ValueError("teacher_tokens and teacher_logits differ in shape: "
+                         f"{tuple(teacher_tokens.shape)} and {tuple(teacher_logits.shape)}")
+    entries = teacher_tokens.shape[-1]
+    if entries == 0:
+        raise ValueError("a teacher's list holds at least one entry")
+    with torch.autocast("cuda", enabled=False):
+        loss = _Distillation.apply(
+            _as_rows(logits), teacher_tokens.reshape(-1, entries),
+            teacher_logits.detach().reshape(-1, entries), float(temperature), int(ignore_index),
+            reduction)
+    return loss.reshape(shape) if reduction == "none" else loss
+
+
+class _Embedding(torch.autograd.Function):
+    """Scaled lookup; saves the tokens alone."""
+
+    @staticmethod
+    def forward(ctx, weight, tokens, scale, padding_idx, dtype):
+        ctx.save_for_backward(tokens)
+        ctx.meta = (weight.shape[0], scale, padding_idx, weight.dtype)
+        return ops.embedding_forward(tokens, weight, scale, dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (tokens,) = ctx.saved_tensors
+        vocab, scale, padding_idx, wdtype = ctx.meta
+        return (ops.embedding_backward(tokens, grad, vocab, scale, padding_idx, wdtype), None,
+                None, None, None)
+
+
+def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0,
+              padding_idx: int | None = None, dtype: torch.dtype | None = None) -> Tensor:
+    """``scale * weight[tokens]``: ``tokens`` [...] (int64 or int32, CUDA),
+    ``weight`` [V, D] (FP32 or BF16) -> [..., D] in ``dtype`` (FP32 or BF16;
+    the table's by default), rounded once.
+
+    The table's gradient is dense, in the table's dtype: FP32 sums over the
+    tokens sorted by id, in order of position, so it is the same every time.
+    Tokens equal to ``padding_idx`` (negative: from the end, as in
+    ``torch.nn.functional.embedding``) take no part in it.  A token outside
+    [0, V) gives a NaN row and is raised at the next synchronisation (device
+    status 8)."""
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
+    if padding_idx is not None:
+        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} lies outside the table of "
+                             f"{weight.shape[0]} rows")
+        padding_idx = int(padding_idx) % weight.shape[0]
+    out = _Embedding.apply(weight, tokens.reshape(-1), float(scale), padding_idx,
+                           dtype or weight.dtype)
+    return out.reshape(*tokens.shape, weight.shape[1])
 
 
 class CoreInputProjection(torch.autograd.Function):

@@ -192,6 +192,9 @@ def b200_status() -> dict[str, object]:
             "local_field_gather": "gather + inverse-index reverse (no atomics)",
             "linear_cross_entropy": "tcgen05 readout GEMM with softmax epilogues (BF16)",
             "cross_entropy_from_logits": "one-pass log-sum-exp and softmax-gradient sweeps",
+            "token_log_probs": "one-pass scores, entropy and top alternatives of each row",
+            "distillation_loss": "one sweep a row against a teacher's top logits",
+            "embedding": "scaled lookup; gradient by sorted tokens (no atomics)",
             "core_input_projections": "tcgen05 GEMM, W(x) and Wg(x) in one launch (BF16)",
             "recurrent_matrix_gradient": "tcgen05 GEMM, grad Ug and grad A in one launch (BF16)",
         },

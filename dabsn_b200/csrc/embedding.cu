@@ -1,0 +1,412 @@
+// Scaled embedding lookup and the gradient of its table.
+//
+//   out[i, :] = scale * weight[token_i, :]            (rounded once, to out's type)
+//   dweight[v, :] = scale * sum over i with token_i = v of dout[i, :]
+//
+// Both are bound by memory: the lookup writes N x D and reads the rows used,
+// the gradient reads N x D and writes the whole table (zeros where no token
+// points).  The gradient's sums run over the tokens sorted by id, positions
+// ascending inside an id, so no atomics are needed and the result does not
+// depend on scheduling: a stable radix sort of (id, position), digits of at
+// most eight bits, then one sum per run of equal ids in FP32, rounded once to
+// the table's type.
+//
+// Tokens outside [0, V) give NaN rows and status 8, and take no part in the
+// gradient; nor do tokens equal to the padding id.
+#include <algorithm>
+
+#include "../../include/dabsn_b200.h"
+#include "common.cuh"
+
+namespace dabsn {
+namespace {
+
+typedef __nv_bfloat16 bf16;
+
+constexpr int EM_THREADS = 256;
+constexpr int EM_STATUS_BAD_TOKEN = 8;
+
+// Eight consecutive elements as FP32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<bf16>(const bf16* p, float (&v)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <>
+__device__ __forceinline__ void store8<bf16>(bf16* p, const float (&v)[8]) {
+  uint4 u;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = u;
+}
+
+// W elements at p: a 16- or 32-byte vector (W = 8) or one element (W = 1).
+template <int W, typename T>
+__device__ __forceinline__ void load_w(const T* p, float (&v)[W]) {
+  if constexpr (W == 8)
+    load8<T>(p, v);
+  else
+    v[0] = to_f<T>(__ldg(p));
+}
+template <int W, typename T>
+__device__ __forceinline__ void store_w(T* p, const float (&v)[W]) {
+  if constexpr (W == 8)
+    store8<T>(p, v);
+  else
+    p[0] = from_f<T>(v[0]);
+}
+
+// ---------------------------------------------------------------------------
+// Lookup: each CTA copies a group of rows, a thread per vector.
+// ---------------------------------------------------------------------------
+template <typename TW, typename TO, int W>
+__global__ void __launch_bounds__(EM_THREADS) embedding_fwd_kernel(
+    long long N, int V, int units, int group, const int64_t* __restrict__ tokens,
+    const TW* __restrict__ weight, long long ldw, float scale, TO* __restrict__ out,
+    int* status) {
+  const long long r0 = (long long)blockIdx.x * group;
+  const int here = (int)min((long long)group, N - r0);
+  for (int e = threadIdx.x; e < here * units; e += EM_THREADS) {
+    const int i = e / units, u = e - i * units;
+    const long long r = r0 + i;
+    const long long t = tokens[r];
+    float v[W];
+    if (t >= 0 && t < V) {
+      load_w<W, TW>(weight + (size_t)t * ldw + (size_t)u * W, v);
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] *= scale;
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] = __int_as_float(0x7fc00000);
+      if (u == 0 && status) atomicExch(status, EM_STATUS_BAD_TOKEN);
+    }
+    store_w<W, TO>(out + ((size_t)r * units + u) * W, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Stable radix sort of (id, position).  A block owns a contiguous tile of the
+// input; one launch counts its digits, the next places its elements after
+// those of smaller digits and of earlier blocks.
+// ---------------------------------------------------------------------------
+constexpr int RS_ITEMS = 16;
+constexpr int RS_UNIT = EM_THREADS * RS_ITEMS;  // elements ranked at a time
+constexpr int RS_MAX_BLOCKS = 256;
+constexpr int RS_DIGITS = 256;
+constexpr int RS_WARPS = EM_THREADS / 32;
+
+struct SortPlan {
+  int blocks, tile, passes, bits;
+};
+
+SortPlan sort_plan(int64_t N, int64_t V) {
+  SortPlan p;
+  const int64_t units = std::max<int64_t>(1, (N + RS_UNIT - 1) / RS_UNIT);
+  const int64_t per = (units + RS_MAX_BLOCKS - 1) / RS_MAX_BLOCKS;
+  p.tile = (int)std::min<int64_t>(per * RS_UNIT, 0x7fffffff / RS_UNIT * RS_UNIT);
+  p.blocks = (int)((units + per - 1) / per);
+  int nbits = 1;
+  while ((int64_t(1) << nbits) <= V) ++nbits;  // ids 0 .. V, V for those left out
+  p.passes = (nbits + 7) / 8;
+  p.bits = (nbits + p.passes - 1) / p.passes;
+  return p;
+}
+
+struct SortSpace {
+  int* key[2];
+  int* pos[2];
+  int* hist;  // [blocks][RS_DIGITS]
+};
+
+SortSpace sort_space(void* ws, int64_t N) {
+  SortSpace s;
+  int* p = (int*)ws;
+  for (int i = 0; i < 2; ++i) {
+    s.key[i] = p;
+    s.pos[i] = p + N;
+    p += 2 * N;
+  }
+  s.hist = p;
+  return s;
+}
+
+// What the first pass sorts by: the id, or V for an element left out.
+__device__ __forceinline__ int sort_key(long long t, int V, long long padding) {
+  return t < 0 || t >= V || t == padding ? V : (int)t;
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(EM_THREADS) sort_count_kernel(
+    int N, int V, long long padding, int tile, int shift, int mask,
+    const int64_t* __restrict__ tokens, const int* __restrict__ key, int* __restrict__ hist) {
+  __shared__ int count[RS_DIGITS];
+  for (int d = threadIdx.x; d < RS_DIGITS; d += EM_THREADS) count[d] = 0;
+  __syncthreads();
+  const long long first = (long long)blockIdx.x * tile;
+  const long long last = min(first + tile, (long long)N);
+  for (long long i = first + threadIdx.x; i < last; i += EM_THREADS) {
+    const int k = FIRST ? sort_key(tokens[i], V, padding) : key[i];
+    atomicAdd(&count[(k >> shift) & mask], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < RS_DIGITS; d += EM_THREADS)
+    hist[blockIdx.x * RS_DIGITS + d] = count[d];
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(EM_THREADS) sort_place_kernel(
+    int N, int V, long long padding, int tile, int shift, int mask,
+    const int64_t* __restrict__ tokens, const int* __restrict__ key, const int* __restrict__ pos,
+    const int* __restrict__ hist, int* __restrict__ key_out, int* __restrict__ pos_out) {
+  static_assert(RS_DIGITS == EM_THREADS, "one digit per thread");
+  __shared__ int next[RS_DIGITS];              // where the digit's next element goes
+  __shared__ int offset[RS_WARPS][RS_DIGITS];  // counts, then places, of each warp
+  __shared__ int warp_total[RS_WARPS];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  {
+    int before = 0, total = 0;
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int n = hist[b * RS_DIGITS + t];
+      if (b < (int)blockIdx.x) before += n;
+      total += n;
+    }
+    int scan = total;  // inclusive over the digits of this warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) warp_total[warp] = scan;
+    __syncthreads();
+    int base = scan - total;
+    for (int w = 0; w < warp; ++w) base += warp_total[w];
+    next[t] = base + before;
+  }
+  const long long first = (long long)blockIdx.x * tile;
+  const long long last = min(first + tile, (long long)N);
+  for (long long unit = first; unit < last; unit += RS_UNIT) {
+    for (int w = 0; w < RS_WARPS; ++w) offset[w][t] = 0;
+    __syncthreads();
+    // a warp ranks 512 consecutive elements, 32 at a time, in order
+    int k[RS_ITEMS], rank[RS_ITEMS];
+#pragma unroll
+    for (int j = 0; j < RS_ITEMS; ++j) {
+      const long long i = unit + warp * (32 * RS_ITEMS) + j * 32 + lane;
+      k[j] = i < last ? (FIRST ? sort_key(tokens[i], V, padding) : key[i]) : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < RS_ITEMS; ++j) {
+      const bool in = k[j] >= 0;
+      const int digit = in ? (k[j] >> shift) & mask : RS_DIGITS;
+      const unsigned peers = __match_any_sync(0xffffffffu, digit);
+      const int seen = in ? offset[warp][digit] : 0;
+      rank[j] = seen + __popc(peers & ((1u << lane) - 1));
+      __syncwarp();
+      if (in && (peers >> lane) == 1u) offset[warp][digit] = seen + __popc(peers);
+      __syncwarp();
+    }
+    __syncthreads();
+    {
+      int at = next[t];
+      for (int w = 0; w < RS_WARPS; ++w) {
+        const int n = offset[w][t];
+        offset[w][t] = at;
+        at += n;
+      }
+      next[t] = at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < RS_ITEMS; ++j) {
+      if (k[j] < 0) continue;
+      const long long i = unit + warp * (32 * RS_ITEMS) + j * 32 + lane;
+      const int dst = offset[warp][(k[j] >> shift) & mask] + rank[j];
+      key_out[dst] = k[j];
+      pos_out[dst] = FIRST ? (int)i : pos[i];
+    }
+    __syncthreads();
+  }
+}
+
+// First sorted element whose key is not below v.
+__device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
+  int lo = 0, hi = N;
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (key[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// One CTA per table row: the sum of its tokens' gradient rows.
+template <typename TG, typename TW, int W>
+__global__ void __launch_bounds__(EM_THREADS) embedding_grad_kernel(
+    int N, int V, int units, const int* __restrict__ key, const int* __restrict__ pos,
+    const TG* __restrict__ dout, float scale, TW* __restrict__ dweight) {
+  __shared__ int edge[2];
+  const int v = blockIdx.x;
+  if (threadIdx.x < 2) edge[threadIdx.x] = lower_bound(key, N, v + (int)threadIdx.x);
+  __syncthreads();
+  const int a = edge[0], b = edge[1];
+  for (int u = threadIdx.x; u < units; u += EM_THREADS) {
+    float sum[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) sum[k] = 0.f;
+    for (int i = a; i < b; ++i) {
+      float g[W];
+      load_w<W, TG>(dout + ((size_t)pos[i] * units + u) * W, g);
+#pragma unroll
+      for (int k = 0; k < W; ++k) sum[k] += g[k];
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) sum[k] *= scale;
+    store_w<W, TW>(dweight + ((size_t)v * units + u) * W, sum);
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_embedding(const char* what, int wdtype, int odtype, int64_t N, int64_t V, int64_t D) {
+  if (N < 0 || N > INT32_MAX || V <= 0 || V >= INT32_MAX || D <= 0 || D > INT32_MAX / 8) {
+    set_error("%s: unsupported sizes N=%lld V=%lld D=%lld", what, (long long)N, (long long)V,
+              (long long)D);
+    return DABSN_ERR_SHAPE;
+  }
+  for (int d : {wdtype, odtype})
+    if (d != DABSN_F32 && d != DABSN_BF16) {
+      set_error("%s: tables and outputs must be FP32 or BF16", what);
+      return DABSN_ERR_DTYPE;
+    }
+  return DABSN_OK;
+}
+
+template <typename TW, typename TO>
+int launch_lookup(int64_t N, int64_t V, int64_t D, const int64_t* tokens, const void* weight,
+                  int64_t ldw, float scale, void* out, cudaStream_t st) {
+  const bool vec = D % 8 == 0 && ldw % 8 == 0 && aligned16(weight) && aligned16(out);
+  const int units = (int)(vec ? D / 8 : D);
+  const int group = std::max(1, 4 * EM_THREADS / units);
+  const unsigned grid = (unsigned)((N + group - 1) / group);
+  if (vec)
+    embedding_fwd_kernel<TW, TO, 8><<<grid, EM_THREADS, 0, st>>>(
+        N, (int)V, units, group, tokens, (const TW*)weight, ldw, scale, (TO*)out,
+        device_status());
+  else
+    embedding_fwd_kernel<TW, TO, 1><<<grid, EM_THREADS, 0, st>>>(
+        N, (int)V, units, group, tokens, (const TW*)weight, ldw, scale, (TO*)out,
+        device_status());
+  return launch_status("embedding_fwd");
+}
+
+template <typename TG, typename TW>
+int launch_grad(int64_t N, int64_t V, int64_t D, const int* key, const int* pos,
+                const void* dout, float scale, void* dweight, cudaStream_t st) {
+  const bool vec = D % 8 == 0 && aligned16(dout) && aligned16(dweight);
+  const int units = (int)(vec ? D / 8 : D);
+  if (vec)
+    embedding_grad_kernel<TG, TW, 8><<<(unsigned)V, EM_THREADS, 0, st>>>(
+        (int)N, (int)V, units, key, pos, (const TG*)dout, scale, (TW*)dweight);
+  else
+    embedding_grad_kernel<TG, TW, 1><<<(unsigned)V, EM_THREADS, 0, st>>>(
+        (int)N, (int)V, units, key, pos, (const TG*)dout, scale, (TW*)dweight);
+  return launch_status("embedding_bwd");
+}
+
+}  // namespace
+}  // namespace dabsn
+
+using namespace dabsn;
+
+extern "C" int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, int64_t V,
+                                   int64_t D, const int64_t* tokens, const void* weight,
+                                   int64_t ldw, float scale, void* out, void* stream) {
+  const int bad = check_embedding("embedding_fwd", weight_dtype, out_dtype, N, V, D);
+  if (bad) return bad;
+  if (ldw < D) {
+    set_error("embedding_fwd: row stride %lld below the width %lld", (long long)ldw,
+              (long long)D);
+    return DABSN_ERR_SHAPE;
+  }
+  if (N == 0) return DABSN_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (weight_dtype == DABSN_BF16)
+    return out_dtype == DABSN_BF16
+               ? launch_lookup<bf16, bf16>(N, V, D, tokens, weight, ldw, scale, out, st)
+               : launch_lookup<bf16, float>(N, V, D, tokens, weight, ldw, scale, out, st);
+  return out_dtype == DABSN_BF16
+             ? launch_lookup<float, bf16>(N, V, D, tokens, weight, ldw, scale, out, st)
+             : launch_lookup<float, float>(N, V, D, tokens, weight, ldw, scale, out, st);
+}
+
+extern "C" size_t dabsn_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D) {
+  if (N < 0 || N > INT32_MAX || V <= 0 || V >= INT32_MAX || D <= 0) return 0;
+  const SortPlan p = sort_plan(N, V);
+  return ((size_t)4 * N + (size_t)p.blocks * RS_DIGITS) * sizeof(int);
+}
+
+extern "C" int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, int64_t V,
+                                   int64_t D, const int64_t* tokens, int64_t padding_idx,
+                                   const void* dout, float scale, void* dweight, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  const int bad = check_embedding("embedding_bwd", weight_dtype, out_dtype, N, V, D);
+  if (bad) return bad;
+  if (workspace_bytes < dabsn_embedding_bwd_workspace(N, V, D)) {
+    set_error("embedding_bwd: workspace of %zu bytes is too small", workspace_bytes);
+    return DABSN_ERR_UNSUPPORTED;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  const SortPlan plan = sort_plan(N, V);
+  const SortSpace s = sort_space(workspace, N);
+  const int mask = (1 << plan.bits) - 1;
+  const int n = (int)N, v = (int)V;
+  for (int pass = 0; pass < plan.passes && N > 0; ++pass) {
+    const int shift = pass * plan.bits, to = pass & 1, from = to ^ 1;
+    if (pass == 0) {
+      sort_count_kernel<true><<<plan.blocks, EM_THREADS, 0, st>>>(
+          n, v, padding_idx, plan.tile, shift, mask, tokens, nullptr, s.hist);
+      sort_place_kernel<true><<<plan.blocks, EM_THREADS, 0, st>>>(
+          n, v, padding_idx, plan.tile, shift, mask, tokens, nullptr, nullptr, s.hist, s.key[to],
+          s.pos[to]);
+    } else {
+      sort_count_kernel<false><<<plan.blocks, EM_THREADS, 0, st>>>(
+          n, v, padding_idx, plan.tile, shift, mask, nullptr, s.key[from], s.hist);
+      sort_place_kernel<false><<<plan.blocks, EM_THREADS, 0, st>>>(
+          n, v, padding_idx, plan.tile, shift, mask, nullptr, s.key[from], s.pos[from], s.hist,
+          s.key[to], s.pos[to]);
+    }
+  }
+  const int* key = s.key[(plan.passes - 1) & 1];
+  const int* pos = s.pos[(plan.passes - 1) & 1];
+  if (out_dtype == DABSN_BF16)
+    return weight_dtype == DABSN_BF16
+               ? launch_grad<bf16, bf16>(N, V, D, key, pos, dout, scale, dweight, st)
+               : launch_grad<bf16, float>(N, V, D, key, pos, dout, scale, dweight, st);
+  return weight_dtype == DABSN_BF16
+             ? launch_grad<float, bf16>(N, V, D, key, pos, dout, scale, dweight, st)
+             : launch_grad<float, float>(N, V, D, key, pos, dout, scale, dweight, st);
+}

@@ -835,6 +835,203 @@ def ce_logits_backward(logits: Tensor, targets: Tensor, ignore_index: int, lse: 
 
 
 # ---------------------------------------------------------------------------
+# Token log-probabilities, distillation, embedding
+# ---------------------------------------------------------------------------
+TOP_K_MAX = 128
+TEACHER_ENTRIES_MAX = 256
+
+
+def _logit_rows(logits: Tensor) -> tuple[int, int, int]:
+    """(rows, V, row stride) of a matrix of logits with contiguous rows."""
+    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError("dabsn_b200: logits must be [rows, V] with contiguous rows")
+    rows, V = logits.shape
+    if V < 1:
+        raise ValueError("dabsn_b200: logits need at least one vocabulary entry")
+    # torch leaves the stride of a single row arbitrary
+    return rows, V, (logits.stride(0) if rows > 1 else V)
+
+
+def _temperature(temperature: float) -> float:
+    t = float(temperature)
+    if not (0.0 < t < float("inf")) or not ctypes.c_float(1.0 / t).value < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    return t
+
+
+def _int_rows(t: Tensor, shape, what: str) -> Tensor:
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what} must hold int64 or int32 ids, got {t.dtype}")
+    return t.detach().to(torch.int64).contiguous()
+
+
+def token_scores_forward(logits: Tensor, tokens: Tensor, top_k: int, temperature: float,
+                         ignore_index: int, with_stats: bool = True):
+    """logits [rows, V] (FP32/BF16, rows contiguous), tokens [rows].  Returns
+    (log_prob [rows], entropy [rows], top values [rows, k], top ids [rows, k],
+    statistics [rows, 2] or None), FP32 and int64."""
+    dev = _require_cuda(logits, tokens)
+    rows, V, ld = _logit_rows(logits)
+    code, temperature = act_code(logits.dtype), _temperature(temperature)
+    tokens = _int_rows(tokens, (rows,), "tokens")
+    k = int(top_k)
+    if not 0 <= k <= min(TOP_K_MAX, V):
+        raise ValueError(f"top_k must lie in [0, {min(TOP_K_MAX, V)}], got {top_k}")
+    f32 = dict(device=dev, dtype=torch.float32)
+    log_prob, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
+    stats = torch.empty((rows, 2), **f32) if with_stats else None
+    top_values = torch.empty((rows, k), **f32)
+    top_ids = torch.empty((rows, k), device=dev, dtype=torch.int64)
+    lib = N.load()
+    with torch.cuda.device(dev), _timed("token_scores_fwd", dev):
+        st = lib.dabsn_token_scores_fwd(
+            code, rows, V, ld, _ptr(logits), _ptr(tokens), int(ignore_index), temperature, k,
+            _ptr(log_prob), _ptr(entropy), _ptr(stats), _ptr(top_values), _ptr(top_ids),
+            _stream(dev))
+    N.check(st, "token_scores_fwd")
+    return log_prob, entropy, top_values, top_ids, stats
+
+
+def token_scores_backward(logits: Tensor, tokens: Tensor, temperature: float, ignore_index: int,
+                          stats: Tensor, entropy: Tensor, grad_log_prob: Tensor | None,
+                          grad_entropy: Tensor | None) -> Tensor:
+    """dlogits [rows, V] in the logits' dtype from the gradients of the
+    log-probabilities and of the entropies (either may be None)."""
+    dev = _require_cuda(logits, tokens, stats, entropy, grad_log_prob, grad_entropy)
+    rows, V, ld = _logit_rows(logits)
+    tokens = _int_rows(tokens, (rows,), "tokens")
+    g, h = _grad_or_none(grad_log_prob), _grad_or_none(grad_entropy)
+    dl = torch.empty((rows, V), device=dev, dtype=logits.dtype)
+    lib = N.load()
+    with torch.cuda.device(dev), _timed("token_scores_bwd", dev):
+        st = lib.dabsn_token_scores_bwd(
+            act_code(logits.dtype), rows, V, ld, _ptr(logits), _ptr(tokens), int(ignore_index),
+            _temperature(temperature), _ptr(stats), _ptr(entropy), _ptr(g), _ptr(h), _ptr(dl),
+            _stream(dev))
+    N.check(st, "token_scores_bwd")
+    return dl
+
+
+def distill_prep(teacher_tokens: Tensor, teacher_logits: Tensor, vocab: int, temperature: float,
+                 ignore_index: int) -> Tensor:
+    """The teacher's lists [rows, K] as probabilities, in the buffer that the
+    distillation kernels read: ids, probabilities, equal ids merged, which rows
+    have a loss, and how many."""
+    dev = _require_cuda(teacher_tokens, teacher_logits)
+    if teacher_tokens.dim() != 2:
+        raise ValueError("teacher_tokens must be [rows, entries]")
+    rows, K = teacher_tokens.shape
+    if not 1 <= K <= TEACHER_ENTRIES_MAX:
+        raise ValueError(f"a teacher's list holds 1 to {TEACHER_ENTRIES_MAX} entries, got {K}")
+    ids = _int_rows(teacher_tokens, (rows, K), "teacher_tokens")
+    if tuple(teacher_logits.shape) != (rows, K):
+        raise ValueError(f"teacher_logits has shape {tuple(teacher_logits.shape)}, expected "
+                         f"{(rows, K)}")
+    tl = teacher_logits.detach().contiguous()
+    code, temperature = act_code(tl.dtype), _temperature(temperature)
+    lib = N.load()
+    lists = torch.empty(int(lib.dabsn_distill_list_bytes(rows, K)), device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev), _timed("distill_prep", dev):
+        st = lib.dabsn_distill_prep(code, rows, vocab, K, _ptr(ids), _ptr(tl), temperature,
+                                    int(ignore_index), _ptr(lists), _stream(dev))
+    N.check(st, "distill_prep")
+    return lists
+
+
+def distill_forward(logits: Tensor, lists: Tensor, entries: int, temperature: float):
+    """(row losses [rows] FP32, statistics [rows, 2]) of the student's logits
+    [rows, V] against prepared lists."""
+    dev = _require_cuda(logits, lists)
+    rows, V, ld = _logit_rows(logits)
+    loss = torch.empty(rows, device=dev, dtype=torch.float32)
+    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    lib = N.load()
+    with torch.cuda.device(dev), _timed("distill_fwd", dev):
+        st = lib.dabsn_distill_fwd(act_code(logits.dtype), rows, V, ld, _ptr(logits), entries,
+                                   _ptr(lists), _temperature(temperature), _ptr(loss),
+                                   _ptr(stats), _stream(dev))
+    N.check(st, "distill_fwd")
+    return loss, stats
+
+
+def distill_reduce(row_loss: Tensor, lists: Tensor, entries: int, mean: bool) -> Tensor:
+    """Sum of the row losses, or their mean over the rows that have one; FP32 []."""
+    dev = _require_cuda(row_loss, lists)
+    out = torch.empty((), device=dev, dtype=torch.float32)
+    lib = N.load()
+    with torch.cuda.device(dev), _timed("distill_reduce", dev):
+        st = lib.dabsn_distill_reduce(row_loss.shape[0], entries, _ptr(row_loss), _ptr(lists),
+                                      int(mean), _ptr(out), _stream(dev))
+    N.check(st, "distill_reduce")
+    return out
+
+
+def distill_backward(logits: Tensor, lists: Tensor, entries: int, temperature: float,
+                     stats: Tensor, mean: bool, weight: Tensor) -> Tensor:
+    """dlogits [rows, V] for row weights ``weight`` ([rows], or [] for all
+    rows), divided by the number of rows with a loss if ``mean``."""
+    dev = _require_cuda(logits, lists, stats, weight)
+    rows, V, ld = _logit_rows(logits)
+    w = weight.detach().to(torch.float32).contiguous()
+    dl = torch.empty((rows, V), device=dev, dtype=logits.dtype)
+    lib = N.load()
+    with torch.cuda.device(dev), _timed("distill_bwd", dev):
+        st = lib.dabsn_distill_bwd(act_code(logits.dtype), rows, V, ld, _ptr(logits), entries,
+                                   _ptr(lists), _temperature(temperature), _ptr(stats),
+                                   int(mean), _ptr(w), int(w.dim() > 0), _ptr(dl), _stream(dev))
+    N.check(st, "distill_bwd")
+    return dl
+
+
+def embedding_forward(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
+    """scale * weight[tokens] in ``dtype``: tokens [N], weight [V, D] -> [N, D]."""
+    dev = _require_cuda(weight, tokens)
+    if weight.dim() != 2:
+        raise ValueError("the embedding table must be [V, D]")
+    V, D = weight.shape
+    if V < 1 or D < 1:
+        raise ValueError(f"an embedding table of shape {tuple(weight.shape)} is empty")
+    if tokens.dim() != 1:
+        raise ValueError("tokens must be [N]")
+    n = tokens.shape[0]
+    ids = _int_rows(tokens, (n,), "tokens")
+    w = weight.detach()
+    if w.stride(1) != 1 or w.stride(0) < D:
+        w = w.contiguous()
+    ldw = w.stride(0) if V > 1 else D
+    out = torch.empty((n, D), device=dev, dtype=dtype)
+    lib = N.load()
+    with torch.cuda.device(dev), _timed("embedding_fwd", dev):
+        st = lib.dabsn_embedding_fwd(act_code(w.dtype), act_code(dtype), n, V, D, _ptr(ids),
+                                     _ptr(w), ldw, float(scale), _ptr(out), _stream(dev))
+    N.check(st, "embedding_fwd")
+    return out
+
+
+def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: float,
+                       padding_idx: int | None, dtype: torch.dtype) -> Tensor:
+    """The table's gradient [vocab, D] in ``dtype`` from grad_out [N, D]: sums
+    over equal tokens in FP32, in order of position (no atomics)."""
+    dev = _require_cuda(grad_out, tokens)
+    n, D = grad_out.shape
+    ids = _int_rows(tokens, (n,), "tokens")
+    g = grad_out.detach().contiguous()
+    dw = torch.empty((vocab, D), device=dev, dtype=dtype)
+    lib = N.load()
+    ws = torch.empty(int(lib.dabsn_embedding_bwd_workspace(n, vocab, D)), device=dev,
+                     dtype=torch.uint8)
+    with torch.cuda.device(dev), _timed("embedding_bwd", dev):
+        st = lib.dabsn_embedding_bwd(
+            act_code(g.dtype), act_code(dtype), n, vocab, D, _ptr(ids),
+            -1 if padding_idx is None else int(padding_idx), _ptr(g), float(scale), _ptr(dw),
+            _ptr(ws), ws.numel(), _stream(dev))
+    N.check(st, "embedding_bwd")
+    return dw
+
+
+# ---------------------------------------------------------------------------
 # Dense products around the scan on the tcgen05 GEMM (BF16)
 # ---------------------------------------------------------------------------
 def input_proj_forward(x: Tensor, W: Tensor, Wg: Tensor, bias_g: Tensor | None):

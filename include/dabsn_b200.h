@@ -484,6 +484,66 @@ int dabsn_read_wide_bwd(int64_t B, int64_t T, int64_t N, int64_t H, int mode,
                         void* dnext, float* dbias, float* dbank_cocktail, float* rowpart,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* Log-probabilities of given tokens, with entropy and top alternatives.
+ *   logits [rows, V] FP32/BF16, rows contiguous and `ld` elements apart, any
+ *   alignment; tokens [rows] int64 (rows of ignore_index are not read);
+ *   temperature > 0; 0 <= top_k <= min(128, V).
+ *   log_prob, entropy [rows] FP32; stats FP32 [rows, 2] (maximum, sum of
+ *   exponentials; for the reverse, may be null); top_values FP32 and top_ids
+ *   int64 [rows, top_k], most likely first, equal logits by the lower id.
+ * Reverse: dlogits [rows, V] contiguous, in the logits' dtype, for gradients
+ * of log_prob and entropy (FP32 [rows], either may be null).
+ * A token outside [0, V) gives NaN and device status 8. */
+int dabsn_token_scores_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
+                           const int64_t* tokens, int64_t ignore_index, float temperature,
+                           int64_t top_k, float* log_prob, float* entropy, float* stats,
+                           float* top_values, int64_t* top_ids, void* stream);
+int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
+                           const int64_t* tokens, int64_t ignore_index, float temperature,
+                           const float* stats, const float* entropy, const float* g_log_prob,
+                           const float* g_entropy, void* dlogits, void* stream);
+
+/* Distillation from a teacher's top logits: temperature^2 KL(q || softmax(
+ * logits / temperature)), q the softmax of the teacher's logits over the
+ * entries that a row lists (1 <= K <= 256; entries of ignore_index are absent).
+ *   prep: teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K] ->
+ *   `list`, dabsn_distill_list_bytes(rows, K) bytes, 8-byte aligned, which the
+ *   other three read; an id outside [0, V) gives a NaN loss and status 8.
+ *   fwd: row_loss [rows], stats [rows, 2] FP32 (stats for the reverse, may be
+ *   null).  reduce: result FP32 [1], the sum of the row losses, divided by the
+ *   number of rows that list anything if `mean`.
+ *   bwd: dlogits [rows, V] contiguous, in the logits' dtype, for row weights
+ *   weight[r * weight_stride], divided by the same number if `mean`. */
+size_t dabsn_distill_list_bytes(int64_t rows, int64_t K);
+int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
+                       const int64_t* teacher_tokens, const void* teacher_logits,
+                       float temperature, int64_t ignore_index, void* list, void* stream);
+int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
+                      int64_t K, const void* list, float temperature, float* row_loss,
+                      float* stats, void* stream);
+int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
+                      int64_t K, const void* list, float temperature, const float* stats,
+                      int mean, const float* weight, int64_t weight_stride, void* dlogits,
+                      void* stream);
+int dabsn_distill_reduce(int64_t rows, int64_t K, const float* row_loss, const void* list,
+                         int mean, float* result, void* stream);
+
+/* Scaled embedding lookup: out [N, D] = scale * weight[tokens], weight [V, D]
+ * with rows `ldw` elements apart; tables and outputs FP32 or BF16.  A token
+ * outside [0, V) gives a NaN row and device status 8.
+ * Reverse: dweight [V, D] contiguous = scale * sums of dout [N, D] over equal
+ * tokens, in order of position (FP32, no atomics); tokens outside [0, V) and
+ * tokens equal to padding_idx (-1: none) take no part.  `workspace` holds at
+ * least dabsn_embedding_bwd_workspace bytes, 16-byte aligned. */
+int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, int64_t V, int64_t D,
+                        const int64_t* tokens, const void* weight, int64_t ldw, float scale,
+                        void* out, void* stream);
+size_t dabsn_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D);
+int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, int64_t V, int64_t D,
+                        const int64_t* tokens, int64_t padding_idx, const void* dout,
+                        float scale, void* dweight, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,100 @@
+"""What the vocabulary operators refuse, before anything is launched."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import dabsn_b200
+from dabsn_b200 import _native, ops
+
+
+def _logits(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_shapes_are_checked():
+    x = _logits(4, 10)
+    with pytest.raises(ValueError, match="tokens"):
+        dabsn_b200.token_log_probs(x, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="teacher_tokens"):
+        dabsn_b200.distillation_loss(x, torch.zeros(3, 2, dtype=torch.int64), torch.zeros(4, 2))
+    with pytest.raises(ValueError, match="teacher_logits"):
+        dabsn_b200.distillation_loss(x, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4))
+    with pytest.raises(ValueError, match="differ"):
+        dabsn_b200.distillation_loss(x, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 3))
+    with pytest.raises(ValueError, match="at least one entry"):
+        dabsn_b200.distillation_loss(x, torch.zeros(4, 0, dtype=torch.int64), torch.zeros(4, 0))
+    with pytest.raises(ValueError, match="reduction"):
+        dabsn_b200.distillation_loss(x, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2),
+                                     reduction="median")
+    with pytest.raises(ValueError, match="vocabulary"):
+        dabsn_b200.token_log_probs(_logits(4, 0), torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="weight"):
+        dabsn_b200.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5))
+    with pytest.raises(ValueError, match="padding_idx"):
+        dabsn_b200.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4), padding_idx=5)
+
+
+def test_cpu_tensors_are_refused():
+    ids = torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(TypeError, match="CUDA"):
+        dabsn_b200.token_log_probs(_logits(4, 10), ids)
+    with pytest.raises(TypeError, match="CUDA"):
+        dabsn_b200.distillation_loss(_logits(4, 10), ids[:, None], torch.zeros(4, 1))
+    with pytest.raises(TypeError, match="CUDA"):
+        dabsn_b200.embedding(ids, torch.zeros(5, 4))
+
+
+@pytest.mark.parametrize("t", [0.0, -1.0, float("inf"), float("nan"), 1e-45])
+def test_temperatures(t):
+    with pytest.raises(ValueError, match="temperature"):
+        ops._temperature(t)
+
+
+def test_ids_must_be_integers():
+    with pytest.raises(TypeError, match="int64 or int32"):
+        ops._int_rows(torch.zeros(4), (4,), "tokens")
+    assert ops._int_rows(torch.zeros(4, dtype=torch.int32), (4,), "t").dtype == torch.int64
+
+
+NULL = ctypes.c_void_p(0)
+
+
+def test_entry_points_check_sizes_before_launching():
+    """The C entry points refuse what their kernels do not cover; nothing is
+    launched, so null pointers are never read."""
+    lib = _native.load()
+    f = ctypes.c_float
+
+    def scores(dtype=0, rows=4, V=10, ld=10, t=1.0, k=0):
+        return lib.dabsn_token_scores_fwd(dtype, rows, V, ld, NULL, NULL, -100, f(t), k,
+                                          *([NULL] * 6))
+
+    assert scores(rows=0) == 0
+    assert scores(rows=-1) and scores(V=0) and scores(ld=9) and scores(V=2 ** 31 - 1, ld=2 ** 31)
+    assert scores(dtype=2) and scores(t=0.0) and scores(t=float("nan"))
+    assert scores(k=11) and scores(V=1000, ld=1000, k=129) and scores(k=-1)
+
+    def distill(dtype=0, rows=4, V=10, ld=10, K=2, t=1.0):
+        return lib.dabsn_distill_fwd(dtype, rows, V, ld, NULL, K, NULL, f(t), *([NULL] * 3))
+
+    assert distill(rows=0) == 0
+    assert distill(K=0) and distill(K=257) and distill(dtype=7) and distill(t=float("inf"))
+    assert lib.dabsn_distill_prep(0, 4, 0, 2, NULL, NULL, f(1.0), -100, NULL, NULL)
+    assert lib.dabsn_distill_reduce(-1, 2, NULL, NULL, 1, NULL, NULL)
+    assert lib.dabsn_distill_bwd(0, 4, 10, 9, NULL, 2, NULL, f(1.0), NULL, 1, NULL, 0, NULL, NULL)
+
+    def lookup(w=0, o=0, N=4, V=10, D=8, ldw=8):
+        return lib.dabsn_embedding_fwd(w, o, N, V, D, NULL, NULL, ldw, f(1.0), NULL, NULL)
+
+    assert lookup(N=0) == 0
+    assert lookup(w=3) and lookup(o=3) and lookup(D=0) and lookup(V=0) and lookup(ldw=7)
+    assert lookup(N=2 ** 31)
+    need = lib.dabsn_embedding_bwd_workspace(1000, 50, 8)
+    assert need > 0 and lib.dabsn_embedding_bwd_workspace(-1, 50, 8) == 0
+    assert lib.dabsn_embedding_bwd(0, 0, 1000, 50, 8, NULL, -1, NULL, f(1.0), NULL, NULL,
+                                   need - 1, NULL)
+    assert b"workspace" in lib.dabsn_last_error()
