@@ -630,20 +630,27 @@ class TokenLogProbs(NamedTuple):
     top_tokens: Tensor
 
 
+def _differentiates(t: Tensor) -> bool:
+    """Whether a call has to record its reverse; without one the operators
+    below run their forward directly (a node costs a single token's call more
+    than its kernel)."""
+    return t.requires_grad and torch.is_grad_enabled()
+
+
 class _TokenScores(torch.autograd.Function):
     """Log-probability and entropy of every row, differentiable in the logits;
     saves the logits and two numbers a row."""
 
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
-        flat = logits.detach()
         log_prob, entropy, top_values, top_ids, stats = ops.token_scores_forward(
-            flat, tokens, top_k, temperature, ignore_index, ctx.needs_input_grad[0])
-        ctx.mark_non_differentiable(top_values, top_ids)
+            logits, tokens, top_k, temperature, ignore_index)
         ctx.set_materialize_grads(False)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, tokens, stats, entropy)
+        ctx.save_for_backward(logits, tokens, stats, entropy)
         ctx.meta = (temperature, ignore_index)
+        if not top_k:
+            return log_prob, entropy
+        ctx.mark_non_differentiable(top_values, top_ids)
         return log_prob, entropy, top_values, top_ids
 
     @staticmethod
@@ -652,9 +659,8 @@ class _TokenScores(torch.autograd.Function):
         if g_log_prob is None and g_entropy is None:
             return None, None, None, None, None
         logits, tokens, stats, entropy = ctx.saved_tensors
-        temperature, ignore_index = ctx.meta
-        dl = ops.token_scores_backward(logits.detach(), tokens, temperature, ignore_index, stats,
-                                       entropy, g_log_prob, g_entropy)
+        dl = ops.token_scores_backward(logits, tokens, *ctx.meta, stats, entropy, g_log_prob,
+                                       g_entropy)
         return dl, None, None, None, None
 
 
@@ -663,11 +669,12 @@ def _as_rows(logits: Tensor) -> Tensor:
     allow one."""
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError("logits must have a vocabulary axis with at least one entry")
-    flat = logits.reshape(-1, logits.shape[-1])
-    rows_apart = flat.shape[0] <= 1 or flat.stride(0) >= flat.shape[1]
-    if (flat.stride(1) != 1 and flat.shape[1] > 1) or not rows_apart:
-        flat = flat.contiguous()
-    return flat
+    if logits.dim() != 2:
+        logits = logits.reshape(-1, logits.shape[-1])
+    rows, vocab = logits.shape
+    if (logits.stride(1) != 1 and vocab > 1) or (rows > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    return logits
 
 
 def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperature: float = 1.0,
@@ -691,12 +698,24 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens has shape {tuple(tokens.shape)}, expected "
                          f"{tuple(logits.shape[:-1])}")
-    shape = tokens.shape
-    with torch.autocast("cuda", enabled=False):
-        out = _TokenScores.apply(_as_rows(logits), tokens.reshape(-1), int(top_k),
-                                 float(temperature), int(ignore_index))
-    return TokenLogProbs(out[0].reshape(shape), out[1].reshape(shape),
-                         out[2].reshape(*shape, top_k), out[3].reshape(*shape, top_k))
+    shape, top_k = tokens.shape, int(top_k)
+    rows = _as_rows(logits)
+    flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
+    if _differentiates(rows):
+        out = _TokenScores.apply(rows, flat, top_k, temperature, int(ignore_index))
+    else:
+        out = ops.token_scores_forward(rows, flat, top_k, temperature, int(ignore_index), False)
+    log_prob, entropy = out[:2]
+    if top_k:
+        top_values, top_ids = out[2:4]
+    else:
+        top_values = log_prob.new_empty((flat.shape[0], 0))
+        top_ids = flat.new_empty((flat.shape[0], 0), dtype=torch.int64)
+    if tokens.dim() != 1:
+        log_prob, entropy = log_prob.reshape(shape), entropy.reshape(shape)
+        top_values = top_values.reshape(*shape, top_k)
+        top_ids = top_ids.reshape(*shape, top_k)
+    return TokenLogProbs(log_prob, entropy, top_values, top_ids)
 
 
 class _Distillation(torch.autograd.Function):
@@ -705,25 +724,30 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, ignore_index,
                 reduction):
-        entries = teacher_tokens.shape[1]
-        lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
-                                 ignore_index)
-        loss, stats = ops.distill_forward(logits.detach(), lists, entries, temperature)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, lists, stats)
-        ctx.meta = (entries, temperature, reduction)
-        if reduction == "none":
-            return loss
-        return ops.distill_reduce(loss, lists, entries, reduction == "mean")
+        loss, lists, row_stats = _distill(logits, teacher_tokens, teacher_logits, temperature,
+                                          ignore_index, reduction)
+        ctx.save_for_backward(logits, lists, row_stats)
+        ctx.meta = (teacher_tokens.shape[1], temperature, reduction)
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         logits, lists, stats = ctx.saved_tensors
         entries, temperature, reduction = ctx.meta
-        dl = ops.distill_backward(logits.detach(), lists, entries, temperature, stats,
+        dl = ops.distill_backward(logits, lists, entries, temperature, stats,
                                   reduction == "mean", grad)
         return dl, None, None, None, None, None
+
+
+def _distill(logits, teacher_tokens, teacher_logits, temperature, ignore_index, reduction):
+    entries = teacher_tokens.shape[1]
+    lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
+                             ignore_index)
+    loss, stats = ops.distill_forward(logits, lists, entries, temperature)
+    if reduction != "none":
+        loss = ops.distill_reduce(loss, lists, entries, reduction == "mean")
+    return loss, lists, stats
 
 
 def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor, *,
@@ -758,12 +782,14 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     entries = teacher_tokens.shape[-1]
     if entries == 0:
         raise ValueError("a teacher's list holds at least one entry")
-    with torch.autocast("cuda", enabled=False):
-        loss = _Distillation.apply(
-            _as_rows(logits), teacher_tokens.reshape(-1, entries),
-            teacher_logits.detach().reshape(-1, entries), float(temperature), int(ignore_index),
+    rows = _as_rows(logits)
+    if teacher_tokens.dim() != 2:
+        teacher_tokens = teacher_tokens.reshape(-1, entries)
+        teacher_logits = teacher_logits.reshape(-1, entries)
+    args = (rows, teacher_tokens, teacher_logits.detach(), temperature, int(ignore_index),
             reduction)
-    return loss.reshape(shape) if reduction == "none" else loss
+    loss = _Distillation.apply(*args) if _differentiates(rows) else _distill(*args)[0]
+    return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
 class _Embedding(torch.autograd.Function):
@@ -803,9 +829,9 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0,
             raise ValueError(f"padding_idx {padding_idx} lies outside the table of "
                              f"{weight.shape[0]} rows")
         padding_idx = int(padding_idx) % weight.shape[0]
-    out = _Embedding.apply(weight, tokens.reshape(-1), float(scale), padding_idx,
-                           dtype or weight.dtype)
-    return out.reshape(*tokens.shape, weight.shape[1])
+    args = (weight, tokens, float(scale), padding_idx, dtype or weight.dtype)
+    return (_Embedding.apply(*args) if _differentiates(weight) else
+            ops.embedding_forward(tokens, weight, args[2], args[4]))
 
 
 class CoreInputProjection(torch.autograd.Function):

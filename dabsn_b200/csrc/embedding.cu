@@ -263,29 +263,165 @@ __device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
   return lo;
 }
 
-// One CTA per table row: the sum of its tokens' gradient rows.
+// ---------------------------------------------------------------------------
+// Sums over runs of equal ids.  Token frequencies are skewed (the first of
+// 32000 Zipf tokens has a tenth of all positions), so the work is cut along
+// the sorted positions, not along the ids: a group of threads sums a chunk of
+// them, one 8-element unit of the columns a thread, and stores every run that
+// lies inside the chunk.  A run that crosses a boundary leaves an FP32 partial
+// sum in each chunk it touches (slot 1 where it begins, slot 0 where it goes
+// on), which the join adds up in order.
+// ---------------------------------------------------------------------------
+struct GradPlan {
+  int chunk, chunks;   // sorted positions in a chunk, number of chunks
+  int units;           // of the columns
+  int wide, tiles;     // units that a group covers, column tiles
+  int groups;          // chunks that a CTA works on side by side
+  int blocks;          // CTAs for the chunks (x tiles), before those for absent rows
+  int zero_blocks;
+};
+
+constexpr int GR_CHUNK_MAX = 128;
+constexpr int GR_ZERO_ROWS = 32;
+constexpr int GR_JOIN_UNITS = 64;
+
+GradPlan grad_plan(int64_t N, int64_t V, int units) {
+  GradPlan g;
+  g.units = units;
+  g.tiles = (units + EM_THREADS - 1) / EM_THREADS;
+  g.wide = (units + g.tiles - 1) / g.tiles;
+  g.groups = std::min(EM_THREADS / g.wide, 32);
+  g.chunk = N >= 32768 ? GR_CHUNK_MAX : 32;
+  g.chunks = (int)((N + g.chunk - 1) / g.chunk);
+  g.blocks = (g.chunks + g.groups - 1) / g.groups;
+  g.zero_blocks = (int)((V + GR_ZERO_ROWS - 1) / GR_ZERO_ROWS);
+  return g;
+}
+
 template <typename TG, typename TW, int W>
 __global__ void __launch_bounds__(EM_THREADS) embedding_grad_kernel(
-    int N, int V, int units, const int* __restrict__ key, const int* __restrict__ pos,
-    const TG* __restrict__ dout, float scale, TW* __restrict__ dweight) {
-  __shared__ int edge[2];
-  const int v = blockIdx.x;
-  if (threadIdx.x < 2) edge[threadIdx.x] = lower_bound(key, N, v + (int)threadIdx.x);
-  __syncthreads();
-  const int a = edge[0], b = edge[1];
-  for (int u = threadIdx.x; u < units; u += EM_THREADS) {
-    float sum[W];
+    int N, int V, GradPlan g, const int* __restrict__ key, const int* __restrict__ pos,
+    const TG* __restrict__ dout, float scale, TW* __restrict__ dweight,
+    float* __restrict__ partial) {
+  constexpr int AHEAD = 8;  // gradient rows in flight
+  const int t = threadIdx.x;
+  if ((int)blockIdx.x >= g.blocks) {
+    // rows that no token points at
+    __shared__ bool absent[GR_ZERO_ROWS];
+    const int v0 = ((int)blockIdx.x - g.blocks) * GR_ZERO_ROWS;
+    if (t < GR_ZERO_ROWS) {
+      const int v = v0 + t;
+      const int at = v < V ? lower_bound(key, N, v) : 0;
+      absent[t] = v < V && (at >= N || key[at] != v);
+    }
+    __syncthreads();
+    const float zero[W] = {};
+    const int u0 = blockIdx.y * g.wide, u1 = min(u0 + g.wide, g.units);
+    for (int r = 0; r < GR_ZERO_ROWS; ++r) {
+      if (!absent[r]) continue;
+      for (int u = u0 + t; u < u1; u += EM_THREADS)
+        store_w<W, TW>(dweight + ((size_t)(v0 + r) * g.units + u) * W, zero);
+    }
+    return;
+  }
+  const int group = t / g.wide;
+  const int chunk = blockIdx.x * g.groups + group;
+  const int u = blockIdx.y * g.wide + t % g.wide;
+  if (group >= g.groups || chunk >= g.chunks || u >= g.units) return;
+  const int i0 = chunk * g.chunk, i1 = min(i0 + g.chunk, N);
+  const int before = i0 > 0 ? key[i0 - 1] : -1;
+  const int after = i1 < N ? key[i1] : -1;
+  int cur = key[i0];
+  bool first = true;
+  float sum[W];
 #pragma unroll
-    for (int k = 0; k < W; ++k) sum[k] = 0.f;
-    for (int i = a; i < b; ++i) {
-      float g[W];
-      load_w<W, TG>(dout + ((size_t)pos[i] * units + u) * W, g);
+  for (int k = 0; k < W; ++k) sum[k] = 0.f;
+  auto flush = [&](bool last) {
+    if (cur >= V) return;
+    const bool began = first && cur == before;
+    const bool goes_on = last && cur == after;
+    if (!began && !goes_on) {
+      float out[W];
 #pragma unroll
-      for (int k = 0; k < W; ++k) sum[k] += g[k];
+      for (int k = 0; k < W; ++k) out[k] = sum[k] * scale;
+      store_w<W, TW>(dweight + ((size_t)cur * g.units + u) * W, out);
+    } else {
+      store_w<W, float>(partial + (((size_t)chunk * 2 + (began ? 0 : 1)) * g.units + u) * W, sum);
+    }
+  };
+  for (int i = i0; i < i1 && cur < V; i += AHEAD) {
+    float v[AHEAD][W];
+    int k[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      k[a] = i + a < i1 ? key[i + a] : -1;
+      if (k[a] >= 0 && k[a] < V)
+        load_w<W, TG>(dout + ((size_t)pos[i + a] * g.units + u) * W, v[a]);
     }
 #pragma unroll
-    for (int k = 0; k < W; ++k) sum[k] *= scale;
-    store_w<W, TW>(dweight + ((size_t)v * units + u) * W, sum);
+    for (int a = 0; a < AHEAD; ++a) {
+      if (k[a] < 0) break;
+      if (k[a] != cur) {
+        flush(false);
+        first = false;
+        cur = k[a];
+#pragma unroll
+        for (int j = 0; j < W; ++j) sum[j] = 0.f;
+      }
+      if (cur < V) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) sum[j] += v[a][j];
+      }
+    }
+  }
+  flush(true);
+}
+
+// One CTA per chunk and tile of GR_JOIN_UNITS units: where a run begins in the
+// chunk and goes on, adds up its partial sums.  Four threads share a unit, each
+// every fourth partial.
+template <typename TW, int W>
+__global__ void __launch_bounds__(EM_THREADS) embedding_join_kernel(
+    int N, int V, GradPlan g, const int* __restrict__ key, const float* __restrict__ partial,
+    float scale, TW* __restrict__ dweight) {
+  constexpr int SLICES = EM_THREADS / GR_JOIN_UNITS;
+  __shared__ float sh[SLICES][GR_JOIN_UNITS * W];
+  const int chunk = blockIdx.x;
+  const int i0 = chunk * g.chunk, i1 = min(i0 + g.chunk, N);
+  if (i1 >= N) return;
+  const int id = key[i1 - 1];
+  if (id >= V || key[i1] != id) return;               // nothing goes on
+  if (key[i0] == id && i0 > 0 && key[i0 - 1] == id) return;  // begun earlier
+  // chunks it goes on into: mostly the next one alone
+  int n = 1;
+  if (i1 + g.chunk <= N && key[i1 + g.chunk - 1] == id)
+    n = (lower_bound(key, N, id + 1) - 1) / g.chunk - chunk;
+  const int lane = threadIdx.x % GR_JOIN_UNITS, slice = threadIdx.x / GR_JOIN_UNITS;
+  const int u = blockIdx.y * GR_JOIN_UNITS + lane;
+  const bool in = u < g.units;
+  float sum[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) sum[k] = 0.f;
+  if (in) {
+#pragma unroll 4
+    for (int j = slice; j <= n; j += SLICES) {
+      float v[W];
+      load_w<W, float>(
+          partial + (((size_t)(chunk + j) * 2 + (j == 0 ? 1 : 0)) * g.units + u) * W, v);
+#pragma unroll
+      for (int k = 0; k < W; ++k) sum[k] += v[k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) sh[slice][k * GR_JOIN_UNITS + lane] = sum[k];
+  __syncthreads();
+  if (slice == 0 && in) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      for (int o = 1; o < SLICES; ++o) sum[k] += sh[o][k * GR_JOIN_UNITS + lane];
+      sum[k] *= scale;
+    }
+    store_w<W, TW>(dweight + ((size_t)id * g.units + u) * W, sum);
   }
 }
 
@@ -323,18 +459,39 @@ int launch_lookup(int64_t N, int64_t V, int64_t D, const int64_t* tokens, const 
   return launch_status("embedding_fwd");
 }
 
+// Bytes of the sort's arrays, rounded up so that the partial sums behind them
+// are aligned; of the partial sums.
+size_t sort_bytes(int64_t N, int64_t V) {
+  const size_t n = ((size_t)4 * N + (size_t)sort_plan(N, V).blocks * RS_DIGITS) * sizeof(int);
+  return (n + 15) / 16 * 16;
+}
+size_t partial_bytes(int64_t N, int64_t D) {
+  const size_t chunks = (size_t)grad_plan(N, 1, 1).chunks;
+  return chunks * 2 * (size_t)D * sizeof(float);
+}
+
+template <typename TG, typename TW, int W>
+int launch_grad_w(int64_t N, int64_t V, int units, const int* key, const int* pos,
+                  const void* dout, float scale, void* dweight, float* partial,
+                  cudaStream_t st) {
+  const GradPlan g = grad_plan(N, V, units);
+  embedding_grad_kernel<TG, TW, W><<<dim3(g.blocks + g.zero_blocks, g.tiles), EM_THREADS, 0, st>>>(
+      (int)N, (int)V, g, key, pos, (const TG*)dout, scale, (TW*)dweight, partial);
+  if (g.chunks > 1)
+    embedding_join_kernel<TW, W>
+        <<<dim3(g.chunks, (units + GR_JOIN_UNITS - 1) / GR_JOIN_UNITS), EM_THREADS, 0, st>>>(
+            (int)N, (int)V, g, key, partial, scale, (TW*)dweight);
+  return launch_status("embedding_bwd");
+}
+
 template <typename TG, typename TW>
 int launch_grad(int64_t N, int64_t V, int64_t D, const int* key, const int* pos,
-                const void* dout, float scale, void* dweight, cudaStream_t st) {
-  const bool vec = D % 8 == 0 && aligned16(dout) && aligned16(dweight);
-  const int units = (int)(vec ? D / 8 : D);
-  if (vec)
-    embedding_grad_kernel<TG, TW, 8><<<(unsigned)V, EM_THREADS, 0, st>>>(
-        (int)N, (int)V, units, key, pos, (const TG*)dout, scale, (TW*)dweight);
-  else
-    embedding_grad_kernel<TG, TW, 1><<<(unsigned)V, EM_THREADS, 0, st>>>(
-        (int)N, (int)V, units, key, pos, (const TG*)dout, scale, (TW*)dweight);
-  return launch_status("embedding_bwd");
+                const void* dout, float scale, void* dweight, float* partial, cudaStream_t st) {
+  const bool vec = D % 8 == 0 && aligned16(dout) && aligned16(dweight) && aligned16(partial);
+  return vec ? launch_grad_w<TG, TW, 8>(N, V, (int)(D / 8), key, pos, dout, scale, dweight,
+                                        partial, st)
+             : launch_grad_w<TG, TW, 1>(N, V, (int)D, key, pos, dout, scale, dweight, partial,
+                                        st);
 }
 
 }  // namespace
@@ -365,8 +522,7 @@ extern "C" int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, i
 
 extern "C" size_t dabsn_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D) {
   if (N < 0 || N > INT32_MAX || V <= 0 || V >= INT32_MAX || D <= 0) return 0;
-  const SortPlan p = sort_plan(N, V);
-  return ((size_t)4 * N + (size_t)p.blocks * RS_DIGITS) * sizeof(int);
+  return sort_bytes(N, V) + partial_bytes(N, D);
 }
 
 extern "C" int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, int64_t V,
@@ -402,11 +558,12 @@ extern "C" int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, i
   }
   const int* key = s.key[(plan.passes - 1) & 1];
   const int* pos = s.pos[(plan.passes - 1) & 1];
+  float* partial = (float*)((char*)workspace + sort_bytes(N, V));
   if (out_dtype == DABSN_BF16)
     return weight_dtype == DABSN_BF16
-               ? launch_grad<bf16, bf16>(N, V, D, key, pos, dout, scale, dweight, st)
-               : launch_grad<bf16, float>(N, V, D, key, pos, dout, scale, dweight, st);
+               ? launch_grad<bf16, bf16>(N, V, D, key, pos, dout, scale, dweight, partial, st)
+               : launch_grad<bf16, float>(N, V, D, key, pos, dout, scale, dweight, partial, st);
   return weight_dtype == DABSN_BF16
-             ? launch_grad<float, bf16>(N, V, D, key, pos, dout, scale, dweight, st)
-             : launch_grad<float, float>(N, V, D, key, pos, dout, scale, dweight, st);
+             ? launch_grad<float, bf16>(N, V, D, key, pos, dout, scale, dweight, partial, st)
+             : launch_grad<float, float>(N, V, D, key, pos, dout, scale, dweight, partial, st);
 }

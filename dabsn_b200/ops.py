@@ -837,8 +837,38 @@ def ce_logits_backward(logits: Tensor, targets: Tensor, ignore_index: int, lse: 
 # ---------------------------------------------------------------------------
 # Token log-probabilities, distillation, embedding
 # ---------------------------------------------------------------------------
+# These run on single tokens too, where the host's work is what a call costs:
+# arguments go to the C entry points as plain integers, nothing is detached or
+# converted that is as it should be, and the device is switched only when
+# another one is current.
 TOP_K_MAX = 128
 TEACHER_ENTRIES_MAX = 256
+
+
+def _run(name: str, dev: torch.device, fn, *args, launches: int = 1) -> None:
+    """One C entry point on the current stream of ``dev``."""
+    if KERNEL_EVENTS is None and torch.cuda.current_device() == dev.index:
+        LAUNCH_COUNT["n"] += launches
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev), _timed(name, dev, launches):
+            st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if st != 0:
+        N.check(st, name)
+
+
+def _same_cuda(first: Tensor, *others: Tensor | None) -> torch.device:
+    dev = first.device
+    if dev.type != "cuda":
+        raise TypeError("dabsn_b200 kernels require CUDA tensors")
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError("dabsn_b200: all tensors must be on the same device")
+    return dev
+
+
+def _addr(t: Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
 def _logit_rows(logits: Tensor) -> tuple[int, int, int]:
@@ -860,37 +890,42 @@ def _temperature(temperature: float) -> float:
 
 
 def _int_rows(t: Tensor, shape, what: str) -> Tensor:
-    if tuple(t.shape) != tuple(shape):
+    """Contiguous int64 ids of the given shape."""
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"{what} must hold int64 or int32 ids, got {t.dtype}")
-    return t.detach().to(torch.int64).contiguous()
+    if t.dtype is not torch.int64:
+        if t.dtype is not torch.int32:
+            raise TypeError(f"{what} must hold int64 or int32 ids, got {t.dtype}")
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _dense_f32(t: Tensor | None) -> Tensor | None:
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
 
 
 def token_scores_forward(logits: Tensor, tokens: Tensor, top_k: int, temperature: float,
                          ignore_index: int, with_stats: bool = True):
     """logits [rows, V] (FP32/BF16, rows contiguous), tokens [rows].  Returns
-    (log_prob [rows], entropy [rows], top values [rows, k], top ids [rows, k],
-    statistics [rows, 2] or None), FP32 and int64."""
-    dev = _require_cuda(logits, tokens)
+    (log_prob [rows], entropy [rows], top values and ids [rows, k] or None for
+    k = 0, statistics [rows, 2] or None), FP32 and int64."""
+    dev = _same_cuda(logits, tokens)
     rows, V, ld = _logit_rows(logits)
     code, temperature = act_code(logits.dtype), _temperature(temperature)
     tokens = _int_rows(tokens, (rows,), "tokens")
     k = int(top_k)
     if not 0 <= k <= min(TOP_K_MAX, V):
         raise ValueError(f"top_k must lie in [0, {min(TOP_K_MAX, V)}], got {top_k}")
-    f32 = dict(device=dev, dtype=torch.float32)
-    log_prob, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
-    stats = torch.empty((rows, 2), **f32) if with_stats else None
-    top_values = torch.empty((rows, k), **f32)
-    top_ids = torch.empty((rows, k), device=dev, dtype=torch.int64)
-    lib = N.load()
-    with torch.cuda.device(dev), _timed("token_scores_fwd", dev):
-        st = lib.dabsn_token_scores_fwd(
-            code, rows, V, ld, _ptr(logits), _ptr(tokens), int(ignore_index), temperature, k,
-            _ptr(log_prob), _ptr(entropy), _ptr(stats), _ptr(top_values), _ptr(top_ids),
-            _stream(dev))
-    N.check(st, "token_scores_fwd")
+    log_prob = torch.empty(rows, device=dev, dtype=torch.float32)
+    entropy = torch.empty(rows, device=dev, dtype=torch.float32)
+    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32) if with_stats else None
+    top_values = torch.empty((rows, k), device=dev, dtype=torch.float32) if k else None
+    top_ids = torch.empty((rows, k), device=dev, dtype=torch.int64) if k else None
+    _run("token_scores_fwd", dev, N.load().dabsn_token_scores_fwd, code, rows, V, ld,
+         logits.data_ptr(), tokens.data_ptr(), ignore_index, temperature, k, log_prob.data_ptr(),
+         entropy.data_ptr(), _addr(stats), _addr(top_values), _addr(top_ids))
     return log_prob, entropy, top_values, top_ids, stats
 
 
@@ -899,18 +934,14 @@ def token_scores_backward(logits: Tensor, tokens: Tensor, temperature: float, ig
                           grad_entropy: Tensor | None) -> Tensor:
     """dlogits [rows, V] in the logits' dtype from the gradients of the
     log-probabilities and of the entropies (either may be None)."""
-    dev = _require_cuda(logits, tokens, stats, entropy, grad_log_prob, grad_entropy)
+    dev = _same_cuda(logits, tokens, stats, entropy, grad_log_prob, grad_entropy)
     rows, V, ld = _logit_rows(logits)
     tokens = _int_rows(tokens, (rows,), "tokens")
-    g, h = _grad_or_none(grad_log_prob), _grad_or_none(grad_entropy)
+    g, h = _dense_f32(grad_log_prob), _dense_f32(grad_entropy)
     dl = torch.empty((rows, V), device=dev, dtype=logits.dtype)
-    lib = N.load()
-    with torch.cuda.device(dev), _timed("token_scores_bwd", dev):
-        st = lib.dabsn_token_scores_bwd(
-            act_code(logits.dtype), rows, V, ld, _ptr(logits), _ptr(tokens), int(ignore_index),
-            _temperature(temperature), _ptr(stats), _ptr(entropy), _ptr(g), _ptr(h), _ptr(dl),
-            _stream(dev))
-    N.check(st, "token_scores_bwd")
+    _run("token_scores_bwd", dev, N.load().dabsn_token_scores_bwd, act_code(logits.dtype), rows,
+         V, ld, logits.data_ptr(), tokens.data_ptr(), ignore_index, _temperature(temperature),
+         stats.data_ptr(), entropy.data_ptr(), _addr(g), _addr(h), dl.data_ptr())
     return dl
 
 
@@ -919,52 +950,44 @@ def distill_prep(teacher_tokens: Tensor, teacher_logits: Tensor, vocab: int, tem
     """The teacher's lists [rows, K] as probabilities, in the buffer that the
     distillation kernels read: ids, probabilities, equal ids merged, which rows
     have a loss, and how many."""
-    dev = _require_cuda(teacher_tokens, teacher_logits)
+    dev = _same_cuda(teacher_tokens, teacher_logits)
     if teacher_tokens.dim() != 2:
         raise ValueError("teacher_tokens must be [rows, entries]")
     rows, K = teacher_tokens.shape
     if not 1 <= K <= TEACHER_ENTRIES_MAX:
         raise ValueError(f"a teacher's list holds 1 to {TEACHER_ENTRIES_MAX} entries, got {K}")
     ids = _int_rows(teacher_tokens, (rows, K), "teacher_tokens")
-    if tuple(teacher_logits.shape) != (rows, K):
+    if teacher_logits.shape != (rows, K):
         raise ValueError(f"teacher_logits has shape {tuple(teacher_logits.shape)}, expected "
                          f"{(rows, K)}")
-    tl = teacher_logits.detach().contiguous()
+    tl = teacher_logits if teacher_logits.is_contiguous() else teacher_logits.contiguous()
     code, temperature = act_code(tl.dtype), _temperature(temperature)
     lib = N.load()
-    lists = torch.empty(int(lib.dabsn_distill_list_bytes(rows, K)), device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev), _timed("distill_prep", dev):
-        st = lib.dabsn_distill_prep(code, rows, vocab, K, _ptr(ids), _ptr(tl), temperature,
-                                    int(ignore_index), _ptr(lists), _stream(dev))
-    N.check(st, "distill_prep")
+    lists = torch.empty(lib.dabsn_distill_list_bytes(rows, K), device=dev, dtype=torch.uint8)
+    _run("distill_prep", dev, lib.dabsn_distill_prep, code, rows, vocab, K, ids.data_ptr(),
+         tl.data_ptr(), temperature, ignore_index, lists.data_ptr())
     return lists
 
 
 def distill_forward(logits: Tensor, lists: Tensor, entries: int, temperature: float):
     """(row losses [rows] FP32, statistics [rows, 2]) of the student's logits
     [rows, V] against prepared lists."""
-    dev = _require_cuda(logits, lists)
+    dev = _same_cuda(logits, lists)
     rows, V, ld = _logit_rows(logits)
     loss = torch.empty(rows, device=dev, dtype=torch.float32)
     stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
-    lib = N.load()
-    with torch.cuda.device(dev), _timed("distill_fwd", dev):
-        st = lib.dabsn_distill_fwd(act_code(logits.dtype), rows, V, ld, _ptr(logits), entries,
-                                   _ptr(lists), _temperature(temperature), _ptr(loss),
-                                   _ptr(stats), _stream(dev))
-    N.check(st, "distill_fwd")
+    _run("distill_fwd", dev, N.load().dabsn_distill_fwd, act_code(logits.dtype), rows, V, ld,
+         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature),
+         loss.data_ptr(), stats.data_ptr())
     return loss, stats
 
 
 def distill_reduce(row_loss: Tensor, lists: Tensor, entries: int, mean: bool) -> Tensor:
     """Sum of the row losses, or their mean over the rows that have one; FP32 []."""
-    dev = _require_cuda(row_loss, lists)
+    dev = _same_cuda(row_loss, lists)
     out = torch.empty((), device=dev, dtype=torch.float32)
-    lib = N.load()
-    with torch.cuda.device(dev), _timed("distill_reduce", dev):
-        st = lib.dabsn_distill_reduce(row_loss.shape[0], entries, _ptr(row_loss), _ptr(lists),
-                                      int(mean), _ptr(out), _stream(dev))
-    N.check(st, "distill_reduce")
+    _run("distill_reduce", dev, N.load().dabsn_distill_reduce, row_loss.shape[0], entries,
+         row_loss.data_ptr(), lists.data_ptr(), int(mean), out.data_ptr())
     return out
 
 
@@ -972,62 +995,50 @@ def distill_backward(logits: Tensor, lists: Tensor, entries: int, temperature: f
                      stats: Tensor, mean: bool, weight: Tensor) -> Tensor:
     """dlogits [rows, V] for row weights ``weight`` ([rows], or [] for all
     rows), divided by the number of rows with a loss if ``mean``."""
-    dev = _require_cuda(logits, lists, stats, weight)
+    dev = _same_cuda(logits, lists, stats, weight)
     rows, V, ld = _logit_rows(logits)
-    w = weight.detach().to(torch.float32).contiguous()
+    w = _dense_f32(weight)
     dl = torch.empty((rows, V), device=dev, dtype=logits.dtype)
-    lib = N.load()
-    with torch.cuda.device(dev), _timed("distill_bwd", dev):
-        st = lib.dabsn_distill_bwd(act_code(logits.dtype), rows, V, ld, _ptr(logits), entries,
-                                   _ptr(lists), _temperature(temperature), _ptr(stats),
-                                   int(mean), _ptr(w), int(w.dim() > 0), _ptr(dl), _stream(dev))
-    N.check(st, "distill_bwd")
+    _run("distill_bwd", dev, N.load().dabsn_distill_bwd, act_code(logits.dtype), rows, V, ld,
+         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature),
+         stats.data_ptr(), int(mean), w.data_ptr(), int(w.dim() > 0), dl.data_ptr())
     return dl
 
 
 def embedding_forward(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
-    """scale * weight[tokens] in ``dtype``: tokens [N], weight [V, D] -> [N, D]."""
-    dev = _require_cuda(weight, tokens)
+    """scale * weight[tokens] in ``dtype``: tokens [...], weight [V, D] -> [..., D]."""
+    dev = _same_cuda(weight, tokens)
     if weight.dim() != 2:
         raise ValueError("the embedding table must be [V, D]")
     V, D = weight.shape
     if V < 1 or D < 1:
         raise ValueError(f"an embedding table of shape {tuple(weight.shape)} is empty")
-    if tokens.dim() != 1:
-        raise ValueError("tokens must be [N]")
-    n = tokens.shape[0]
-    ids = _int_rows(tokens, (n,), "tokens")
-    w = weight.detach()
+    ids = _int_rows(tokens, tokens.shape, "tokens")
+    w = weight
     if w.stride(1) != 1 or w.stride(0) < D:
         w = w.contiguous()
-    ldw = w.stride(0) if V > 1 else D
-    out = torch.empty((n, D), device=dev, dtype=dtype)
-    lib = N.load()
-    with torch.cuda.device(dev), _timed("embedding_fwd", dev):
-        st = lib.dabsn_embedding_fwd(act_code(w.dtype), act_code(dtype), n, V, D, _ptr(ids),
-                                     _ptr(w), ldw, float(scale), _ptr(out), _stream(dev))
-    N.check(st, "embedding_fwd")
+    out = torch.empty((*tokens.shape, D), device=dev, dtype=dtype)
+    _run("embedding_fwd", dev, N.load().dabsn_embedding_fwd, act_code(w.dtype), act_code(dtype),
+         ids.numel(), V, D, ids.data_ptr(), w.data_ptr(), w.stride(0) if V > 1 else D, scale,
+         out.data_ptr())
     return out
 
 
 def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: float,
                        padding_idx: int | None, dtype: torch.dtype) -> Tensor:
-    """The table's gradient [vocab, D] in ``dtype`` from grad_out [N, D]: sums
+    """The table's gradient [vocab, D] in ``dtype`` from grad_out [..., D]: sums
     over equal tokens in FP32, in order of position (no atomics)."""
-    dev = _require_cuda(grad_out, tokens)
-    n, D = grad_out.shape
-    ids = _int_rows(tokens, (n,), "tokens")
-    g = grad_out.detach().contiguous()
+    dev = _same_cuda(grad_out, tokens)
+    ids = _int_rows(tokens, grad_out.shape[:-1], "tokens")
+    n, D = ids.numel(), grad_out.shape[-1]
+    g = grad_out if grad_out.is_contiguous() else grad_out.contiguous()
     dw = torch.empty((vocab, D), device=dev, dtype=dtype)
     lib = N.load()
-    ws = torch.empty(int(lib.dabsn_embedding_bwd_workspace(n, vocab, D)), device=dev,
-                     dtype=torch.uint8)
-    with torch.cuda.device(dev), _timed("embedding_bwd", dev):
-        st = lib.dabsn_embedding_bwd(
-            act_code(g.dtype), act_code(dtype), n, vocab, D, _ptr(ids),
-            -1 if padding_idx is None else int(padding_idx), _ptr(g), float(scale), _ptr(dw),
-            _ptr(ws), ws.numel(), _stream(dev))
-    N.check(st, "embedding_bwd")
+    need = lib.dabsn_embedding_bwd_workspace(n, vocab, D)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    _run("embedding_bwd", dev, lib.dabsn_embedding_bwd, act_code(g.dtype), act_code(dtype), n,
+         vocab, D, ids.data_ptr(), -1 if padding_idx is None else padding_idx, g.data_ptr(),
+         scale, dw.data_ptr(), ws.data_ptr(), need)
     return dw
 
 
