@@ -719,35 +719,42 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
 
 
 class _Distillation(torch.autograd.Function):
-    """Row losses (reduction "none"), their sum or their mean."""
+    """Row losses (reduction "none"), their sum or their mean.  For the last two
+    the forward writes the gradient too (one pass over the logits instead of
+    two and a half); the first reverse hands it out, after the kernel that
+    writes it anew where the upstream gradient is not 1.  A later reverse, and
+    one captured in another graph than the forward, starts from the logits."""
 
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, ignore_index,
                 reduction):
-        loss, lists, row_stats = _distill(logits, teacher_tokens, teacher_logits, temperature,
-                                          ignore_index, reduction)
-        ctx.save_for_backward(logits, lists, row_stats)
-        ctx.meta = (teacher_tokens.shape[1], temperature, reduction)
-        return loss
+        entries, mean = teacher_tokens.shape[1], reduction == "mean"
+        lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
+                                 ignore_index)
+        both = None
+        if reduction != "none":
+            both = ops.distill_gradient(logits, lists, entries, temperature, mean)
+        if both is None:
+            (loss, stats), ctx.ready = ops.distill_forward(logits, lists, entries,
+                                                           temperature), None
+        else:
+            loss, stats, ctx.ready = both
+            ctx.capture = ops.capture_id(logits.device)
+        ctx.save_for_backward(logits, lists, stats)
+        ctx.meta = (entries, temperature, reduction)
+        return loss if reduction == "none" else ops.distill_reduce(loss, lists, entries, mean)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         logits, lists, stats = ctx.saved_tensors
         entries, temperature, reduction = ctx.meta
+        ready, ctx.ready = ctx.ready, None
+        if ready is not None and ctx.capture != ops.capture_id(logits.device):
+            ready = None
         dl = ops.distill_backward(logits, lists, entries, temperature, stats,
-                                  reduction == "mean", grad)
+                                  reduction == "mean", grad, ready)
         return dl, None, None, None, None, None
-
-
-def _distill(logits, teacher_tokens, teacher_logits, temperature, ignore_index, reduction):
-    entries = teacher_tokens.shape[1]
-    lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
-                             ignore_index)
-    loss, stats = ops.distill_forward(logits, lists, entries, temperature)
-    if reduction != "none":
-        loss = ops.distill_reduce(loss, lists, entries, reduction == "mean")
-    return loss, lists, stats
 
 
 def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor, *,
@@ -786,9 +793,16 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     if teacher_tokens.dim() != 2:
         teacher_tokens = teacher_tokens.reshape(-1, entries)
         teacher_logits = teacher_logits.reshape(-1, entries)
-    args = (rows, teacher_tokens, teacher_logits.detach(), temperature, int(ignore_index),
-            reduction)
-    loss = _Distillation.apply(*args) if _differentiates(rows) else _distill(*args)[0]
+    ignore_index = int(ignore_index)
+    if _differentiates(rows):
+        loss = _Distillation.apply(rows, teacher_tokens, teacher_logits.detach(), temperature,
+                                   ignore_index, reduction)
+    else:
+        lists = ops.distill_prep(teacher_tokens, teacher_logits, rows.shape[1], temperature,
+                                 ignore_index)
+        loss, _ = ops.distill_forward(rows, lists, entries, temperature)
+        if reduction != "none":
+            loss = ops.distill_reduce(loss, lists, entries, reduction == "mean")
     return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 

@@ -25,7 +25,7 @@ using namespace rowsm;
 
 constexpr int DT_THREADS = 256;
 constexpr int DT_MAX_K = 256;
-constexpr int DT_PREP_THREADS = 512;
+constexpr int DT_PREP_THREADS = 256;
 constexpr int DT_STATUS_BAD_TOKEN = 8;
 
 // Entry of a row's list after preparation: id (-1: absent), q, and q summed
@@ -39,7 +39,7 @@ struct Entries {
 
 int prep_blocks(int64_t rows) {
   const int64_t warps = DT_PREP_THREADS / 32;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + warps - 1) / warps, 148));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + warps - 1) / warps, 148 * 4));
 }
 
 Entries entries_of(void* ws, int64_t rows, int64_t K) {
@@ -51,15 +51,16 @@ Entries entries_of(void* ws, int64_t rows, int64_t K) {
   return e;
 }
 
-template <typename T>
+// One warp a row, PER entries a lane.
+template <typename T, int PER>
 __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
     long long rows, int V, int K, const int64_t* __restrict__ ids, const T* __restrict__ logits,
     float inv_t, long long ignore_index, Entries out, int* status) {
-  constexpr int PER = DT_MAX_K / 32;
   __shared__ int live_rows[DT_PREP_THREADS / 32];
+  constexpr int TABLE = 128 * PER;  // four slots an entry
+  __shared__ int table[DT_PREP_THREADS / 32][TABLE];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long nwarps = (long long)gridDim.x * (DT_PREP_THREADS / 32);
-  const int per = (K + 31) / 32;
   int counted = 0;
   for (long long r = (long long)blockIdx.x * (DT_PREP_THREADS / 32) + warp; r < rows;
        r += nwarps) {
@@ -72,18 +73,19 @@ __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
       id[i] = -1;
       q[i] = -INFINITY;
       const int k = lane + 32 * i;
-      if (i < per && k < K) {
+      if (k < K) {
         const long long t = ids[r * K + k];
+        const float x = to_f<T>(logits[r * K + k]);
         if (t != ignore_index) {
           if (t >= 0 && t < V) {
             id[i] = (int)t;
-            q[i] = to_f<T>(logits[r * K + k]);
-            m = fmaxf(m, q[i]);
+            q[i] = x;
           } else {
             bad = true;
           }
         }
       }
+      m = fmaxf(m, q[i]);
     }
     m = finite_max(warp_max(m));
     float sum = 0.f;
@@ -100,34 +102,54 @@ __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
     if (bad && status && lane == 0) atomicExch(status, DT_STATUS_BAD_TOKEN);
 #pragma unroll
     for (int i = 0; i < PER; ++i) q[i] *= inv;
-    // merge equal ids into the first of them
-    float all[PER];
+    // An id listed twice is rare: a hash table of the row's ids finds out
+    // whether there is one, and only then are they merged.
 #pragma unroll
-    for (int i = 0; i < PER; ++i) all[i] = 0.f;
-    unsigned later = 0u;  // bit i: an earlier entry has id[i]
-    for (int k = 0; k < K; ++k) {
-      int other = 0;
-      float oq = 0.f;
+    for (int i = 0; i < TABLE / 32; ++i) table[warp][lane + 32 * i] = -1;
+    __syncwarp();
+    bool twice = false;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int v = __shfl_sync(0xffffffffu, id[i], k & 31);
-        const float w = __shfl_sync(0xffffffffu, q[i], k & 31);
-        if (i == (k >> 5)) {
-          other = v;
-          oq = w;
-        }
+    for (int i = 0; i < PER; ++i) {
+      if (id[i] < 0) continue;
+      unsigned slot = (unsigned)id[i] * 2654435761u >> 16;
+      for (int probe = 0; probe < TABLE; ++probe, ++slot) {
+        const int had = atomicCAS(&table[warp][slot % TABLE], -1, id[i]);
+        if (had == id[i]) twice = true;
+        if (had == -1 || had == id[i]) break;
       }
+    }
+    __syncwarp();
+    float all[PER];
+    unsigned later = 0u;  // bit i: an earlier entry has id[i]
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (id[i] == other) {
-          all[i] += oq;
-          if (k < lane + 32 * i) later |= 1u << i;
+    for (int i = 0; i < PER; ++i) all[i] = q[i];
+    if (__any_sync(0xffffffffu, twice)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) all[i] = 0.f;
+      for (int k = 0; k < K; ++k) {
+        int other = 0;
+        float oq = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int v = __shfl_sync(0xffffffffu, id[i], k & 31);
+          const float w = __shfl_sync(0xffffffffu, q[i], k & 31);
+          if (i == (k >> 5)) {
+            other = v;
+            oq = w;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (id[i] == other) {
+            all[i] += oq;
+            if (k < lane + 32 * i) later |= 1u << i;
+          }
+      }
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int k = lane + 32 * i;
-      if (i < per && k < K) {
+      if (k < K) {
         // a list that names a token outside the vocabulary makes its loss NaN
         const float mine = bad ? __int_as_float(0x7fc00000) : q[i];
         out.id[r * K + k] = id[i];
@@ -143,6 +165,21 @@ __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
     for (int w = 0; w < DT_PREP_THREADS / 32; ++w) n += live_rows[w];
     out.counts[blockIdx.x] = n;
   }
+}
+
+template <typename T>
+void launch_prep(int64_t rows, int64_t V, int64_t K, const int64_t* ids, const void* logits,
+                 float inv_t, int64_t ignore_index, const Entries& e, cudaStream_t st) {
+  const int grid = prep_blocks(rows);
+  int* status = device_status();
+#define DISTILL_PREP(PER)                                                          \
+  distill_prep_kernel<T, PER><<<grid, DT_PREP_THREADS, 0, st>>>(                   \
+      rows, (int)V, (int)K, ids, (const T*)logits, inv_t, ignore_index, e, status)
+  if (K <= 32) DISTILL_PREP(1);
+  else if (K <= 64) DISTILL_PREP(2);
+  else if (K <= 128) DISTILL_PREP(4);
+  else DISTILL_PREP(8);
+#undef DISTILL_PREP
 }
 
 // sum_k q_k (log q_k - log p_id_k) over the entries of this thread.
@@ -176,7 +213,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     }
     const T* row = logits + (size_t)r * ld;
     const Stats all =
-        block_merge<DT_THREADS>(sweep<T, DT_THREADS>(row, V, threadIdx.x, c), part, c);
+        block_merge<DT_THREADS>(sweep<T, DT_THREADS, false>(row, V, threadIdx.x, c), part, c);
     const float m = finite_max(all.mx);
     if (threadIdx.x < 32) {
       const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K,
@@ -199,16 +236,22 @@ __device__ __forceinline__ float mean_scale(const int* counts, int blocks) {
   return 1.f / (float)max(n, 1);
 }
 
-template <typename T, bool SAME>
+// `unless_one`: dlogits holds the gradient for weight 1 already, and a weight of
+// 1 (the usual one: nothing behind a mean but backward()) leaves it as it is.
+// Any other weight starts from the logits again, so that every element is
+// rounded once.
+template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
     int mean_blocks, float temperature, const float2* __restrict__ stats,
-    const float* __restrict__ weight, long long wstride, T* __restrict__ dlogits) {
+    const float* __restrict__ weight, long long wstride, bool unless_one,
+    T* __restrict__ dlogits, long long ldd) {
+  if (unless_one && *weight == 1.f) return;
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
   const float scale = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = logits + (size_t)r * ld;
-    T* drow = dlogits + (size_t)r * V;
+    T* drow = dlogits + (size_t)r * ldd;
     const float2 ms = stats[r];
     if (!list.live[r] || ms.y == 0.f) {
       zero_row<T, DT_THREADS>(drow, V, threadIdx.x);
@@ -216,15 +259,314 @@ __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     }
     const float w = scale * weight[r * wstride];
     const float A = w / ms.y;
-    grad_sweep<T, DT_THREADS, false, SAME>(row, drow, V, threadIdx.x, ms.x, c, A, 0.f);
+    grad_sweep<T, DT_THREADS, false>(row, drow, V, threadIdx.x, ms.x, c, A, 0.f);
     __syncthreads();  // listed elements are rounded once, with their own term
     for (int k = threadIdx.x; k < K; k += DT_THREADS) {
       const int id = list.id[r * K + k];
       const float q = list.q[r * K + k].y;
       if (id >= 0 && q > 0.f)
-        drow[id] = from_f<T>(grad_value<false>(to_f<T>(row[id]), ms.x, c, A, 0.f) - w * q);
+        drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), ms.x, c, A, 0.f)));
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// Small vocabularies: a warp holds a row in registers (four vectors a lane), so
+// loss and gradient take one read, and a CTA eight rows.
+// ---------------------------------------------------------------------------
+template <typename T>
+constexpr int warp_row() {
+  return 4 * 32 * Vec<T>::N;
+}
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
+    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
+    T* __restrict__ dlogits, long long ldd) {
+  const int lane = threadIdx.x & 31;
+  const long long r = (long long)blockIdx.x * (DT_THREADS / 32) + (threadIdx.x >> 5);
+  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
+  const float w =
+      GRAD ? temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f) : 0.f;
+  if (r >= rows) return;
+  const T* row = logits + (size_t)r * ld;
+  T* drow = GRAD ? dlogits + (size_t)r * ldd : nullptr;
+  if (!list.live[r]) {
+    if (GRAD) zero_row<T, 32>(drow, V, lane);
+    if (lane == 0) {
+      loss[r] = 0.f;
+      if (stats) stats[r] = make_float2(0.f, 0.f);
+    }
+    return;
+  }
+  const RowShape s = row_shape(row, V);
+  const uint4* pv = reinterpret_cast<const uint4*>(row + s.head);
+  uint4 raw[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    constexpr unsigned ni = Vec<T>::kNegInf;
+    raw[u] = lane + 32 * u < s.nv ? __ldg(pv + lane + 32 * u) : make_uint4(ni, ni, ni, ni);
+  }
+  const float head = lane < s.head ? to_f<T>(row[lane]) : -INFINITY;
+  const float tail = lane < s.tail ? to_f<T>(row[s.tail0 + lane]) : -INFINITY;
+  Stats st;
+  add_vectors<T, 4, false>(st, raw, c);
+  add_value(st, head, c);
+  add_value(st, tail, c);
+  st.sd = 0.f;
+  st = warp_merge(st, c);
+  const float m = finite_max(st.mx);
+  const bool empty = st.s == 0.f;
+  const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K, lane, m,
+                                            inv_t, logf(st.s), empty));
+  if (lane == 0) {
+    loss[r] = temperature * temperature * l;
+    if (stats) stats[r] = make_float2(m, st.s);
+  }
+  if (!GRAD) return;
+  const float A = empty ? 0.f : w / st.s;
+  const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), A2 = pair(A, A);
+  uint4* dv = reinterpret_cast<uint4*>(drow + s.head);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + 32 * u < s.nv)
+      dv[lane + 32 * u] = grad_vector<T, false>(raw[u], m2, c2, A2, A2);
+  if (lane < s.head) drow[lane] = from_f<T>(grad_value<false>(head, m, c, A, 0.f));
+  if (lane < s.tail) drow[s.tail0 + lane] = from_f<T>(grad_value<false>(tail, m, c, A, 0.f));
+  __syncwarp();  // listed elements are rounded once, with their own term
+  for (int k = lane; k < K && !empty; k += 32) {
+    const int id = list.id[r * K + k];
+    const float q = list.q[r * K + k].y;
+    if (id >= 0 && q > 0.f)
+      drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Loss and gradient in one pass over the logits (weights known beforehand: the
+// sum or the mean of the rows' losses, upstream gradient 1).
+//
+// The row stays on the SM between its statistics and its gradient: every
+// thread copies its own vectors into its own slots of shared memory
+// (cp.async), so neither sweep needs a barrier with another thread, and the
+// copies of the next row are issued slot by slot as the gradient of this one
+// leaves them: reads, arithmetic and writes of neighbouring rows overlap, with
+// three CTAs an SM.  What bounds it is HBM: V read and V written a row.  A row
+// that does not fit a third of an SM's shared memory is shared by a cluster of
+// 2, 4 or 8 CTAs, which merge their statistics through distributed shared
+// memory; so is a row when there are fewer rows than SMs.
+// ---------------------------------------------------------------------------
+constexpr int DF_THREADS = 256;
+static_assert(DT_MAX_K <= DF_THREADS, "a thread holds at most one entry");
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src)
+               : "memory");
+}
+
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
+    int mean_blocks, float temperature, int share, float* __restrict__ loss,
+    float2* __restrict__ stats, T* __restrict__ dlogits, long long ldd) {
+  extern __shared__ uint4 slots[];  // [vectors of a thread][DF_THREADS]
+  __shared__ float part[DF_THREADS / 32][3];
+  __shared__ float peer[2][8][2];
+  __shared__ float loss_part[DF_THREADS / 32];
+  const int t = threadIdx.x;
+  const int cl = SPLIT ? (int)cluster_nctarank() : 1;
+  const int rank = SPLIT ? (int)cluster_ctarank() : 0;
+  const long long stride = gridDim.x / cl;
+  const int a = min(rank * share, V), n = min(share, V - a);
+  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
+  const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
+
+  // The next row from r on that has a loss; the others' gradient is zero.
+  auto next_live = [&](long long r) {
+    while (r < rows && !list.live[r]) {
+      zero_row<T, DF_THREADS>(dlogits + (size_t)r * ldd + a, n, t);
+      if (t == 0 && rank == 0) {
+        loss[r] = 0.f;
+        stats[r] = make_float2(0.f, 0.f);
+      }
+      r += stride;
+    }
+    return r;
+  };
+
+  long long r = next_live(blockIdx.x / cl);
+  float edge[2] = {0.f, 0.f};  // this thread's head and tail element
+  auto load_edges = [&](const T* p, const RowShape& s) {
+    if (t < s.head) edge[0] = to_f<T>(p[t]);
+    if (t < s.tail) edge[1] = to_f<T>(p[s.tail0 + t]);
+  };
+  if (r < rows) {
+    const T* p = logits + (size_t)r * ld + a;
+    const RowShape s = row_shape(p, n);
+    for (int k = t; k < s.nv; k += DF_THREADS)
+      cp_async16(&slots[k], reinterpret_cast<const uint4*>(p + s.head) + k);
+    load_edges(p, s);
+  }
+  cp_async_commit();
+  if (SPLIT) cluster_sync_all();  // every CTA runs before another writes to it
+  for (int turn = 0; r < rows; turn ^= 1) {
+    const T* row = logits + (size_t)r * ld;
+    const RowShape s = row_shape(row + a, n);
+    int id = -1;
+    float2 q = make_float2(0.f, 0.f);
+    float x = 0.f;
+    if (t < K) {
+      id = list.id[r * K + t];
+      q = list.q[r * K + t];
+      if (id >= 0) x = to_f<T>(row[id]);
+    }
+    cp_async_wait<0>();
+    Stats st;
+    {
+      int k = t;
+      for (; k + 3 * DF_THREADS < s.nv; k += 4 * DF_THREADS) {
+        const uint4 raw[4] = {slots[k], slots[k + DF_THREADS], slots[k + 2 * DF_THREADS],
+                              slots[k + 3 * DF_THREADS]};
+        add_vectors<T, 4, false>(st, raw, c);
+      }
+      for (; k < s.nv; k += DF_THREADS) {
+        const uint4 raw[1] = {slots[k]};
+        add_vectors<T, 1, false>(st, raw, c);
+      }
+      if (t < s.head) add_value(st, edge[0], c);
+      if (t < s.tail) add_value(st, edge[1], c);
+    }
+    st.sd = 0.f;
+    st = block_merge<DF_THREADS>(st, part, c);
+    if (SPLIT) {
+      if (t < cl) {
+        const uint32_t to = map_shared_rank(&peer[turn][rank][0], t);
+        st_cluster_f32(to, st.mx);
+        st_cluster_f32(to + 4, st.s);
+      }
+      __syncwarp();
+      cluster_sync_all();
+      Stats all;
+      for (int o = 0; o < cl; ++o) {
+        Stats b;
+        b.mx = peer[turn][o][0];
+        b.s = peer[turn][o][1];
+        merge(all, b, c);
+      }
+      st = all;
+    }
+    const float m = finite_max(st.mx);
+    const bool empty = st.s == 0.f;
+    if (rank == 0) {
+      float l = 0.f;
+      if (q.x != q.x) l = q.x;
+      if (id >= 0 && q.x > 0.f)
+        l = q.x * (logf(q.x) - (empty ? -INFINITY : (x - m) * inv_t - logf(st.s)));
+      l = warp_sum(l);
+      if ((t & 31) == 0) loss_part[t >> 5] = l;
+    }
+
+    // gradient, and the next row's copies
+    const float A = empty ? 0.f : w / st.s;
+    const long long rn = next_live(r + stride);
+    const T* pn = logits + (size_t)(rn < rows ? rn : r) * ld + a;
+    RowShape sn = row_shape(pn, n);
+    if (rn >= rows) sn.nv = sn.head = sn.tail = 0;
+    const uint4* nv = reinterpret_cast<const uint4*>(pn + sn.head);
+    T* drow = dlogits + (size_t)r * ldd;
+    uint4* dv = reinterpret_cast<uint4*>(drow + a + s.head);
+    {
+      const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), A2 = pair(A, A);
+      // rows of other alignments differ by a vector at most
+      const int most = max(s.nv, sn.nv);
+      for (int k = t; k < most; k += 4 * DF_THREADS) {
+        uint4 raw[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (k + u * DF_THREADS < s.nv) raw[u] = slots[k + u * DF_THREADS];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = k + u * DF_THREADS;
+          if (i < s.nv) dv[i] = grad_vector<T, false>(raw[u], m2, c2, A2, A2);
+          if (i < sn.nv) cp_async16(&slots[i], nv + i);
+        }
+      }
+      if (t < s.head)
+        drow[a + t] = from_f<T>(grad_value<false>(edge[0], m, c, A, 0.f));
+      if (t < s.tail)
+        drow[a + s.tail0 + t] = from_f<T>(grad_value<false>(edge[1], m, c, A, 0.f));
+      load_edges(pn, sn);
+    }
+    cp_async_commit();
+    __syncthreads();  // listed elements are rounded once, with their own term
+    if (id >= a && id < a + n && q.y > 0.f && !empty)
+      drow[id] = from_f<T>(fmaf(-w, q.y, grad_value<false>(x, m, c, A, 0.f)));
+    if (rank == 0 && t == 0) {
+      float l = 0.f;
+      for (int i = 0; i < DF_THREADS / 32; ++i) l += loss_part[i];
+      loss[r] = temperature * temperature * l;
+      stats[r] = make_float2(m, st.s);
+    }
+    r = rn;
+  }
+}
+
+// How the fused kernel shares a row: CTAs a row (0: the row does not fit), the
+// elements of each, and its shared memory.
+struct GradPlan {
+  int cl, share, smem, per_sm;
+};
+
+GradPlan grad_plan(int64_t rows, int64_t V, int size) {
+  const int vw = 16 / size, unit = DF_THREADS * 16;
+  GradPlan g;
+  for (g.cl = 1;; g.cl *= 2) {
+    const int64_t share = ((V + g.cl - 1) / g.cl + vw - 1) / vw * vw;
+    const int64_t smem = (share / vw * 16 + unit - 1) / unit * unit;
+    g.share = (int)share;
+    g.smem = (int)std::min<int64_t>(smem, 1 << 30);
+    // three CTAs an SM; a cluster of eight may take all of it
+    const bool fits = smem <= (g.cl == 8 ? 220 : 72) * 1024;
+    const bool idle = rows * g.cl < 148 && share >= 2 * DF_THREADS * vw;
+    if (fits && (!idle || g.cl == 8)) break;
+    if (g.cl == 8) {
+      g.cl = 0;
+      return g;
+    }
+  }
+  g.per_sm = std::min(3, 224 * 1024 / (g.smem + 1024));
+  return g;
+}
+
+template <typename T, bool SPLIT>
+int launch_grad(const GradPlan& g, int64_t rows, int64_t V, int64_t ld, const void* logits,
+                int64_t K, const Entries& e, int mean_blocks, float temperature, float* loss,
+                float* stats, void* dlogits, int64_t ldd, cudaStream_t st) {
+  auto kernel = distill_grad_kernel<T, SPLIT>;
+  if (!kernel_prepared((const void*)kernel, g.smem)) return DABSN_ERR_LAUNCH;
+  const int64_t clusters = std::max<int64_t>(1, std::min<int64_t>(rows, 148 * g.per_sm / g.cl));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * g.cl), 1, 1);
+  cfg.blockDim = dim3(DF_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = g.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = g.cl;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(
+      &cfg, kernel, (long long)rows, (int)V, (long long)ld, (const T*)logits, (int)K, e,
+      mean_blocks, temperature, g.share, loss, (float2*)stats, (T*)dlogits, (long long)ldd);
+  if (err != cudaSuccess) {
+    set_error("distill_grad launch: %s (cluster=%d smem=%d)", cudaGetErrorString(err), g.cl,
+              g.smem);
+    return DABSN_ERR_LAUNCH;
+  }
+  return DABSN_OK;
 }
 
 // result = sum of the row losses (times 1 / live rows if mean_blocks), in a
@@ -297,17 +639,55 @@ extern "C" int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, in
   }
   const Entries e = entries_of(list, rows, K);
   cudaStream_t st = (cudaStream_t)stream;
-  const int grid = prep_blocks(rows);
   if (teacher_dtype == DABSN_BF16)
-    distill_prep_kernel<bf16><<<grid, DT_PREP_THREADS, 0, st>>>(
-        rows, (int)V, (int)K, teacher_tokens, (const bf16*)teacher_logits, 1.f / temperature,
-        ignore_index, e, device_status());
+    launch_prep<bf16>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
+                      ignore_index, e, st);
   else
-    distill_prep_kernel<float><<<grid, DT_PREP_THREADS, 0, st>>>(
-        rows, (int)V, (int)K, teacher_tokens, (const float*)teacher_logits, 1.f / temperature,
-        ignore_index, e, device_status());
+    launch_prep<float>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
+                       ignore_index, e, st);
   return launch_status("distill_prep");
 }
+
+namespace {
+
+template <typename T>
+int fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
+        float temperature, float* row_loss, float* stats, cudaStream_t st) {
+  if (V <= warp_row<T>()) {
+    const int64_t grid = (rows + DT_THREADS / 32 - 1) / (DT_THREADS / 32);
+    distill_warp_kernel<T, false><<<(unsigned)grid, DT_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, (int)K, e, 0, temperature, row_loss, (float2*)stats,
+        nullptr, 0);
+  } else {
+    distill_fwd_kernel<T><<<row_grid(rows), DT_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, (int)K, e, temperature, row_loss, (float2*)stats);
+  }
+  return launch_status("distill_fwd");
+}
+
+template <typename T>
+int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
+         float temperature, int mean_blocks, float* row_loss, float* stats, void* dlogits,
+         int64_t ldd, cudaStream_t st) {
+  if (V <= warp_row<T>()) {
+    const int64_t grid = (rows + DT_THREADS / 32 - 1) / (DT_THREADS / 32);
+    distill_warp_kernel<T, true><<<(unsigned)grid, DT_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
+        (float2*)stats, (T*)dlogits, ldd);
+    return launch_status("distill_grad");
+  }
+  const GradPlan g = grad_plan(rows, V, sizeof(T));
+  if (g.cl == 0) {
+    set_error("distill_grad: a row of %lld logits does not fit", (long long)V);
+    return DABSN_ERR_UNSUPPORTED;
+  }
+  return g.cl > 1 ? launch_grad<T, true>(g, rows, V, ld, logits, K, e, mean_blocks, temperature,
+                                         row_loss, stats, dlogits, ldd, st)
+                  : launch_grad<T, false>(g, rows, V, ld, logits, K, e, mean_blocks, temperature,
+                                          row_loss, stats, dlogits, ldd, st);
+}
+
+}  // namespace
 
 extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
                                  const void* logits, int64_t K, const void* list,
@@ -317,39 +697,61 @@ extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
   if (rows == 0) return DABSN_OK;
   const Entries e = entries_of(const_cast<void*>(list), rows, K);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == DABSN_BF16)
-    distill_fwd_kernel<bf16><<<row_grid(rows), DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const bf16*)logits, (int)K, e, temperature, row_loss, (float2*)stats);
-  else
-    distill_fwd_kernel<float><<<row_grid(rows), DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const float*)logits, (int)K, e, temperature, row_loss,
-        (float2*)stats);
-  return launch_status("distill_fwd");
+  return dtype == DABSN_BF16
+             ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st)
+             : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st);
 }
 
-extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
-                                 const void* logits, int64_t K, const void* list,
-                                 float temperature, const float* stats, int mean,
-                                 const float* weight, int64_t weight_stride, void* dlogits,
-                                 void* stream) {
-  const int bad = check_distill("distill_bwd", dtype, rows, V, ld, K, temperature);
+extern "C" int dabsn_distill_grad_fits(int dtype, int64_t rows, int64_t V) {
+  if (rows < 0 || V <= 0 || V >= INT32_MAX) return 0;
+  return grad_plan(rows, V, dtype == DABSN_BF16 ? 2 : 4).cl > 0;
+}
+
+extern "C" int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld,
+                                  const void* logits, int64_t K, const void* list,
+                                  float temperature, int mean, float* row_loss, float* stats,
+                                  void* dlogits, int64_t ldd, void* stream) {
+  int bad = check_distill("distill_grad", dtype, rows, V, ld, K, temperature);
+  if (!bad)
+    bad = check_gradient_rows("distill_grad", dtype, rows, V, ld, logits, ldd, dlogits);
   if (bad) return bad;
   if (rows == 0) return DABSN_OK;
   const Entries e = entries_of(const_cast<void*>(list), rows, K);
   cudaStream_t st = (cudaStream_t)stream;
   const int mb = mean ? prep_blocks(rows) : 0;
-  const unsigned grid = row_grid(rows);
-  const bool bf = dtype == DABSN_BF16;
-  const bool same = same_phase(logits, ld, dlogits, V, bf ? 2 : 4);
-#define DISTILL_BWD(T, SAME)                                                                  \
-  distill_bwd_kernel<T, SAME><<<grid, DT_THREADS, 0, st>>>(                                   \
-      rows, (int)V, ld, (const T*)logits, (int)K, e, mb, temperature, (const float2*)stats,   \
-      weight, weight_stride, (T*)dlogits)
-  if (bf && same) DISTILL_BWD(bf16, true);
-  else if (bf) DISTILL_BWD(bf16, false);
-  else if (same) DISTILL_BWD(float, true);
-  else DISTILL_BWD(float, false);
-#undef DISTILL_BWD
+  return dtype == DABSN_BF16 ? grad<bf16>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
+                                          stats, dlogits, ldd, st)
+                             : grad<float>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
+                                           stats, dlogits, ldd, st);
+}
+
+extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
+                                 const void* logits, int64_t K, const void* list,
+                                 float temperature, const float* stats, int mean,
+                                 const float* weight, int64_t weight_stride, int unless_one,
+                                 void* dlogits, int64_t ldd, void* stream) {
+  int bad = check_distill("distill_bwd", dtype, rows, V, ld, K, temperature);
+  if (!bad) bad = check_gradient_rows("distill_bwd", dtype, rows, V, ld, logits, ldd, dlogits);
+  if (bad) return bad;
+  if (unless_one && weight_stride != 0) {
+    set_error("distill_bwd: unless_one takes one weight for all rows");
+    return DABSN_ERR_UNSUPPORTED;
+  }
+  if (rows == 0) return DABSN_OK;
+  const Entries e = entries_of(const_cast<void*>(list), rows, K);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int mb = mean ? prep_blocks(rows) : 0;
+  // a launch that mostly finds nothing to do stays one wave of CTAs
+  const unsigned grid =
+      unless_one ? (unsigned)std::min<int64_t>(rows, 148 * 8) : row_grid(rows);
+  if (dtype == DABSN_BF16)
+    distill_bwd_kernel<bf16><<<grid, DT_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const bf16*)logits, (int)K, e, mb, temperature, (const float2*)stats,
+        weight, weight_stride, unless_one != 0, (bf16*)dlogits, ldd);
+  else
+    distill_bwd_kernel<float><<<grid, DT_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const float*)logits, (int)K, e, mb, temperature, (const float2*)stats,
+        weight, weight_stride, unless_one != 0, (float*)dlogits, ldd);
   return launch_status("distill_bwd");
 }
 

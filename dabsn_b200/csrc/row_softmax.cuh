@@ -16,6 +16,7 @@
 
 #include <cfloat>
 
+#include "../../include/dabsn_b200.h"
 #include "common.cuh"
 
 namespace dabsn {
@@ -44,6 +45,36 @@ __device__ __forceinline__ float scaled_gap(float x, float m, float c) {
   return max_nan((x - m) * c, kFloor);
 }
 
+// Two FP32 lanes in one register pair: one instruction does both, which is what
+// keeps the sweeps at the memory's rate (BF16 rows arrive at 11.6 elements a
+// clock and SM; an exponential each leaves about 11 issue slots an element).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // 16-byte vectors of T.
 template <typename T>
 struct Vec;
@@ -58,39 +89,78 @@ struct Vec<bf16> {
   static constexpr unsigned kNegInf = 0xff80ff80u;
 };
 
+// The vector's elements as FP32 pairs.
 template <typename T>
-__device__ __forceinline__ void unpack(const uint4& u, float (&v)[Vec<T>::N]);
+__device__ __forceinline__ void unpack(const uint4& u, f32x2 (&v)[Vec<T>::N / 2]);
 template <>
-__device__ __forceinline__ void unpack<float>(const uint4& u, float (&v)[4]) {
-  v[0] = __uint_as_float(u.x);
-  v[1] = __uint_as_float(u.y);
-  v[2] = __uint_as_float(u.z);
-  v[3] = __uint_as_float(u.w);
+__device__ __forceinline__ void unpack<float>(const uint4& u, f32x2 (&v)[2]) {
+  v[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
+  v[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
 }
 template <>
-__device__ __forceinline__ void unpack<bf16>(const uint4& u, float (&v)[8]) {
+__device__ __forceinline__ void unpack<bf16>(const uint4& u, f32x2 (&v)[4]) {
   const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i)
+    v[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 pack(const float (&v)[Vec<T>::N]);
+__device__ __forceinline__ uint4 pack(const f32x2 (&v)[Vec<T>::N / 2]);
 template <>
-__device__ __forceinline__ uint4 pack<float>(const float (&v)[4]) {
-  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                    __float_as_uint(v[3]));
+__device__ __forceinline__ uint4 pack<float>(const f32x2 (&v)[2]) {
+  const float2 a = split(v[0]), b = split(v[1]);
+  return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x),
+                    __float_as_uint(b.y));
 }
 template <>
-__device__ __forceinline__ uint4 pack<bf16>(const float (&v)[8]) {
+__device__ __forceinline__ uint4 pack<bf16>(const f32x2 (&v)[4]) {
   uint4 u;
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = split(v[i]);
+    h[i] = __floats2bfloat162_rn(f.x, f.y);
+  }
   return u;
+}
+
+// Largest element of U vectors (NaN is passed over; the sums carry it).
+template <typename T, int U>
+__device__ __forceinline__ float vector_max(const uint4 (&raw)[U]);
+template <>
+__device__ __forceinline__ float vector_max<float, 1>(const uint4 (&r)[1]) {
+  return fmaxf(fmaxf(__uint_as_float(r[0].x), __uint_as_float(r[0].y)),
+               fmaxf(__uint_as_float(r[0].z), __uint_as_float(r[0].w)));
+}
+__device__ __forceinline__ unsigned max_bf16x2(unsigned a, unsigned b) {
+  unsigned r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned vector_max2(const uint4& u) {
+  return max_bf16x2(max_bf16x2(u.x, u.y), max_bf16x2(u.z, u.w));
+}
+__device__ __forceinline__ float pair_max(unsigned w) {
+  return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float vector_max<bf16, 1>(const uint4 (&r)[1]) {
+  return pair_max(vector_max2(r[0]));
+}
+template <>
+__device__ __forceinline__ float vector_max<float, 4>(const uint4 (&r)[4]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(r[u].x), __uint_as_float(r[u].y)),
+                       fmaxf(__uint_as_float(r[u].z), __uint_as_float(r[u].w))));
+  return m;
+}
+template <>
+__device__ __forceinline__ float vector_max<bf16, 4>(const uint4 (&r)[4]) {
+  return pair_max(max_bf16x2(max_bf16x2(vector_max2(r[0]), vector_max2(r[1])),
+                             max_bf16x2(vector_max2(r[2]), vector_max2(r[3]))));
 }
 
 // Head, vectors and tail of n elements at p.
@@ -120,12 +190,14 @@ struct Stats {
 
 __device__ __forceinline__ float finite_max(float mx) { return fmaxf(mx, -FLT_MAX); }
 
-// Moves the sums of st to a maximum mx >= st.mx.
+// Moves the sums of st to a maximum mx >= st.mx.  The products are rounded by
+// themselves (not contracted with the sums that follow), so that merging is
+// symmetric and all lanes of a butterfly end with the same bits.
 __device__ __forceinline__ void rescale(Stats& st, float mx, float c) {
   const float g = scaled_gap(finite_max(st.mx), finite_max(mx), c);
   const float f = ex2(g);
-  st.sd = f * fmaf(st.s, g, st.sd);
-  st.s *= f;
+  st.sd = __fmul_rn(f, fmaf(st.s, g, st.sd));
+  st.s = __fmul_rn(st.s, f);
   st.mx = mx;
 }
 
@@ -137,58 +209,71 @@ __device__ __forceinline__ void merge(Stats& a, Stats b, float c) {
   a.sd += b.sd;
 }
 
-template <int N>
-__device__ __forceinline__ void add_values(Stats& st, const float (&v)[N], float c) {
-  float mx = st.mx;
+// Adds one element.
+__device__ __forceinline__ void add_value(Stats& st, float x, float c) {
+  rescale(st, fmaxf(st.mx, x), c);
+  const float d = scaled_gap(x, finite_max(st.mx), c);
+  const float e = ex2(d);
+  st.s += e;
+  st.sd = fmaf(e, d, st.sd);
+}
+
+// Adds U vectors, moving the sums to a new maximum once.  SD: with the sum that
+// the entropy needs (without it -inf needs no clamp: 2^-inf is 0).
+template <typename T, int U, bool SD>
+__device__ __forceinline__ void add_vectors(Stats& st, const uint4 (&raw)[U], float c) {
+  constexpr int P = Vec<T>::N / 2;
+  rescale(st, fmaxf(st.mx, vector_max<T, U>(raw)), c);
+  const float m = finite_max(st.mx);
+  const f32x2 m2 = pair(-m, -m), c2 = pair(c, c);
+  f32x2 s2 = pair(st.s, 0.f), sd2 = pair(st.sd, 0.f);
 #pragma unroll
-  for (int i = 0; i < N; ++i) mx = fmaxf(mx, v[i]);
-  rescale(st, mx, c);
-  const float m = finite_max(mx);
+  for (int u = 0; u < U; ++u) {
+    f32x2 v[P];
+    unpack<T>(raw[u], v);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = scaled_gap(v[i], m, c);
-    const float e = ex2(d);
-    st.s += e;
-    st.sd = fmaf(e, d, st.sd);
+    for (int i = 0; i < P; ++i) {
+      float2 d = split(mul2(add2(v[i], m2), c2));
+      if (SD) {
+        d.x = max_nan(d.x, kFloor);
+        d.y = max_nan(d.y, kFloor);
+      }
+      const f32x2 e = pair(ex2(d.x), ex2(d.y));
+      s2 = add2(s2, e);
+      if (SD) sd2 = fma2(e, pair(d.x, d.y), sd2);
+    }
   }
+  const float2 s = split(s2), sd = split(sd2);
+  st.s = s.x + s.y;
+  if (SD) st.sd = sd.x + sd.y;
 }
 
 // The part of a row of n elements that belongs to thread `t` of THREADS:
 // vectors t, t + THREADS, ...; one head and one tail element for the first
 // threads.  Four vectors are in flight at a time.
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool SD>
 __device__ __forceinline__ Stats sweep(const T* p, int n, int t, float c) {
-  constexpr int VW = Vec<T>::N, U = 4;
+  constexpr int U = 4;
   const RowShape r = row_shape(p, n);
   const uint4* pv = reinterpret_cast<const uint4*>(p + r.head);
   Stats st;
-  for (int i = t; i < r.nv; i += THREADS * U) {
+  int i = t;
+  for (; i + (U - 1) * THREADS < r.nv; i += THREADS * U) {
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = i + u * THREADS;
-      constexpr unsigned ni = Vec<T>::kNegInf;
-      raw[u] = k < r.nv ? __ldg(pv + k) : make_uint4(ni, ni, ni, ni);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[VW];
-      unpack<T>(raw[u], v);
-      add_values<VW>(st, v, c);
-    }
+    for (int u = 0; u < U; ++u) raw[u] = __ldg(pv + i + u * THREADS);
+    add_vectors<T, U, SD>(st, raw, c);
   }
-  float edge[2] = {-INFINITY, -INFINITY};
-  if (t < r.head) edge[0] = to_f<T>(p[t]);
-  if (t < r.tail) edge[1] = to_f<T>(p[r.tail0 + t]);
-  add_values<2>(st, edge, c);
+  for (; i < r.nv; i += THREADS) {
+    const uint4 raw[1] = {__ldg(pv + i)};
+    add_vectors<T, 1, SD>(st, raw, c);
+  }
+  if (t < r.head) add_value(st, to_f<T>(p[t]), c);
+  if (t < r.tail) add_value(st, to_f<T>(p[r.tail0 + t]), c);
   return st;
 }
 
-// Merges the threads' statistics of a CTA in a fixed order; every thread gets
-// the result.  `sh` holds three floats a warp.  Ends with a barrier before the
-// next use of `sh` being the caller's business.
-template <int THREADS>
-__device__ __forceinline__ Stats block_merge(Stats st, float (*sh)[3], float c) {
+__device__ __forceinline__ Stats warp_merge(Stats st, float c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Stats b;
@@ -197,6 +282,15 @@ __device__ __forceinline__ Stats block_merge(Stats st, float (*sh)[3], float c) 
     b.sd = __shfl_xor_sync(0xffffffffu, st.sd, o);
     merge(st, b, c);
   }
+  return st;
+}
+
+// Merges the threads' statistics of a CTA in a fixed order; every thread gets
+// the result.  `sh` holds three floats a warp.  Ends with a barrier before the
+// next use of `sh` being the caller's business.
+template <int THREADS>
+__device__ __forceinline__ Stats block_merge(Stats st, float (*sh)[3], float c) {
+  st = warp_merge(st, c);
   const int warp = threadIdx.x >> 5;
   if ((threadIdx.x & 31) == 0) {
     sh[warp][0] = st.mx;
@@ -228,19 +322,33 @@ __device__ __forceinline__ float grad_value(float x, float m, float c, float A, 
   return ex2((x - m) * c) * A;
 }
 
-// Whether 16-byte vectors of a logits row and of its gradient row start at the
-// same element in every row (else the gradient is stored by element).
-inline bool same_phase(const void* x, long long ld, const void* dx, long long ldd, size_t size) {
-  return ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15u) == 0 &&
-         (((ld - ldd) * (long long)size) & 15) == 0;
+template <typename T, bool HAS_B>
+__device__ __forceinline__ uint4 grad_vector(const uint4& raw, f32x2 m2, f32x2 c2, f32x2 A2,
+                                             f32x2 B2) {
+  constexpr int P = Vec<T>::N / 2;
+  f32x2 v[P];
+  unpack<T>(raw, v);
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    float2 d = split(mul2(add2(v[i], m2), c2));
+    if (HAS_B) {
+      d.x = max_nan(d.x, kFloor);
+      d.y = max_nan(d.y, kFloor);
+    }
+    const f32x2 e = pair(ex2(d.x), ex2(d.y));
+    v[i] = mul2(e, HAS_B ? fma2(B2, pair(d.x, d.y), A2) : A2);
+  }
+  return pack<T>(v);
 }
 
-template <typename T, int THREADS, bool HAS_B, bool SAME>
+template <typename T, int THREADS, bool HAS_B>
 __device__ __forceinline__ void grad_sweep(const T* p, T* q, int n, int t, float m, float c,
                                            float A, float B) {
-  constexpr int VW = Vec<T>::N, U = 4;
+  constexpr int U = 4;
   const RowShape r = row_shape(p, n);
   const uint4* pv = reinterpret_cast<const uint4*>(p + r.head);
+  uint4* qv = reinterpret_cast<uint4*>(q + r.head);
+  const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), A2 = pair(A, A), B2 = pair(B, B);
   for (int i = t; i < r.nv; i += THREADS * U) {
     uint4 raw[U];
 #pragma unroll
@@ -250,17 +358,7 @@ __device__ __forceinline__ void grad_sweep(const T* p, T* q, int n, int t, float
     for (int u = 0; u < U; ++u) {
       const int k = i + u * THREADS;
       if (k >= r.nv) break;
-      float v[VW];
-      unpack<T>(raw[u], v);
-#pragma unroll
-      for (int j = 0; j < VW; ++j) v[j] = grad_value<HAS_B>(v[j], m, c, A, B);
-      T* dst = q + r.head + (size_t)k * VW;
-      if (SAME) {
-        *reinterpret_cast<uint4*>(dst) = pack<T>(v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VW; ++j) dst[j] = from_f<T>(v[j]);
-      }
+      qv[k] = grad_vector<T, HAS_B>(raw[u], m2, c2, A2, B2);
     }
   }
   if (t < r.head) q[t] = from_f<T>(grad_value<HAS_B>(to_f<T>(p[t]), m, c, A, B));
@@ -275,6 +373,24 @@ __device__ __forceinline__ void zero_row(T* q, int n, int t) {
   for (int i = t; i < r.nv; i += THREADS) qv[i] = make_uint4(0u, 0u, 0u, 0u);
   if (t < r.head) q[t] = from_f<T>(0.f);
   if (t < r.tail) q[r.tail0 + t] = from_f<T>(0.f);
+}
+
+// The gradient kernels store the vectors they loaded, so a gradient row starts
+// at the 16-byte phase of its logits row.
+inline int check_gradient_rows(const char* what, int dtype, int64_t rows, int64_t V, int64_t ld,
+                               const void* x, int64_t ldd, const void* dx) {
+  const int64_t size = dtype == DABSN_BF16 ? 2 : 4;
+  if (ldd < V) {
+    set_error("%s: gradient rows %lld apart overlap (V=%lld)", what, (long long)ldd,
+              (long long)V);
+    return DABSN_ERR_SHAPE;
+  }
+  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15u) != 0 ||
+      (rows > 1 && ((ld - ldd) * size & 15) != 0)) {
+    set_error("%s: gradient rows must start at the 16-byte phase of the logits rows", what);
+    return DABSN_ERR_UNSUPPORTED;
+  }
+  return DABSN_OK;
 }
 
 }  // namespace rowsm

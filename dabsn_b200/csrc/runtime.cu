@@ -117,5 +117,15 @@ extern "C" int dabsn_device_status(int reset) {
   return v;
 }
 
+extern "C" uint64_t dabsn_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 extern "C" const char* dabsn_version(void) { return "dabsn_b200 0.1.0 (sm_100a)"; }
 extern "C" const char* dabsn_last_error(void) { return g_last_error; }

@@ -99,10 +99,14 @@ __device__ __forceinline__ void offer_parts(TopkShared& sh, unsigned bound, cons
   for (int e = threadIdx.x; e < n_hot * per; e += TS_THREADS) {
     const int k = sh.hot[e / per] + (e % per) * TS_THREADS;
     if (k >= r.nv) continue;
-    float v[VW];
+    f32x2 v[VW / 2];
     unpack<T>(__ldg(pv + k), v);
 #pragma unroll
-    for (int j = 0; j < VW; ++j) offer(sh, bound, v[j], r.head + k * VW + j);
+    for (int j = 0; j < VW / 2; ++j) {
+      const float2 x = split(v[j]);
+      offer(sh, bound, x.x, r.head + k * VW + 2 * j);
+      offer(sh, bound, x.y, r.head + k * VW + 2 * j + 1);
+    }
   }
   for (int e = threadIdx.x; e < n_hot; e += TS_THREADS) {
     const int t = sh.hot[e];
@@ -197,6 +201,29 @@ __device__ __forceinline__ void store_top(const TopkShared& sh, int k, float m, 
   }
 }
 
+// One thread: the numbers of a row from its merged statistics.
+template <typename T>
+__device__ __forceinline__ void write_scores(const Stats& all, const T* row, long long t, int V,
+                                             bool ignored, float inv_t, float* log_prob,
+                                             float* entropy, float2* stats, int* status) {
+  const float m = finite_max(all.mx);
+  float lp = 0.f, h = 0.f;
+  if (!ignored) {
+    const float log_s = logf(all.s);
+    const bool empty = all.s == 0.f;
+    if (!empty) h = fmaf(-kLn2, all.sd / all.s, log_s);
+    if (t < 0 || t >= V) {
+      lp = __int_as_float(0x7fc00000);
+      if (status) atomicExch(status, STATUS_BAD_TOKEN);
+    } else {
+      lp = empty ? -INFINITY : (to_f<T>(row[t]) - m) * inv_t - log_s;
+    }
+  }
+  *log_prob = lp;
+  *entropy = h;
+  if (stats) *stats = make_float2(m, all.s);
+}
+
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits,
@@ -209,11 +236,9 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const long long t = tokens[r];
     if (t == ignore_index) {
-      if (threadIdx.x == 0) {
-        log_prob[r] = 0.f;
-        entropy[r] = 0.f;
-        if (stats) stats[r] = make_float2(0.f, 0.f);
-      }
+      if (threadIdx.x == 0)
+        write_scores(Stats(), logits, t, V, true, inv_t, log_prob + r, entropy + r,
+                     stats ? stats + r : nullptr, status);
       if (TOP)
         for (int i = threadIdx.x; i < k; i += TS_THREADS) {
           top_values[r * k + i] = -INFINITY;
@@ -222,54 +247,62 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
       continue;
     }
     const T* row = logits + (size_t)r * ld;
-    const Stats own = sweep<T, TS_THREADS>(row, V, threadIdx.x, c);
+    const Stats own = sweep<T, TS_THREADS, true>(row, V, threadIdx.x, c);
     const Stats all = block_merge<TS_THREADS>(own, part, c);
-    const float m = finite_max(all.mx);
-    const bool empty = all.s == 0.f;
-    const float log_s = logf(all.s);
-    if (threadIdx.x == 0) {
-      float lp, h;
-      if (empty) {
-        lp = -INFINITY;
-        h = 0.f;
-      } else {
-        h = fmaf(-kLn2, all.sd / all.s, log_s);
-        lp = 0.f;
-      }
-      if (t < 0 || t >= V) {
-        lp = __int_as_float(0x7fc00000);
-        if (status) atomicExch(status, STATUS_BAD_TOKEN);
-      } else if (!empty) {
-        lp = (to_f<T>(row[t]) - m) * inv_t - log_s;
-      }
-      log_prob[r] = lp;
-      entropy[r] = h;
-      if (stats) stats[r] = make_float2(m, all.s);
-    }
+    if (threadIdx.x == 0)
+      write_scores(all, row, t, V, false, inv_t, log_prob + r, entropy + r,
+                   stats ? stats + r : nullptr, status);
     if (TOP) {
       select_top<T>(top, row, V, k, own.mx);
-      store_top(top, k, m, inv_t, log_s, empty, top_values + r * k, top_ids + r * k);
+      store_top(top, k, finite_max(all.mx), inv_t, logf(all.s), all.s == 0.f,
+                top_values + r * k, top_ids + r * k);
     }
     __syncthreads();
   }
 }
 
-template <typename T, bool HAS_B, bool SAME>
+// Rows short enough for one warp: eight a CTA, no barriers.
+constexpr int TS_WARP_BYTES = 2048;
+
+template <typename T>
+__global__ void __launch_bounds__(TS_THREADS) token_scores_warp_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits,
+    const int64_t* __restrict__ tokens, long long ignore_index, float inv_t,
+    float* __restrict__ log_prob, float* __restrict__ entropy, float2* __restrict__ stats,
+    int* status) {
+  const int lane = threadIdx.x & 31;
+  const long long r = (long long)blockIdx.x * (TS_THREADS / 32) + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const float c = kLog2e * inv_t;
+  const long long t = tokens[r];
+  Stats all;
+  const T* row = logits + (size_t)r * ld;
+  if (t != ignore_index) all = warp_merge(sweep<T, 32, true>(row, V, lane, c), c);
+  if (lane == 0)
+    write_scores(all, row, t, V, t == ignore_index, inv_t, log_prob + r, entropy + r,
+                 stats ? stats + r : nullptr, status);
+}
+
+// A row to every THREADS threads (a warp or the CTA).
+template <typename T, int THREADS, bool HAS_B>
 __global__ void __launch_bounds__(TS_THREADS) token_scores_bwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits,
     const int64_t* __restrict__ tokens, long long ignore_index, float inv_t,
     const float2* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ g_log_prob, const float* __restrict__ g_entropy,
-    T* __restrict__ dlogits) {
+    T* __restrict__ dlogits, long long ldd) {
+  constexpr int GROUPS = TS_THREADS / THREADS;
   const float c = kLog2e * inv_t;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
+  const int lane = threadIdx.x % THREADS;
+  for (long long r = (long long)blockIdx.x * GROUPS + threadIdx.x / THREADS; r < rows;
+       r += (long long)gridDim.x * GROUPS) {
     const T* row = logits + (size_t)r * ld;
-    T* drow = dlogits + (size_t)r * V;
+    T* drow = dlogits + (size_t)r * ldd;
     const long long t = tokens[r];
     const float2 ms = stats[r];
     if (t == ignore_index || ms.y == 0.f) {
       // padding, or a row with every logit masked: nothing to learn
-      zero_row<T, TS_THREADS>(drow, V, threadIdx.x);
+      zero_row<T, THREADS>(drow, V, lane);
       continue;
     }
     const float g = g_log_prob ? g_log_prob[r] * inv_t : 0.f;
@@ -277,10 +310,14 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_bwd_kernel(
     // p_j (log p_j + entropy) = 2^d_j (d_j ln2 - log s + entropy) / s
     const float B = HAS_B ? -h * kLn2 / ms.y : 0.f;
     const float A = -(HAS_B ? fmaf(h, entropy[r] - logf(ms.y), g) : g) / ms.y;
-    grad_sweep<T, TS_THREADS, HAS_B, SAME>(row, drow, V, threadIdx.x, ms.x, c, A, B);
+    grad_sweep<T, THREADS, HAS_B>(row, drow, V, lane, ms.x, c, A, B);
     if (t >= 0 && t < V) {
-      __syncthreads();  // the token's element is rounded once, with its own term
-      if (threadIdx.x == 0)
+      // the token's element is rounded once, with its own term
+      if (THREADS == 32)
+        __syncwarp();
+      else
+        __syncthreads();
+      if (lane == 0)
         drow[t] = from_f<T>(grad_value<HAS_B>(to_f<T>(row[t]), ms.x, c, A, B) + g);
     }
   }
@@ -288,6 +325,10 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_bwd_kernel(
 
 unsigned row_grid(long long rows) {
   return (unsigned)std::min<long long>(rows, 0x7fffffffLL);
+}
+
+unsigned warp_grid(long long rows) {
+  return row_grid((rows + TS_THREADS / 32 - 1) / (TS_THREADS / 32));
 }
 
 int check_rows(const char* what, int dtype, int64_t rows, int64_t V, int64_t ld,
@@ -314,14 +355,17 @@ int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
                float* entropy, float* stats, float* top_values, int64_t* top_ids,
                cudaStream_t st) {
   const float inv_t = 1.f / temperature;
-  const unsigned grid = row_grid(rows);
   int* status = device_status();
   if (k > 0)
-    token_scores_fwd_kernel<T, true><<<grid, TS_THREADS, 0, st>>>(
+    token_scores_fwd_kernel<T, true><<<row_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (int)k, log_prob,
         entropy, (float2*)stats, top_values, top_ids, status);
+  else if (V * sizeof(T) <= TS_WARP_BYTES)
+    token_scores_warp_kernel<T><<<warp_grid(rows), TS_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
+        (float2*)stats, status);
   else
-    token_scores_fwd_kernel<T, false><<<grid, TS_THREADS, 0, st>>>(
+    token_scores_fwd_kernel<T, false><<<row_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, 0, log_prob, entropy,
         (float2*)stats, nullptr, nullptr, status);
   return launch_status("token_scores_fwd");
@@ -330,18 +374,17 @@ int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
 template <typename T, bool HAS_B>
 int launch_bwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const int64_t* tokens,
                int64_t ignore_index, float temperature, const float* stats, const float* entropy,
-               const float* g_log_prob, const float* g_entropy, void* dlogits,
+               const float* g_log_prob, const float* g_entropy, void* dlogits, int64_t ldd,
                cudaStream_t st) {
   const float inv_t = 1.f / temperature;
-  const unsigned grid = row_grid(rows);
-  if (same_phase(logits, ld, dlogits, V, sizeof(T)))
-    token_scores_bwd_kernel<T, HAS_B, true><<<grid, TS_THREADS, 0, st>>>(
+  if (V * sizeof(T) <= TS_WARP_BYTES)
+    token_scores_bwd_kernel<T, 32, HAS_B><<<warp_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (const float2*)stats,
-        entropy, g_log_prob, g_entropy, (T*)dlogits);
+        entropy, g_log_prob, g_entropy, (T*)dlogits, ldd);
   else
-    token_scores_bwd_kernel<T, HAS_B, false><<<grid, TS_THREADS, 0, st>>>(
+    token_scores_bwd_kernel<T, TS_THREADS, HAS_B><<<row_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (const float2*)stats,
-        entropy, g_log_prob, g_entropy, (T*)dlogits);
+        entropy, g_log_prob, g_entropy, (T*)dlogits, ldd);
   return launch_status("token_scores_bwd");
 }
 
@@ -376,22 +419,24 @@ extern "C" int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_
                                       int64_t ignore_index, float temperature,
                                       const float* stats, const float* entropy,
                                       const float* g_log_prob, const float* g_entropy,
-                                      void* dlogits, void* stream) {
-  const int bad = check_rows("token_scores_bwd", dtype, rows, V, ld, temperature);
+                                      void* dlogits, int64_t ldd, void* stream) {
+  int bad = check_rows("token_scores_bwd", dtype, rows, V, ld, temperature);
+  if (!bad)
+    bad = check_gradient_rows("token_scores_bwd", dtype, rows, V, ld, logits, ldd, dlogits);
   if (bad) return bad;
   if (rows == 0) return DABSN_OK;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == DABSN_BF16)
     return g_entropy ? launch_bwd<bf16, true>(rows, V, ld, logits, tokens, ignore_index,
                                               temperature, stats, entropy, g_log_prob, g_entropy,
-                                              dlogits, st)
+                                              dlogits, ldd, st)
                      : launch_bwd<bf16, false>(rows, V, ld, logits, tokens, ignore_index,
                                                temperature, stats, entropy, g_log_prob,
-                                               g_entropy, dlogits, st);
+                                               g_entropy, dlogits, ldd, st);
   return g_entropy ? launch_bwd<float, true>(rows, V, ld, logits, tokens, ignore_index,
                                              temperature, stats, entropy, g_log_prob, g_entropy,
-                                             dlogits, st)
+                                             dlogits, ldd, st)
                    : launch_bwd<float, false>(rows, V, ld, logits, tokens, ignore_index,
                                               temperature, stats, entropy, g_log_prob, g_entropy,
-                                              dlogits, st);
+                                              dlogits, ldd, st);
 }

@@ -882,6 +882,21 @@ def _logit_rows(logits: Tensor) -> tuple[int, int, int]:
     return rows, V, (logits.stride(0) if rows > 1 else V)
 
 
+def _gradient_rows(logits: Tensor, ld: int) -> tuple[Tensor, int]:
+    """An uninitialised gradient of the logits' shape and dtype, and its row
+    stride.  Its rows start at the 16-byte phase of the logits rows, so that
+    the kernels store the vectors they load: contiguous unless the logits start
+    or step off that phase (a view of a padded readout)."""
+    rows, V = logits.shape
+    per = 16 // logits.element_size()
+    first = logits.data_ptr() % 16 // logits.element_size()
+    ldd = V + (ld - V) % per
+    if first == 0 and ldd == V:
+        return torch.empty((rows, V), device=logits.device, dtype=logits.dtype), V
+    store = torch.empty(first + rows * ldd, device=logits.device, dtype=logits.dtype)
+    return store.as_strided((rows, V), (ldd, 1), first), ldd
+
+
 def _temperature(temperature: float) -> float:
     t = float(temperature)
     if not (0.0 < t < float("inf")) or not ctypes.c_float(1.0 / t).value < float("inf"):
@@ -938,10 +953,10 @@ def token_scores_backward(logits: Tensor, tokens: Tensor, temperature: float, ig
     rows, V, ld = _logit_rows(logits)
     tokens = _int_rows(tokens, (rows,), "tokens")
     g, h = _dense_f32(grad_log_prob), _dense_f32(grad_entropy)
-    dl = torch.empty((rows, V), device=dev, dtype=logits.dtype)
+    dl, ldd = _gradient_rows(logits, ld)
     _run("token_scores_bwd", dev, N.load().dabsn_token_scores_bwd, act_code(logits.dtype), rows,
          V, ld, logits.data_ptr(), tokens.data_ptr(), ignore_index, _temperature(temperature),
-         stats.data_ptr(), entropy.data_ptr(), _addr(g), _addr(h), dl.data_ptr())
+         stats.data_ptr(), entropy.data_ptr(), _addr(g), _addr(h), dl.data_ptr(), ldd)
     return dl
 
 
@@ -991,18 +1006,47 @@ def distill_reduce(row_loss: Tensor, lists: Tensor, entries: int, mean: bool) ->
     return out
 
 
+def distill_gradient(logits: Tensor, lists: Tensor, entries: int, temperature: float,
+                     mean: bool):
+    """Row losses, statistics and the logits' gradient for the sum (the mean if
+    ``mean``) of the losses, in one pass over the logits; None where a row is
+    too long for it (then :func:`distill_forward` and
+    :func:`distill_backward`)."""
+    dev = _same_cuda(logits, lists)
+    rows, V, ld = _logit_rows(logits)
+    code, lib = act_code(logits.dtype), N.load()
+    if not lib.dabsn_distill_grad_fits(code, rows, V):
+        return None
+    loss = torch.empty(rows, device=dev, dtype=torch.float32)
+    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    dl, ldd = _gradient_rows(logits, ld)
+    _run("distill_grad", dev, lib.dabsn_distill_grad, code, rows, V, ld, logits.data_ptr(),
+         entries, lists.data_ptr(), _temperature(temperature), int(mean), loss.data_ptr(),
+         stats.data_ptr(), dl.data_ptr(), ldd)
+    return loss, stats, dl
+
+
 def distill_backward(logits: Tensor, lists: Tensor, entries: int, temperature: float,
-                     stats: Tensor, mean: bool, weight: Tensor) -> Tensor:
+                     stats: Tensor, mean: bool, weight: Tensor,
+                     ready: Tensor | None = None) -> Tensor:
     """dlogits [rows, V] for row weights ``weight`` ([rows], or [] for all
-    rows), divided by the number of rows with a loss if ``mean``."""
+    rows), divided by the number of rows with a loss if ``mean``.  ``ready``
+    holds the gradient for weight 1; it is returned, and written again where
+    the (one) weight is another."""
     dev = _same_cuda(logits, lists, stats, weight)
     rows, V, ld = _logit_rows(logits)
     w = _dense_f32(weight)
-    dl = torch.empty((rows, V), device=dev, dtype=logits.dtype)
+    dl, ldd = _gradient_rows(logits, ld) if ready is None else (ready, _logit_rows(ready)[2])
     _run("distill_bwd", dev, N.load().dabsn_distill_bwd, act_code(logits.dtype), rows, V, ld,
          logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature),
-         stats.data_ptr(), int(mean), w.data_ptr(), int(w.dim() > 0), dl.data_ptr())
+         stats.data_ptr(), int(mean), w.data_ptr(), int(w.dim() > 0), int(ready is not None),
+         dl.data_ptr(), ldd)
     return dl
+
+
+def capture_id(device: torch.device) -> int:
+    """Identity of the CUDA graph capture that the current stream is in (0: none)."""
+    return N.load().dabsn_capture_id(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def embedding_forward(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) -> Tensor:

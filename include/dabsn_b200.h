@@ -484,6 +484,9 @@ int dabsn_read_wide_bwd(int64_t B, int64_t T, int64_t N, int64_t H, int mode,
                         void* dnext, float* dbias, float* dbank_cocktail, float* rowpart,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* Identity of the CUDA graph capture that `stream` is in (0: none). */
+uint64_t dabsn_capture_id(void* stream);
+
 /* Log-probabilities of given tokens, with entropy and top alternatives.
  *   logits [rows, V] FP32/BF16, rows contiguous and `ld` elements apart, any
  *   alignment; tokens [rows] int64 (rows of ignore_index are not read);
@@ -491,8 +494,9 @@ int dabsn_read_wide_bwd(int64_t B, int64_t T, int64_t N, int64_t H, int mode,
  *   log_prob, entropy [rows] FP32; stats FP32 [rows, 2] (maximum, sum of
  *   exponentials; for the reverse, may be null); top_values FP32 and top_ids
  *   int64 [rows, top_k], most likely first, equal logits by the lower id.
- * Reverse: dlogits [rows, V] contiguous, in the logits' dtype, for gradients
- * of log_prob and entropy (FP32 [rows], either may be null).
+ * Reverse: dlogits [rows, V] in the logits' dtype, rows `ldd` elements apart
+ * and at the 16-byte phase of the logits rows, for gradients of log_prob and
+ * entropy (FP32 [rows], either may be null).
  * A token outside [0, V) gives NaN and device status 8. */
 int dabsn_token_scores_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                            const int64_t* tokens, int64_t ignore_index, float temperature,
@@ -501,7 +505,7 @@ int dabsn_token_scores_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
 int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                            const int64_t* tokens, int64_t ignore_index, float temperature,
                            const float* stats, const float* entropy, const float* g_log_prob,
-                           const float* g_entropy, void* dlogits, void* stream);
+                           const float* g_entropy, void* dlogits, int64_t ldd, void* stream);
 
 /* Distillation from a teacher's top logits: temperature^2 KL(q || softmax(
  * logits / temperature)), q the softmax of the teacher's logits over the
@@ -512,8 +516,12 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  *   fwd: row_loss [rows], stats [rows, 2] FP32 (stats for the reverse, may be
  *   null).  reduce: result FP32 [1], the sum of the row losses, divided by the
  *   number of rows that list anything if `mean`.
- *   bwd: dlogits [rows, V] contiguous, in the logits' dtype, for row weights
- *   weight[r * weight_stride], divided by the same number if `mean`. */
+ *   bwd: dlogits [rows, V] in the logits' dtype, rows `ldd` elements apart and
+ *   at the 16-byte phase of the logits rows, for row weights weight[r *
+ *   weight_stride], divided by the same number if `mean`; `unless_one` (one
+ *   weight for all rows): dlogits holds the gradient for weight 1 already.
+ *   grad: fwd, and the gradient for weight 1, in one pass over the logits, for
+ *   rows that dabsn_distill_grad_fits. */
 size_t dabsn_distill_list_bytes(int64_t rows, int64_t K);
 int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
                        const int64_t* teacher_tokens, const void* teacher_logits,
@@ -521,10 +529,14 @@ int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
 int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int64_t K, const void* list, float temperature, float* row_loss,
                       float* stats, void* stream);
+int dabsn_distill_grad_fits(int dtype, int64_t rows, int64_t V);
+int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
+                       int64_t K, const void* list, float temperature, int mean,
+                       float* row_loss, float* stats, void* dlogits, int64_t ldd, void* stream);
 int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int64_t K, const void* list, float temperature, const float* stats,
-                      int mean, const float* weight, int64_t weight_stride, void* dlogits,
-                      void* stream);
+                      int mean, const float* weight, int64_t weight_stride, int unless_one,
+                      void* dlogits, int64_t ldd, void* stream);
 int dabsn_distill_reduce(int64_t rows, int64_t K, const float* row_loss, const void* list,
                          int mean, float* result, void* stream);
 

@@ -85,7 +85,18 @@ def test_entry_points_check_sizes_before_launching():
     assert distill(K=0) and distill(K=257) and distill(dtype=7) and distill(t=float("inf"))
     assert lib.dabsn_distill_prep(0, 4, 0, 2, NULL, NULL, f(1.0), -100, NULL, NULL)
     assert lib.dabsn_distill_reduce(-1, 2, NULL, NULL, 1, NULL, NULL)
-    assert lib.dabsn_distill_bwd(0, 4, 10, 9, NULL, 2, NULL, f(1.0), NULL, 1, NULL, 0, NULL, NULL)
+    def reverse(ld=10, ldd=10, x=0, dx=0, unless_one=0, stride=0):
+        return lib.dabsn_distill_bwd(0, 4, 10, ld, x, 2, NULL, f(1.0), NULL, 1, NULL, stride,
+                                     unless_one, dx, ldd, NULL)
+
+    assert reverse(ld=9) and reverse(ldd=9) and reverse(ldd=11) and reverse(x=16, dx=4)
+    assert reverse(unless_one=1, stride=1)
+    assert lib.dabsn_distill_grad(0, 4, 10, 10, 16, 2, NULL, f(1.0), 1, NULL, NULL, 8, 10, NULL)
+    assert b"phase" in lib.dabsn_last_error()
+    assert lib.dabsn_token_scores_bwd(0, 4, 10, 10, 16, NULL, -100, f(1.0), *([NULL] * 4), 4, 10,
+                                      NULL)
+    assert lib.dabsn_distill_grad_fits(1, 32768, 32000) and not lib.dabsn_distill_grad_fits(
+        0, 4, 700000)
 
     def lookup(w=0, o=0, N=4, V=10, D=8, ldw=8):
         return lib.dabsn_embedding_fwd(w, o, N, V, D, NULL, NULL, ldw, f(1.0), NULL, NULL)
