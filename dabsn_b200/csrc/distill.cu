@@ -365,6 +365,21 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
                : "memory");
 }
 
+// Waits until at most `pending` of this thread's latest groups of copies are
+// under way (more strictly where that is over 7).
+__device__ __forceinline__ void cp_async_wait_for(int pending) {
+  switch (pending) {
+    case 0: cp_async_wait<0>(); break;
+    case 1: cp_async_wait<1>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 3: cp_async_wait<3>(); break;
+    case 4: cp_async_wait<4>(); break;
+    case 5: cp_async_wait<5>(); break;
+    case 6: cp_async_wait<6>(); break;
+    default: cp_async_wait<7>(); break;
+  }
+}
+
 template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
@@ -381,6 +396,11 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
   const int a = min(rank * share, V), n = min(share, V - a);
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
   const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
+  // Vectors of a row at most (rows of other alignments have one less).  Copies
+  // are committed in groups of four vectors a thread, as many for every row, so
+  // that the statistics start on the first while the last are under way.
+  const int most = n / Vec<T>::N;
+  const int groups = (most + 4 * DF_THREADS - 1) / (4 * DF_THREADS);
 
   // The next row from r on that has a loss; the others' gradient is zero.
   auto next_live = [&](long long r) {
@@ -404,11 +424,17 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
   if (r < rows) {
     const T* p = logits + (size_t)r * ld + a;
     const RowShape s = row_shape(p, n);
-    for (int k = t; k < s.nv; k += DF_THREADS)
-      cp_async16(&slots[k], reinterpret_cast<const uint4*>(p + s.head) + k);
+    const uint4* v = reinterpret_cast<const uint4*>(p + s.head);
+    for (int k0 = 0; k0 < most; k0 += 4 * DF_THREADS) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = k0 + u * DF_THREADS + t;
+        if (k < s.nv) cp_async16(&slots[k], v + k);
+      }
+      cp_async_commit();
+    }
     load_edges(p, s);
   }
-  cp_async_commit();
   if (SPLIT) cluster_sync_all();  // every CTA runs before another writes to it
   for (int turn = 0; r < rows; turn ^= 1) {
     const T* row = logits + (size_t)r * ld;
@@ -421,22 +447,23 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
       q = list.q[r * K + t];
       if (id >= 0) x = to_f<T>(row[id]);
     }
-    cp_async_wait<0>();
     Stats st;
-    {
-      int k = t;
-      for (; k + 3 * DF_THREADS < s.nv; k += 4 * DF_THREADS) {
+    for (int g = 0; g < groups; ++g) {
+      cp_async_wait_for(groups - 1 - g);
+      const int k = g * 4 * DF_THREADS + t;
+      if (k + 3 * DF_THREADS < s.nv) {
         const uint4 raw[4] = {slots[k], slots[k + DF_THREADS], slots[k + 2 * DF_THREADS],
                               slots[k + 3 * DF_THREADS]};
         add_vectors<T, 4, false>(st, raw, c);
+      } else {
+        for (int i = k; i < s.nv; i += DF_THREADS) {
+          const uint4 raw[1] = {slots[i]};
+          add_vectors<T, 1, false>(st, raw, c);
+        }
       }
-      for (; k < s.nv; k += DF_THREADS) {
-        const uint4 raw[1] = {slots[k]};
-        add_vectors<T, 1, false>(st, raw, c);
-      }
-      if (t < s.head) add_value(st, edge[0], c);
-      if (t < s.tail) add_value(st, edge[1], c);
     }
+    if (t < s.head) add_value(st, edge[0], c);
+    if (t < s.tail) add_value(st, edge[1], c);
     st.sd = 0.f;
     st = block_merge<DF_THREADS>(st, part, c);
     if (SPLIT) {
@@ -447,14 +474,12 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
       }
       __syncwarp();
       cluster_sync_all();
-      Stats all;
-      for (int o = 0; o < cl; ++o) {
-        Stats b;
-        b.mx = peer[turn][o][0];
-        b.s = peer[turn][o][1];
-        merge(all, b, c);
+      Stats other;  // empty for lanes past the cluster
+      if ((t & 7) < cl) {
+        other.mx = peer[turn][t & 7][0];
+        other.s = peer[turn][t & 7][1];
       }
-      st = all;
+      st = warp_merge<8>(other, c);
     }
     const float m = finite_max(st.mx);
     const bool empty = st.s == 0.f;
@@ -478,19 +503,26 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     uint4* dv = reinterpret_cast<uint4*>(drow + a + s.head);
     {
       const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), A2 = pair(A, A);
-      // rows of other alignments differ by a vector at most
-      const int most = max(s.nv, sn.nv);
-      for (int k = t; k < most; k += 4 * DF_THREADS) {
-        uint4 raw[4];
+      const int least = min(s.nv, sn.nv);
+      for (int g = 0; g < groups; ++g) {
+        const int k = g * 4 * DF_THREADS + t;
+        if (k + 3 * DF_THREADS < least) {
+          uint4 raw[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (k + u * DF_THREADS < s.nv) raw[u] = slots[k + u * DF_THREADS];
+          for (int u = 0; u < 4; ++u) raw[u] = slots[k + u * DF_THREADS];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = k + u * DF_THREADS;
-          if (i < s.nv) dv[i] = grad_vector<T, false>(raw[u], m2, c2, A2, A2);
-          if (i < sn.nv) cp_async16(&slots[i], nv + i);
+          for (int u = 0; u < 4; ++u) {
+            const int i = k + u * DF_THREADS;
+            dv[i] = grad_vector<T, false>(raw[u], m2, c2, A2, A2);
+            cp_async16(&slots[i], nv + i);
+          }
+        } else {
+          for (int i = k; i < min(k + 4 * DF_THREADS, most); i += DF_THREADS) {
+            if (i < s.nv) dv[i] = grad_vector<T, false>(slots[i], m2, c2, A2, A2);
+            if (i < sn.nv) cp_async16(&slots[i], nv + i);
+          }
         }
+        cp_async_commit();
       }
       if (t < s.head)
         drow[a + t] = from_f<T>(grad_value<false>(edge[0], m, c, A, 0.f));
@@ -498,7 +530,6 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
         drow[a + s.tail0 + t] = from_f<T>(grad_value<false>(edge[1], m, c, A, 0.f));
       load_edges(pn, sn);
     }
-    cp_async_commit();
     __syncthreads();  // listed elements are rounded once, with their own term
     if (id >= a && id < a + n && q.y > 0.f && !empty)
       drow[id] = from_f<T>(fmaf(-w, q.y, grad_value<false>(x, m, c, A, 0.f)));

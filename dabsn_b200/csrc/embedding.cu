@@ -25,6 +25,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int EM_THREADS = 256;
 constexpr int EM_STATUS_BAD_TOKEN = 8;
+constexpr int64_t EM_MAX_N = INT32_MAX - (1 << 16);  // positions are 32-bit, with a chunk to spare
 
 // Eight consecutive elements as FP32.
 template <typename T>
@@ -62,21 +63,47 @@ __device__ __forceinline__ void store8<bf16>(bf16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = u;
 }
 
-// W elements at p: a 16- or 32-byte vector (W = 8) or one element (W = 1).
+// W elements at p: an aligned vector (W = 8, or 4) or one element (W = 1).
 template <int W, typename T>
 __device__ __forceinline__ void load_w(const T* p, float (&v)[W]) {
-  if constexpr (W == 8)
+  if constexpr (W == 8) {
     load8<T>(p, v);
-  else
+  } else if constexpr (W == 4) {
+    static_assert(sizeof(T) == 4, "16 bytes");
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  } else {
     v[0] = to_f<T>(__ldg(p));
+  }
 }
 template <int W, typename T>
 __device__ __forceinline__ void store_w(T* p, const float (&v)[W]) {
-  if constexpr (W == 8)
+  if constexpr (W == 8) {
     store8<T>(p, v);
-  else
+  } else if constexpr (W == 4 && sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else if constexpr (W == 4) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+  } else {
     p[0] = from_f<T>(v[0]);
+  }
 }
+
+// A 16-byte vector (or one element) as it was loaded, and as FP32.
+template <int W, typename T>
+struct Raw {
+  T v[W];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (W > 1) {
+      static_assert(W * sizeof(T) == 16, "16 bytes");
+      *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+      v[0] = __ldg(p);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return to_f<T>(v[i]); }
+};
 
 // ---------------------------------------------------------------------------
 // Lookup: each CTA copies a group of rows, a thread per vector.
@@ -111,7 +138,7 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_fwd_kernel(
 // input; one launch counts its digits, the next places its elements after
 // those of smaller digits and of earlier blocks.
 // ---------------------------------------------------------------------------
-constexpr int RS_ITEMS = 16;
+constexpr int RS_ITEMS = 4;
 constexpr int RS_UNIT = EM_THREADS * RS_ITEMS;  // elements ranked at a time
 constexpr int RS_MAX_BLOCKS = 256;
 constexpr int RS_DIGITS = 256;
@@ -284,14 +311,15 @@ struct GradPlan {
 constexpr int GR_CHUNK_MAX = 128;
 constexpr int GR_ZERO_ROWS = 32;
 constexpr int GR_JOIN_UNITS = 64;
+constexpr int GR_POSITIONS = 4096;  // of the chunks of a CTA, at most
 
 GradPlan grad_plan(int64_t N, int64_t V, int units) {
   GradPlan g;
   g.units = units;
   g.tiles = (units + EM_THREADS - 1) / EM_THREADS;
   g.wide = (units + g.tiles - 1) / g.tiles;
-  g.groups = std::min(EM_THREADS / g.wide, 32);
   g.chunk = N >= 32768 ? GR_CHUNK_MAX : 32;
+  g.groups = std::min(EM_THREADS / g.wide, GR_POSITIONS / GR_CHUNK_MAX);
   g.chunks = (int)((N + g.chunk - 1) / g.chunk);
   g.blocks = (g.chunks + g.groups - 1) / g.groups;
   g.zero_blocks = (int)((V + GR_ZERO_ROWS - 1) / GR_ZERO_ROWS);
@@ -299,7 +327,7 @@ GradPlan grad_plan(int64_t N, int64_t V, int units) {
 }
 
 template <typename TG, typename TW, int W>
-__global__ void __launch_bounds__(EM_THREADS) embedding_grad_kernel(
+__global__ void __launch_bounds__(EM_THREADS, 4) embedding_grad_kernel(
     int N, int V, GradPlan g, const int* __restrict__ key, const int* __restrict__ pos,
     const TG* __restrict__ dout, float scale, TW* __restrict__ dweight,
     float* __restrict__ partial) {
@@ -324,18 +352,28 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_grad_kernel(
     }
     return;
   }
+  // the keys and positions of the CTA's chunks, with the keys before and after
+  __shared__ int keys[GR_POSITIONS + 2], places[GR_POSITIONS];
+  const int c0 = blockIdx.x * g.groups * g.chunk;
+  const int count = min(g.groups * g.chunk, N - c0);
+  for (int i = t; i < count + 2; i += EM_THREADS) {
+    const int at = c0 + i - 1;
+    keys[i] = at >= 0 && at < N ? key[at] : -1;
+    if (i < count) places[i] = pos[c0 + i];
+  }
+  __syncthreads();
   const int group = t / g.wide;
   const int chunk = blockIdx.x * g.groups + group;
   const int u = blockIdx.y * g.wide + t % g.wide;
   if (group >= g.groups || chunk >= g.chunks || u >= g.units) return;
-  const int i0 = chunk * g.chunk, i1 = min(i0 + g.chunk, N);
-  const int before = i0 > 0 ? key[i0 - 1] : -1;
-  const int after = i1 < N ? key[i1] : -1;
-  int cur = key[i0];
+  const int i0 = group * g.chunk, i1 = min(i0 + g.chunk, count);
+  const int* k = keys + 1;
+  const int before = k[i0 - 1], after = k[i1];
+  int cur = k[i0];
   bool first = true;
   float sum[W];
 #pragma unroll
-  for (int k = 0; k < W; ++k) sum[k] = 0.f;
+  for (int j = 0; j < W; ++j) sum[j] = 0.f;
   auto flush = [&](bool last) {
     if (cur >= V) return;
     const bool began = first && cur == before;
@@ -343,35 +381,31 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_grad_kernel(
     if (!began && !goes_on) {
       float out[W];
 #pragma unroll
-      for (int k = 0; k < W; ++k) out[k] = sum[k] * scale;
+      for (int j = 0; j < W; ++j) out[j] = sum[j] * scale;
       store_w<W, TW>(dweight + ((size_t)cur * g.units + u) * W, out);
     } else {
       store_w<W, float>(partial + (((size_t)chunk * 2 + (began ? 0 : 1)) * g.units + u) * W, sum);
     }
   };
+  const TG* column = dout + (size_t)u * W;
   for (int i = i0; i < i1 && cur < V; i += AHEAD) {
-    float v[AHEAD][W];
-    int k[AHEAD];
+    Raw<W, TG> v[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (i + a < i1) v[a].load(column + (size_t)places[i + a] * g.units * W);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      k[a] = i + a < i1 ? key[i + a] : -1;
-      if (k[a] >= 0 && k[a] < V)
-        load_w<W, TG>(dout + ((size_t)pos[i + a] * g.units + u) * W, v[a]);
-    }
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      if (k[a] < 0) break;
-      if (k[a] != cur) {
+      if (i + a >= i1) break;
+      if (k[i + a] != cur) {
         flush(false);
         first = false;
-        cur = k[a];
+        cur = k[i + a];
+        if (cur >= V) break;
 #pragma unroll
         for (int j = 0; j < W; ++j) sum[j] = 0.f;
       }
-      if (cur < V) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) sum[j] += v[a][j];
-      }
+      for (int j = 0; j < W; ++j) sum[j] += v[a].at(j);
     }
   }
   flush(true);
@@ -389,13 +423,23 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_join_kernel(
   const int chunk = blockIdx.x;
   const int i0 = chunk * g.chunk, i1 = min(i0 + g.chunk, N);
   if (i1 >= N) return;
-  const int id = key[i1 - 1];
-  if (id >= V || key[i1] != id) return;               // nothing goes on
-  if (key[i0] == id && i0 > 0 && key[i0 - 1] == id) return;  // begun earlier
-  // chunks it goes on into: mostly the next one alone
+  // read together: a CTA that finds nothing to do costs one round trip
+  const int id = key[i1 - 1], next = key[i1], first = key[i0];
+  const int before = key[max(i0 - 1, 0)], far = key[min(i1 + g.chunk, N) - 1];
+  if (id >= V || next != id) return;                       // nothing goes on
+  if (first == id && i0 > 0 && before == id) return;       // begun earlier
+  // chunks it goes on into (mostly the next one alone): those that begin with
+  // its id, EM_THREADS of them looked at in one round trip
   int n = 1;
-  if (i1 + g.chunk <= N && key[i1 + g.chunk - 1] == id)
-    n = (lower_bound(key, N, id + 1) - 1) / g.chunk - chunk;
+  if (i1 + g.chunk <= N && far == id) {
+    n = 0;
+    for (int c = chunk + 1;; c += EM_THREADS) {
+      const long long at = ((long long)c + threadIdx.x) * g.chunk;
+      const int found = __syncthreads_count(at < N && key[at] == id);
+      n += found;
+      if (found < EM_THREADS) break;
+    }
+  }
   const int lane = threadIdx.x % GR_JOIN_UNITS, slice = threadIdx.x / GR_JOIN_UNITS;
   const int u = blockIdx.y * GR_JOIN_UNITS + lane;
   const bool in = u < g.units;
@@ -403,7 +447,7 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_join_kernel(
 #pragma unroll
   for (int k = 0; k < W; ++k) sum[k] = 0.f;
   if (in) {
-#pragma unroll 4
+#pragma unroll 8
     for (int j = slice; j <= n; j += SLICES) {
       float v[W];
       load_w<W, float>(
@@ -428,7 +472,7 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_join_kernel(
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_embedding(const char* what, int wdtype, int odtype, int64_t N, int64_t V, int64_t D) {
-  if (N < 0 || N > INT32_MAX || V <= 0 || V >= INT32_MAX || D <= 0 || D > INT32_MAX / 8) {
+  if (N < 0 || N > EM_MAX_N || V <= 0 || V >= INT32_MAX || D <= 0 || D > INT32_MAX / 8) {
     set_error("%s: unsupported sizes N=%lld V=%lld D=%lld", what, (long long)N, (long long)V,
               (long long)D);
     return DABSN_ERR_SHAPE;
@@ -487,8 +531,9 @@ int launch_grad_w(int64_t N, int64_t V, int units, const int* key, const int* po
 template <typename TG, typename TW>
 int launch_grad(int64_t N, int64_t V, int64_t D, const int* key, const int* pos,
                 const void* dout, float scale, void* dweight, float* partial, cudaStream_t st) {
-  const bool vec = D % 8 == 0 && aligned16(dout) && aligned16(dweight) && aligned16(partial);
-  return vec ? launch_grad_w<TG, TW, 8>(N, V, (int)(D / 8), key, pos, dout, scale, dweight,
+  constexpr int W = 16 / sizeof(TG);
+  const bool vec = D % W == 0 && aligned16(dout) && aligned16(dweight) && aligned16(partial);
+  return vec ? launch_grad_w<TG, TW, W>(N, V, (int)(D / W), key, pos, dout, scale, dweight,
                                         partial, st)
              : launch_grad_w<TG, TW, 1>(N, V, (int)D, key, pos, dout, scale, dweight, partial,
                                         st);
@@ -521,7 +566,7 @@ extern "C" int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, i
 }
 
 extern "C" size_t dabsn_embedding_bwd_workspace(int64_t N, int64_t V, int64_t D) {
-  if (N < 0 || N > INT32_MAX || V <= 0 || V >= INT32_MAX || D <= 0) return 0;
+  if (N < 0 || N > EM_MAX_N || V <= 0 || V >= INT32_MAX || D <= 0) return 0;
   return sort_bytes(N, V) + partial_bytes(N, D);
 }
 

@@ -8,7 +8,7 @@
 // temperature the statistics are
 //   m  = max x,   s = sum 2^d,   sd = sum d 2^d,   d = (x - m) c,
 // all FP32; (x - m) is formed first, so a row far from zero loses nothing.
-// d is clamped from below at -150, where 2^d flushes to zero: a masked logit
+// d is clamped from below at -127, where 2^d flushes to zero: a masked logit
 // (-inf, or the type's lowest value) adds 0 to both sums instead of 0 * -inf.
 // The maximum is clamped at -FLT_MAX, so that s == 0 exactly when every logit
 // is -inf.  NaN and +inf make s NaN.
@@ -26,7 +26,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kFloor = -150.f;  // 2^kFloor is zero in FP32
+constexpr float kFloor = -127.f;  // 2^kFloor is flushed to zero
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -73,6 +73,16 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   f32x2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
+}
+
+__device__ __forceinline__ f32x2 clamp2(f32x2 d) {
+  const float2 v = split(d);
+  return pair(max_nan(v.x, kFloor), max_nan(v.y, kFloor));
+}
+
+__device__ __forceinline__ f32x2 ex2_pair(f32x2 d) {
+  const float2 v = split(d);
+  return pair(ex2(v.x), ex2(v.y));
 }
 
 // 16-byte vectors of T.
@@ -201,14 +211,6 @@ __device__ __forceinline__ void rescale(Stats& st, float mx, float c) {
   st.mx = mx;
 }
 
-__device__ __forceinline__ void merge(Stats& a, Stats b, float c) {
-  const float mx = fmaxf(a.mx, b.mx);
-  rescale(a, mx, c);
-  rescale(b, mx, c);
-  a.s += b.s;
-  a.sd += b.sd;
-}
-
 // Adds one element.
 __device__ __forceinline__ void add_value(Stats& st, float x, float c) {
   rescale(st, fmaxf(st.mx, x), c);
@@ -233,14 +235,11 @@ __device__ __forceinline__ void add_vectors(Stats& st, const uint4 (&raw)[U], fl
     unpack<T>(raw[u], v);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      float2 d = split(mul2(add2(v[i], m2), c2));
-      if (SD) {
-        d.x = max_nan(d.x, kFloor);
-        d.y = max_nan(d.y, kFloor);
-      }
-      const f32x2 e = pair(ex2(d.x), ex2(d.y));
+      f32x2 d = mul2(add2(v[i], m2), c2);
+      if (SD) d = clamp2(d);
+      const f32x2 e = ex2_pair(d);
       s2 = add2(s2, e);
-      if (SD) sd2 = fma2(e, pair(d.x, d.y), sd2);
+      if (SD) sd2 = fma2(e, d, sd2);
     }
   }
   const float2 s = split(s2), sd = split(sd2);
@@ -264,49 +263,59 @@ __device__ __forceinline__ Stats sweep(const T* p, int n, int t, float c) {
     for (int u = 0; u < U; ++u) raw[u] = __ldg(pv + i + u * THREADS);
     add_vectors<T, U, SD>(st, raw, c);
   }
-  for (; i < r.nv; i += THREADS) {
-    const uint4 raw[1] = {__ldg(pv + i)};
-    add_vectors<T, 1, SD>(st, raw, c);
+  if (i < r.nv) {  // one to three more, loaded together
+    uint4 raw[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (i + u * THREADS < r.nv) raw[u] = __ldg(pv + i + u * THREADS);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (i + u * THREADS < r.nv) {
+        const uint4 one[1] = {raw[u]};
+        add_vectors<T, 1, SD>(st, one, c);
+      }
   }
   if (t < r.head) add_value(st, to_f<T>(p[t]), c);
   if (t < r.tail) add_value(st, to_f<T>(p[r.tail0 + t]), c);
   return st;
 }
 
+// The merged statistics of groups of LANES lanes, the same bits in each: the
+// maximum first, one rescaling, then plain sums.
+template <int LANES = 32>
 __device__ __forceinline__ Stats warp_merge(Stats st, float c) {
+  float mx = st.mx;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats b;
-    b.mx = __shfl_xor_sync(0xffffffffu, st.mx, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    b.sd = __shfl_xor_sync(0xffffffffu, st.sd, o);
-    merge(st, b, c);
+  for (int o = LANES / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  rescale(st, mx, c);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+    st.sd += __shfl_xor_sync(0xffffffffu, st.sd, o);
   }
   return st;
 }
 
 // Merges the threads' statistics of a CTA in a fixed order; every thread gets
-// the result.  `sh` holds three floats a warp.  Ends with a barrier before the
-// next use of `sh` being the caller's business.
+// the result.  `sh` holds three floats a warp; a barrier must come between this
+// call and the next.
 template <int THREADS>
 __device__ __forceinline__ Stats block_merge(Stats st, float (*sh)[3], float c) {
+  constexpr int WARPS = THREADS / 32;
+  static_assert((WARPS & (WARPS - 1)) == 0 && WARPS <= 32, "a power of two");
   st = warp_merge(st, c);
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) {
     sh[warp][0] = st.mx;
     sh[warp][1] = st.s;
     sh[warp][2] = st.sd;
   }
   __syncthreads();
   Stats all;
-  for (int w = 0; w < THREADS / 32; ++w) {
-    Stats b;
-    b.mx = sh[w][0];
-    b.s = sh[w][1];
-    b.sd = sh[w][2];
-    merge(all, b, c);
-  }
-  return all;
+  all.mx = sh[lane % WARPS][0];
+  all.s = sh[lane % WARPS][1];
+  all.sd = sh[lane % WARPS][2];
+  return warp_merge<WARPS>(all, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -330,13 +339,9 @@ __device__ __forceinline__ uint4 grad_vector(const uint4& raw, f32x2 m2, f32x2 c
   unpack<T>(raw, v);
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    float2 d = split(mul2(add2(v[i], m2), c2));
-    if (HAS_B) {
-      d.x = max_nan(d.x, kFloor);
-      d.y = max_nan(d.y, kFloor);
-    }
-    const f32x2 e = pair(ex2(d.x), ex2(d.y));
-    v[i] = mul2(e, HAS_B ? fma2(B2, pair(d.x, d.y), A2) : A2);
+    f32x2 d = mul2(add2(v[i], m2), c2);
+    if (HAS_B) d = clamp2(d);
+    v[i] = mul2(ex2_pair(d), HAS_B ? fma2(B2, d, A2) : A2);
   }
   return pack<T>(v);
 }

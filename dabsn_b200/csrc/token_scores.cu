@@ -28,176 +28,231 @@ typedef unsigned long long u64;
 
 constexpr int TS_THREADS = 256;
 constexpr int TS_MAX_K = 128;
-constexpr int TS_CAP = 512;  // candidates above the bound, and as many equal to it
+constexpr int TS_CAP = 1024;  // candidates of a row
 constexpr int STATUS_BAD_TOKEN = 8;
 
 // Order of the alternatives as unsigned keys: larger logit, larger key; -0
-// equals +0; NaN is above everything; 0 is below every logit.
+// equals +0; 0 is below every logit.  (A row with NaN has no order: it takes
+// another way.)
 __device__ __forceinline__ unsigned order_key(float x) {
-  if (x != x) return 0xffffffffu;
   const unsigned u = __float_as_uint(x + 0.f);
   return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned k) {
-  if (k == 0xffffffffu) return __int_as_float(0x7fc00000);
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 // One candidate: larger is better; equal logits rank by the lower index.
 __device__ __forceinline__ u64 candidate(unsigned key, int index) {
   return ((u64)key << 32) | (unsigned)~index;
 }
+__device__ __forceinline__ int candidate_index(u64 c) { return ~(int)(unsigned)c; }
 
+// Shared memory of a CTA of THREADS threads that selects.
+template <int THREADS>
 struct TopkShared {
-  unsigned keys[TS_THREADS];
-  short hot[TS_THREADS];
-  u64 above[TS_CAP], equal[TS_CAP];
-  int n_above, n_equal, n_hot;
+  unsigned keys[THREADS];
+  short hot[THREADS];
+  u64 found[TS_CAP];
+  int n_found, n_equal, n_hot;
   unsigned bound;
-  int warp_count[TS_THREADS / 32];
+  int warp_count[THREADS / 32];
 };
 
-// The k-th largest of the threads' keys, found bit by bit by one warp (0 when
-// fewer than k threads have any element: everything is a candidate then).
-__device__ __forceinline__ unsigned kth_key(const unsigned* keys, int k) {
-  constexpr int PER = TS_THREADS / 32;
+// One warp: a bound that at least k of the threads' keys reach, and the list of
+// the threads whose key reaches it.  The bound is found two bits at a time below
+// the bits that all keys share: the k-th largest key, or (unless `exact`) the
+// first prefix of it that few more than k reach; 0 when fewer than k threads
+// have any element.  A BF16 key is its upper half.
+template <typename T, int THREADS>
+__device__ __forceinline__ void find_bound(TopkShared<THREADS>& sh, int k, bool exact) {
+  constexpr int PER = THREADS / 32, LAST = sizeof(T) == 2 ? 16 : 0;
   const int lane = threadIdx.x & 31;
-  unsigned own[PER];
+  unsigned own[PER], hi = 0u, lo = 0xffffffffu;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) own[i] = keys[lane + 32 * i];
-  unsigned t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const unsigned cand = t | (1u << bit);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) n += own[i] >= cand;
-    if (__reduce_add_sync(0xffffffffu, n) >= k) t = cand;
+  for (int i = 0; i < PER; ++i) {
+    own[i] = sh.keys[lane + 32 * i];
+    hi = max(hi, own[i]);
+    lo = min(lo, own[i]);
   }
-  return t;
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  const int open = (33 - __clz((int)(hi ^ lo))) & ~1;  // lower bits that differ, rounded up
+  unsigned t = open >= 32 ? 0u : hi >> open << open;
+  for (int bit = open - 2; bit >= LAST; bit -= 2) {
+    // how many keys reach each of the three next steps, in one sum
+    const unsigned step = 1u << bit;
+    unsigned n = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      n += (own[i] >= t + step) + ((own[i] >= t + 2 * step) << 10) +
+           ((own[i] >= t + 3 * step) << 20);
+    n = __reduce_add_sync(0xffffffffu, n);
+    const int n1 = n & 1023, n2 = n >> 10 & 1023, n3 = n >> 20;
+    const int took = n3 >= k ? 3 : n2 >= k ? 2 : n1 >= k ? 1 : 0;
+    t += took * step;
+    if (!exact && took > 0 && (took == 3 ? n3 : took == 2 ? n2 : n1) <= k + 8) break;
+  }
+  // the lower half of a BF16 key: zeros from zero up, ones below
+  if (LAST == 16 && exact) {
+    t &= 0xffff0000u;
+    if (t != 0u && !(t & 0x80000000u)) t |= 0xffffu;
+  }
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool hot = own[i] != 0u && own[i] >= t;
+    const unsigned votes = __ballot_sync(0xffffffffu, hot);
+    if (hot) sh.hot[count + __popc(votes & ((1u << lane) - 1))] = (short)(lane + 32 * i);
+    count += __popc(votes);
+  }
+  if (lane == 0) {
+    sh.bound = t;
+    sh.n_hot = count;
+  }
 }
 
-__device__ __forceinline__ void offer(TopkShared& sh, unsigned bound, float x, int index) {
-  const unsigned key = order_key(x);
-  if (key > bound) {
-    const int at = atomicAdd(&sh.n_above, 1);
-    if (at < TS_CAP) sh.above[at] = candidate(key, index);
-  } else if (key == bound) {
-    if (*(volatile int*)&sh.n_equal <= TS_CAP) {
-      const int at = atomicAdd(&sh.n_equal, 1);
-      if (at < TS_CAP) sh.equal[at] = candidate(key, index);
-    }
-  }
-}
-
-// Offers every element of the row that a thread of `hot` read in the sweep.
-template <typename T>
-__device__ __forceinline__ void offer_parts(TopkShared& sh, unsigned bound, const T* p, int n,
-                                            int n_hot) {
+// Visits every element of the row that a thread of `hot` read in the sweep, a
+// vector to a thread at a time: visit(x, index) for the elements from `low` on;
+// vectors below it cost their maximum.
+template <typename T, int THREADS, typename Visit>
+__device__ __forceinline__ void visit_parts(const TopkShared<THREADS>& sh, const T* p, int n,
+                                            int n_hot, float low, Visit visit) {
   constexpr int VW = Vec<T>::N;
   const RowShape r = row_shape(p, n);
   const uint4* pv = reinterpret_cast<const uint4*>(p + r.head);
-  const int per = (r.nv + TS_THREADS - 1) / TS_THREADS;
-  for (int e = threadIdx.x; e < n_hot * per; e += TS_THREADS) {
-    const int k = sh.hot[e / per] + (e % per) * TS_THREADS;
+  const int per = (r.nv + THREADS - 1) / THREADS;
+  for (int e = threadIdx.x; e < n_hot * per; e += THREADS) {
+    const int h = e / per, k = sh.hot[h] + (e - h * per) * THREADS;
     if (k >= r.nv) continue;
+    const uint4 raw[1] = {__ldg(pv + k)};
+    if (vector_max<T, 1>(raw) < low) continue;
     f32x2 v[VW / 2];
-    unpack<T>(__ldg(pv + k), v);
+    unpack<T>(raw[0], v);
 #pragma unroll
     for (int j = 0; j < VW / 2; ++j) {
       const float2 x = split(v[j]);
-      offer(sh, bound, x.x, r.head + k * VW + 2 * j);
-      offer(sh, bound, x.y, r.head + k * VW + 2 * j + 1);
+      if (x.x >= low) visit(x.x, r.head + k * VW + 2 * j);
+      if (x.y >= low) visit(x.y, r.head + k * VW + 2 * j + 1);
     }
   }
-  for (int e = threadIdx.x; e < n_hot; e += TS_THREADS) {
-    const int t = sh.hot[e];
-    if (t < r.head) offer(sh, bound, to_f<T>(p[t]), t);
-    if (t < r.tail) offer(sh, bound, to_f<T>(p[r.tail0 + t]), r.tail0 + t);
+  for (int h = threadIdx.x; h < n_hot; h += THREADS) {
+    const int t = sh.hot[h];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {  // the part's head and tail element
+      if (t >= (side == 0 ? r.head : r.tail)) continue;
+      const int i = side == 0 ? t : r.tail0 + t;
+      const float x = to_f<T>(p[i]);
+      if (x >= low) visit(x, i);
+    }
   }
 }
 
-// The row's k largest logits into sh.above / sh.equal (n_above and n_equal of
-// them, at least k together); `mx` is the maximum of this thread's part.
-template <typename T>
-__device__ void select_top(TopkShared& sh, const T* p, int n, int k, float mx) {
+template <int THREADS>
+__device__ __forceinline__ void keep(TopkShared<THREADS>& sh, unsigned key, int index) {
+  const int at = atomicAdd(&sh.n_found, 1);
+  if (at < TS_CAP) sh.found[at] = candidate(key, index);
+}
+
+// More logits reach the bound than are kept: a flat row, a masked one with
+// fewer than k logits left, one built against the bound.  With the k-th largest
+// key of the threads (or, where too many lie above that too, of the row): what
+// lies above it, and of the logits equal to it the lowest indices, in order.
+template <typename T, int THREADS>
+__device__ __noinline__ void select_top_slow(TopkShared<THREADS>& sh, const T* p, int n, int k) {
   const int t = threadIdx.x;
-  const RowShape r = row_shape(p, n);
-  const bool any = t < r.nv || t < r.head || t < r.tail;
-  const unsigned key = any ? order_key(mx) : 0u;
-  sh.keys[t] = key;
-  if (t == 0) sh.n_above = sh.n_equal = sh.n_hot = 0;
-  __syncthreads();
-  if (t < 32) {
-    const unsigned b = kth_key(sh.keys, k);
-    if (t == 0) sh.bound = b;
-  }
+  if (t < 32) find_bound<T, THREADS>(sh, k, true);
+  if (t == 0) sh.n_found = 0;
   __syncthreads();
   unsigned bound = sh.bound;
-  if (any && key >= bound) sh.hot[atomicAdd(&sh.n_hot, 1)] = (short)t;
+  auto above = [&](float x, int index) {
+    const unsigned key = order_key(x);
+    if (key > bound) keep(sh, key, index);
+  };
+  const float low = bound == 0u ? -INFINITY : key_value(bound);
+  // strictly above, so the next number is where the visit starts
+  visit_parts<T, THREADS>(sh, p, n, sh.n_hot, bound == 0u ? low : key_value(bound + 1u), above);
   __syncthreads();
-  offer_parts<T>(sh, bound, p, n, sh.n_hot);
-  __syncthreads();
-  if (sh.n_above > TS_CAP) {
-    // A row built against the bound: find its exact k-th largest key, by bits,
-    // over the whole row, and take what lies above it (fewer than k).
+  if (sh.n_found > TS_CAP) {
     bound = 0;
     for (int bit = 31; bit >= 0; --bit) {
       const unsigned cand = bound | (1u << bit);
       __syncthreads();
-      if (t == 0) sh.n_above = 0;
+      if (t == 0) sh.n_found = 0;
       __syncthreads();
       int c = 0;
-      for (int i = t; i < n; i += TS_THREADS) c += order_key(to_f<T>(p[i])) >= cand;
+      for (int i = t; i < n; i += THREADS) c += order_key(to_f<T>(p[i])) >= cand;
       c = __reduce_add_sync(0xffffffffu, c);
-      if ((t & 31) == 0) atomicAdd(&sh.n_above, c);
+      if ((t & 31) == 0) atomicAdd(&sh.n_found, c);
       __syncthreads();
-      if (sh.n_above >= k) bound = cand;
+      if (sh.n_found >= k) bound = cand;
     }
     __syncthreads();
-    if (t == 0) sh.n_above = sh.n_equal = 0;
+    if (t == 0) sh.n_found = 0;
     __syncthreads();
-    for (int i = t; i < n; i += TS_THREADS) offer(sh, bound, to_f<T>(p[i]), i);
+    for (int i = t; i < n; i += THREADS) above(to_f<T>(p[i]), i);
     __syncthreads();
   }
-  const int need = k - sh.n_above;
-  if (need > 0 && sh.n_equal > TS_CAP) {
-    // More logits equal to the bound than were kept (a masked row with fewer
-    // than k logits left, a flat row): the lowest indices, in order.
-    int found = 0;
-    for (int base = 0; base < n && found < need; base += TS_THREADS) {
-      const int i = base + t;
-      const bool hit = i < n && order_key(to_f<T>(p[i])) == bound;
-      const unsigned votes = __ballot_sync(0xffffffffu, hit);
-      __syncthreads();
-      if ((t & 31) == 0) sh.warp_count[t >> 5] = __popc(votes);
-      __syncthreads();
-      int at = found + __popc(votes & ((1u << (t & 31)) - 1));
-      for (int w = 0; w < TS_THREADS / 32; ++w) {
-        if (w < (t >> 5)) at += sh.warp_count[w];
-        found += sh.warp_count[w];
-      }
-      if (hit && at < need) sh.equal[at] = candidate(bound, i);
+  const int have = sh.n_found, need = k - have;
+  int got = 0;
+  for (int base = 0; base < n && got < need; base += THREADS) {
+    const int i = base + t;
+    const bool hit = i < n && order_key(to_f<T>(p[i])) == bound;
+    const unsigned votes = __ballot_sync(0xffffffffu, hit);
+    __syncthreads();
+    if ((t & 31) == 0) sh.warp_count[t >> 5] = __popc(votes);
+    __syncthreads();
+    int at = got + __popc(votes & ((1u << (t & 31)) - 1));
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < (t >> 5)) at += sh.warp_count[w];
+      got += sh.warp_count[w];
     }
-    __syncthreads();
-    if (t == 0) sh.n_equal = need;
-    __syncthreads();
+    if (hit && at < need) sh.found[have + at] = candidate(bound, i);
   }
+  __syncthreads();
+  if (t == 0 && need > 0) sh.n_found = k;
+  __syncthreads();
 }
 
-// Ranks the candidates and stores the first k: ids, and log-probabilities
-// (x - m) inv_t - log_s.
-__device__ __forceinline__ void store_top(const TopkShared& sh, int k, float m, float inv_t,
-                                          float log_s, bool empty, float* values, int64_t* ids) {
-  const int na = sh.n_above, ne = na >= k ? 0 : sh.n_equal;
-  for (int c = threadIdx.x; c < na + ne; c += TS_THREADS) {
-    const u64 mine = c < na ? sh.above[c] : sh.equal[c - na];
+// This thread's key: the maximum of its part of the row.  A barrier comes
+// between this and select_top.
+template <typename T, int THREADS>
+__device__ __forceinline__ void offer_part(TopkShared<THREADS>& sh, const T* p, int n, float mx) {
+  const int t = threadIdx.x;
+  const RowShape r = row_shape(p, n);
+  const bool any = t < r.nv || t < r.head || t < r.tail;
+  sh.keys[t] = any ? order_key(mx) : 0u;
+  if (t == 0) sh.n_found = 0;
+}
+
+// Candidates for the k largest of the row's n logits (no NaN, not all -inf)
+// into sh.found, sh.n_found of them (k at least).
+template <typename T, int THREADS>
+__device__ __forceinline__ void select_top(TopkShared<THREADS>& sh, const T* p, int n, int k) {
+  if (threadIdx.x < 32) find_bound<T, THREADS>(sh, k, false);
+  __syncthreads();
+  const unsigned bound = sh.bound;
+  // Below the key of -inf the bound admits masked logits: the other way takes
+  // those in order.
+  if (bound > order_key(-INFINITY)) {
+    visit_parts<T, THREADS>(sh, p, n, sh.n_hot, key_value(bound), [&](float x, int index) {
+      if (*(volatile int*)&sh.n_found <= TS_CAP) keep(sh, order_key(x), index);
+    });
+    __syncthreads();
+    if (sh.n_found <= TS_CAP) return;
+  }
+  __syncthreads();
+  select_top_slow<T, THREADS>(sh, p, n, k);
+}
+
+// Calls put(rank, candidate) for the k best candidates.
+template <int THREADS, typename Put>
+__device__ __forceinline__ void rank_found(const TopkShared<THREADS>& sh, int k, Put put) {
+  const int n = sh.n_found;
+  for (int c = threadIdx.x; c < n; c += THREADS) {
+    const u64 mine = sh.found[c];
     int rank = 0;
-    for (int o = 0; o < na; ++o) rank += sh.above[o] > mine;
-    for (int o = 0; o < ne; ++o) rank += sh.equal[o] > mine;
-    if (rank < k) {
-      const float x = key_value((unsigned)(mine >> 32));
-      values[rank] = empty ? -INFINITY : (x - m) * inv_t - log_s;
-      ids[rank] = (int64_t)(unsigned)~(unsigned)mine;
-    }
+    for (int o = 0; o < n; ++o) rank += sh.found[o] > mine;
+    if (rank < k) put(rank, mine);
   }
 }
 
@@ -224,14 +279,14 @@ __device__ __forceinline__ void write_scores(const Stats& all, const T* row, lon
   if (stats) *stats = make_float2(m, all.s);
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
+template <typename T, int THREADS, bool TOP>
+__device__ __forceinline__ void token_scores_rows(
     long long rows, int V, long long ld, const T* __restrict__ logits,
     const int64_t* __restrict__ tokens, long long ignore_index, float inv_t, int k,
     float* __restrict__ log_prob, float* __restrict__ entropy, float2* __restrict__ stats,
     float* __restrict__ top_values, int64_t* __restrict__ top_ids, int* status) {
-  __shared__ float part[TS_THREADS / 32][3];
-  __shared__ TopkShared top;
+  __shared__ float part[THREADS / 32][3];
+  __shared__ TopkShared<THREADS> top;
   const float c = kLog2e * inv_t;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const long long t = tokens[r];
@@ -240,25 +295,60 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
         write_scores(Stats(), logits, t, V, true, inv_t, log_prob + r, entropy + r,
                      stats ? stats + r : nullptr, status);
       if (TOP)
-        for (int i = threadIdx.x; i < k; i += TS_THREADS) {
+        for (int i = threadIdx.x; i < k; i += THREADS) {
           top_values[r * k + i] = -INFINITY;
           top_ids[r * k + i] = -1;
         }
       continue;
     }
     const T* row = logits + (size_t)r * ld;
-    const Stats own = sweep<T, TS_THREADS, true>(row, V, threadIdx.x, c);
-    const Stats all = block_merge<TS_THREADS>(own, part, c);
+    const Stats own = sweep<T, THREADS, true>(row, V, threadIdx.x, c);
+    if (TOP) offer_part<T, THREADS>(top, row, V, own.mx);
+    const Stats all = block_merge<THREADS>(own, part, c);
     if (threadIdx.x == 0)
       write_scores(all, row, t, V, false, inv_t, log_prob + r, entropy + r,
                    stats ? stats + r : nullptr, status);
     if (TOP) {
-      select_top<T>(top, row, V, k, own.mx);
-      store_top(top, k, finite_max(all.mx), inv_t, logf(all.s), all.s == 0.f,
-                top_values + r * k, top_ids + r * k);
+      const float m = finite_max(all.mx), log_s = logf(all.s);
+      float* values = top_values + r * k;
+      int64_t* ids = top_ids + r * k;
+      if (all.s > 0.f) {
+        select_top<T, THREADS>(top, row, V, k);
+        rank_found(top, k, [&](int rank, u64 best) {
+          values[rank] = (key_value((unsigned)(best >> 32)) - m) * inv_t - log_s;
+          ids[rank] = candidate_index(best);
+        });
+      } else {  // all -inf (s == 0), or no order (s is NaN): the first ids
+        for (int i = threadIdx.x; i < k; i += THREADS) {
+          values[i] = all.s == 0.f ? -INFINITY : all.s;
+          ids[i] = i;
+        }
+      }
     }
     __syncthreads();
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits,
+    const int64_t* __restrict__ tokens, long long ignore_index, float inv_t,
+    float* __restrict__ log_prob, float* __restrict__ entropy, float2* __restrict__ stats,
+    int* status) {
+  token_scores_rows<T, TS_THREADS, false>(rows, V, ld, logits, tokens, ignore_index, inv_t, 0,
+                                          log_prob, entropy, stats, nullptr, nullptr, status);
+}
+
+// Eight CTAs an SM: the selection is a chain of short steps between barriers,
+// which only other rows can fill.
+template <typename T>
+__global__ void __launch_bounds__(TS_THREADS, 8) token_scores_top_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits,
+    const int64_t* __restrict__ tokens, long long ignore_index, float inv_t, int k,
+    float* __restrict__ log_prob, float* __restrict__ entropy, float2* __restrict__ stats,
+    float* __restrict__ top_values, int64_t* __restrict__ top_ids, int* status) {
+  token_scores_rows<T, TS_THREADS, true>(rows, V, ld, logits, tokens, ignore_index, inv_t, k,
+                                         log_prob, entropy, stats, top_values, top_ids, status);
 }
 
 // Rows short enough for one warp: eight a CTA, no barriers.
@@ -357,7 +447,7 @@ int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
   const float inv_t = 1.f / temperature;
   int* status = device_status();
   if (k > 0)
-    token_scores_fwd_kernel<T, true><<<row_grid(rows), TS_THREADS, 0, st>>>(
+    token_scores_top_kernel<T><<<row_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (int)k, log_prob,
         entropy, (float2*)stats, top_values, top_ids, status);
   else if (V * sizeof(T) <= TS_WARP_BYTES)
@@ -365,9 +455,9 @@ int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
         (float2*)stats, status);
   else
-    token_scores_fwd_kernel<T, false><<<row_grid(rows), TS_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, 0, log_prob, entropy,
-        (float2*)stats, nullptr, nullptr, status);
+    token_scores_fwd_kernel<T><<<row_grid(rows), TS_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
+        (float2*)stats, status);
   return launch_status("token_scores_fwd");
 }
 
