@@ -132,7 +132,6 @@ _SIGNATURES = {
     "dabsn_distill_bwd": (
         [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _i32, _vp, _i64, _i32, _vp,
          _i64, _vp], _i32),
-    "dabsn_distill_grad_fits": ([_i32, _i64, _i64], _i32),
     "dabsn_distill_grad": (
         [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _i32, _vp, _vp, _vp, _i64, _vp],
         _i32),

@@ -731,14 +731,12 @@ class _Distillation(torch.autograd.Function):
         entries, mean = teacher_tokens.shape[1], reduction == "mean"
         lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
                                  ignore_index)
-        both = None
-        if reduction != "none":
-            both = ops.distill_gradient(logits, lists, entries, temperature, mean)
-        if both is None:
-            (loss, stats), ctx.ready = ops.distill_forward(logits, lists, entries,
-                                                           temperature), None
+        if reduction == "none":
+            loss, stats = ops.distill_forward(logits, lists, entries, temperature)
+            ctx.ready = None
         else:
-            loss, stats, ctx.ready = both
+            loss, stats, ctx.ready = ops.distill_gradient(logits, lists, entries, temperature,
+                                                          mean)
             ctx.capture = ops.capture_id(logits.device)
         ctx.save_for_backward(logits, lists, stats)
         ctx.meta = (entries, temperature, reduction)

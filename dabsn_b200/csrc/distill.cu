@@ -344,20 +344,24 @@ __global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Loss and gradient in one pass over the logits (weights known beforehand: the
-// sum or the mean of the rows' losses, upstream gradient 1).
+// Loss and gradient with one read of the logits from memory (weights known
+// beforehand: the sum or the mean of the rows' losses, upstream gradient 1).
+// What bounds it is HBM: V read and V written a row.
 //
-// The row stays on the SM between its statistics and its gradient: every
-// thread copies its own vectors into its own slots of shared memory
-// (cp.async), so neither sweep needs a barrier with another thread, and the
+// Rows of up to 72 KB stay in shared memory between their statistics and their
+// gradient, three CTAs an SM: every thread copies its own vectors into its own
+// slots (cp.async), so neither sweep waits for another thread's copies, and the
 // copies of the next row are issued slot by slot as the gradient of this one
-// leaves them: reads, arithmetic and writes of neighbouring rows overlap, with
-// three CTAs an SM.  What bounds it is HBM: V read and V written a row.  A row
-// that does not fit a third of an SM's shared memory is shared by a cluster of
-// 2, 4 or 8 CTAs, which merge their statistics through distributed shared
-// memory; so is a row when there are fewer rows than SMs.
+// leaves them: reads, arithmetic and writes of neighbouring rows overlap.
+// Longer rows, and rows too few to fill the SMs that way, are read a second
+// time out of L2 (distill_long_kernel): two CTAs of 1024 threads an SM keep at
+// most 296 rows in flight, 76 MB of BF16 rows of 128000.  32768 BF16 rows of
+// 32000: 700 us the first way (630 us of traffic at the copy rate), 715 us the
+// second; 515 of 128000: 70 us the second way, 87 us with a row shared by the
+// shared memory of a cluster of four CTAs.
 // ---------------------------------------------------------------------------
 constexpr int DF_THREADS = 256;
+constexpr int DF_ROW_BYTES = 72 * 1024;
 static_assert(DT_MAX_K <= DF_THREADS, "a thread holds at most one entry");
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
@@ -380,33 +384,29 @@ __device__ __forceinline__ void cp_async_wait_for(int pending) {
   }
 }
 
-template <typename T, bool SPLIT>
+template <typename T>
 __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, int share, float* __restrict__ loss,
-    float2* __restrict__ stats, T* __restrict__ dlogits, long long ldd) {
+    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
+    T* __restrict__ dlogits, long long ldd) {
   extern __shared__ uint4 slots[];  // [vectors of a thread][DF_THREADS]
   __shared__ float part[DF_THREADS / 32][3];
-  __shared__ float peer[2][8][2];
   __shared__ float loss_part[DF_THREADS / 32];
   const int t = threadIdx.x;
-  const int cl = SPLIT ? (int)cluster_nctarank() : 1;
-  const int rank = SPLIT ? (int)cluster_ctarank() : 0;
-  const long long stride = gridDim.x / cl;
-  const int a = min(rank * share, V), n = min(share, V - a);
+  const long long stride = gridDim.x;
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
   const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
   // Vectors of a row at most (rows of other alignments have one less).  Copies
   // are committed in groups of four vectors a thread, as many for every row, so
   // that the statistics start on the first while the last are under way.
-  const int most = n / Vec<T>::N;
+  const int most = V / Vec<T>::N;
   const int groups = (most + 4 * DF_THREADS - 1) / (4 * DF_THREADS);
 
   // The next row from r on that has a loss; the others' gradient is zero.
   auto next_live = [&](long long r) {
     while (r < rows && !list.live[r]) {
-      zero_row<T, DF_THREADS>(dlogits + (size_t)r * ldd + a, n, t);
-      if (t == 0 && rank == 0) {
+      zero_row<T, DF_THREADS>(dlogits + (size_t)r * ldd, V, t);
+      if (t == 0) {
         loss[r] = 0.f;
         stats[r] = make_float2(0.f, 0.f);
       }
@@ -415,15 +415,15 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     return r;
   };
 
-  long long r = next_live(blockIdx.x / cl);
+  long long r = next_live(blockIdx.x);
   float edge[2] = {0.f, 0.f};  // this thread's head and tail element
   auto load_edges = [&](const T* p, const RowShape& s) {
     if (t < s.head) edge[0] = to_f<T>(p[t]);
     if (t < s.tail) edge[1] = to_f<T>(p[s.tail0 + t]);
   };
   if (r < rows) {
-    const T* p = logits + (size_t)r * ld + a;
-    const RowShape s = row_shape(p, n);
+    const T* p = logits + (size_t)r * ld;
+    const RowShape s = row_shape(p, V);
     const uint4* v = reinterpret_cast<const uint4*>(p + s.head);
     for (int k0 = 0; k0 < most; k0 += 4 * DF_THREADS) {
 #pragma unroll
@@ -435,10 +435,9 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     }
     load_edges(p, s);
   }
-  if (SPLIT) cluster_sync_all();  // every CTA runs before another writes to it
-  for (int turn = 0; r < rows; turn ^= 1) {
+  while (r < rows) {
     const T* row = logits + (size_t)r * ld;
-    const RowShape s = row_shape(row + a, n);
+    const RowShape s = row_shape(row, V);
     int id = -1;
     float2 q = make_float2(0.f, 0.f);
     float x = 0.f;
@@ -466,41 +465,24 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     if (t < s.tail) add_value(st, edge[1], c);
     st.sd = 0.f;
     st = block_merge<DF_THREADS>(st, part, c);
-    if (SPLIT) {
-      if (t < cl) {
-        const uint32_t to = map_shared_rank(&peer[turn][rank][0], t);
-        st_cluster_f32(to, st.mx);
-        st_cluster_f32(to + 4, st.s);
-      }
-      __syncwarp();
-      cluster_sync_all();
-      Stats other;  // empty for lanes past the cluster
-      if ((t & 7) < cl) {
-        other.mx = peer[turn][t & 7][0];
-        other.s = peer[turn][t & 7][1];
-      }
-      st = warp_merge<8>(other, c);
-    }
     const float m = finite_max(st.mx);
     const bool empty = st.s == 0.f;
-    if (rank == 0) {
-      float l = 0.f;
-      if (q.x != q.x) l = q.x;
-      if (id >= 0 && q.x > 0.f)
-        l = q.x * (logf(q.x) - (empty ? -INFINITY : (x - m) * inv_t - logf(st.s)));
-      l = warp_sum(l);
-      if ((t & 31) == 0) loss_part[t >> 5] = l;
-    }
+    float l = 0.f;
+    if (q.x != q.x) l = q.x;
+    if (id >= 0 && q.x > 0.f)
+      l = q.x * (logf(q.x) - (empty ? -INFINITY : (x - m) * inv_t - logf(st.s)));
+    l = warp_sum(l);
+    if ((t & 31) == 0) loss_part[t >> 5] = l;
 
     // gradient, and the next row's copies
     const float A = empty ? 0.f : w / st.s;
     const long long rn = next_live(r + stride);
-    const T* pn = logits + (size_t)(rn < rows ? rn : r) * ld + a;
-    RowShape sn = row_shape(pn, n);
+    const T* pn = logits + (size_t)(rn < rows ? rn : r) * ld;
+    RowShape sn = row_shape(pn, V);
     if (rn >= rows) sn.nv = sn.head = sn.tail = 0;
     const uint4* nv = reinterpret_cast<const uint4*>(pn + sn.head);
     T* drow = dlogits + (size_t)r * ldd;
-    uint4* dv = reinterpret_cast<uint4*>(drow + a + s.head);
+    uint4* dv = reinterpret_cast<uint4*>(drow + s.head);
     {
       const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), A2 = pair(A, A);
       const int least = min(s.nv, sn.nv);
@@ -525,16 +507,16 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
         cp_async_commit();
       }
       if (t < s.head)
-        drow[a + t] = from_f<T>(grad_value<false>(edge[0], m, c, A, 0.f));
+        drow[t] = from_f<T>(grad_value<false>(edge[0], m, c, A, 0.f));
       if (t < s.tail)
-        drow[a + s.tail0 + t] = from_f<T>(grad_value<false>(edge[1], m, c, A, 0.f));
+        drow[s.tail0 + t] = from_f<T>(grad_value<false>(edge[1], m, c, A, 0.f));
       load_edges(pn, sn);
     }
     __syncthreads();  // listed elements are rounded once, with their own term
-    if (id >= a && id < a + n && q.y > 0.f && !empty)
+    if (id >= 0 && q.y > 0.f && !empty)
       drow[id] = from_f<T>(fmaf(-w, q.y, grad_value<false>(x, m, c, A, 0.f)));
-    if (rank == 0 && t == 0) {
-      float l = 0.f;
+    if (t == 0) {
+      l = 0.f;
       for (int i = 0; i < DF_THREADS / 32; ++i) l += loss_part[i];
       loss[r] = temperature * temperature * l;
       stats[r] = make_float2(m, st.s);
@@ -543,61 +525,49 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
   }
 }
 
-// How the fused kernel shares a row: CTAs a row (0: the row does not fit), the
-// elements of each, and its shared memory.
-struct GradPlan {
-  int cl, share, smem, per_sm;
-};
+constexpr int DF_LONG_THREADS = 1024;
 
-GradPlan grad_plan(int64_t rows, int64_t V, int size) {
-  const int vw = 16 / size, unit = DF_THREADS * 16;
-  GradPlan g;
-  for (g.cl = 1;; g.cl *= 2) {
-    const int64_t share = ((V + g.cl - 1) / g.cl + vw - 1) / vw * vw;
-    const int64_t smem = (share / vw * 16 + unit - 1) / unit * unit;
-    g.share = (int)share;
-    g.smem = (int)std::min<int64_t>(smem, 1 << 30);
-    // three CTAs an SM; a cluster of eight may take all of it
-    const bool fits = smem <= (g.cl == 8 ? 220 : 72) * 1024;
-    const bool idle = rows * g.cl < 148 && share >= 2 * DF_THREADS * vw;
-    if (fits && (!idle || g.cl == 8)) break;
-    if (g.cl == 8) {
-      g.cl = 0;
-      return g;
+template <typename T>
+__global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
+    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
+    T* __restrict__ dlogits, long long ldd) {
+  __shared__ float part[DF_LONG_THREADS / 32][3];
+  const int t = threadIdx.x;
+  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
+  const long long r = blockIdx.x;
+  const T* row = logits + (size_t)r * ld;
+  T* drow = dlogits + (size_t)r * ldd;
+  if (!list.live[r]) {
+    zero_row<T, DF_LONG_THREADS>(drow, V, t);
+    if (t == 0) {
+      loss[r] = 0.f;
+      stats[r] = make_float2(0.f, 0.f);
+    }
+    return;
+  }
+  const Stats all = block_merge<DF_LONG_THREADS>(
+      sweep<T, DF_LONG_THREADS, false>(row, V, t, c), part, c);
+  const float m = finite_max(all.mx);
+  const bool empty = all.s == 0.f;
+  const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
+  const float A = empty ? 0.f : w / all.s;
+  grad_sweep<T, DF_LONG_THREADS, false>(row, drow, V, t, m, c, A, 0.f);
+  if (t < 32) {
+    const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K, t, m,
+                                              inv_t, logf(all.s), empty));
+    if (t == 0) {
+      loss[r] = temperature * temperature * l;
+      stats[r] = make_float2(m, all.s);
     }
   }
-  g.per_sm = std::min(3, 224 * 1024 / (g.smem + 1024));
-  return g;
-}
-
-template <typename T, bool SPLIT>
-int launch_grad(const GradPlan& g, int64_t rows, int64_t V, int64_t ld, const void* logits,
-                int64_t K, const Entries& e, int mean_blocks, float temperature, float* loss,
-                float* stats, void* dlogits, int64_t ldd, cudaStream_t st) {
-  auto kernel = distill_grad_kernel<T, SPLIT>;
-  if (!kernel_prepared((const void*)kernel, g.smem)) return DABSN_ERR_LAUNCH;
-  const int64_t clusters = std::max<int64_t>(1, std::min<int64_t>(rows, 148 * g.per_sm / g.cl));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * g.cl), 1, 1);
-  cfg.blockDim = dim3(DF_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = g.smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = g.cl;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = SPLIT ? 1 : 0;
-  const cudaError_t err = cudaLaunchKernelEx(
-      &cfg, kernel, (long long)rows, (int)V, (long long)ld, (const T*)logits, (int)K, e,
-      mean_blocks, temperature, g.share, loss, (float2*)stats, (T*)dlogits, (long long)ldd);
-  if (err != cudaSuccess) {
-    set_error("distill_grad launch: %s (cluster=%d smem=%d)", cudaGetErrorString(err), g.cl,
-              g.smem);
-    return DABSN_ERR_LAUNCH;
+  __syncthreads();  // listed elements are rounded once, with their own term
+  for (int k = t; k < K && !empty; k += DF_LONG_THREADS) {
+    const int id = list.id[r * K + k];
+    const float q = list.q[r * K + k].y;
+    if (id >= 0 && q > 0.f)
+      drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
   }
-  return DABSN_OK;
 }
 
 // result = sum of the row losses (times 1 / live rows if mean_blocks), in a
@@ -625,7 +595,7 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(long long rows,
 
 int check_distill(const char* what, int dtype, int64_t rows, int64_t V, int64_t ld, int64_t K,
                   float temperature) {
-  if (rows < 0 || V <= 0 || V >= INT32_MAX || ld < V) {
+  if (rows < 0 || rows > INT32_MAX || V <= 0 || V >= INT32_MAX || ld < V) {
     set_error("%s: unsupported sizes rows=%lld V=%lld ld=%lld", what, (long long)rows,
               (long long)V, (long long)ld);
     return DABSN_ERR_SHAPE;
@@ -707,15 +677,21 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
         (float2*)stats, (T*)dlogits, ldd);
     return launch_status("distill_grad");
   }
-  const GradPlan g = grad_plan(rows, V, sizeof(T));
-  if (g.cl == 0) {
-    set_error("distill_grad: a row of %lld logits does not fit", (long long)V);
-    return DABSN_ERR_UNSUPPORTED;
+  const int64_t unit = DF_THREADS * 16;
+  const int64_t smem = (V * (int64_t)sizeof(T) + unit - 1) / unit * unit;
+  if (smem > DF_ROW_BYTES || rows <= 2 * 148) {
+    distill_long_kernel<T><<<row_grid(rows), DF_LONG_THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
+        (float2*)stats, (T*)dlogits, ldd);
+    return launch_status("distill_grad");
   }
-  return g.cl > 1 ? launch_grad<T, true>(g, rows, V, ld, logits, K, e, mean_blocks, temperature,
-                                         row_loss, stats, dlogits, ldd, st)
-                  : launch_grad<T, false>(g, rows, V, ld, logits, K, e, mean_blocks, temperature,
-                                          row_loss, stats, dlogits, ldd, st);
+  if (!kernel_prepared((const void*)distill_grad_kernel<T>, DF_ROW_BYTES))
+    return DABSN_ERR_LAUNCH;
+  const int64_t grid = std::min<int64_t>(rows, 3 * 148);
+  distill_grad_kernel<T><<<(unsigned)grid, DF_THREADS, smem, st>>>(
+      rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
+      (float2*)stats, (T*)dlogits, ldd);
+  return launch_status("distill_grad");
 }
 
 }  // namespace
@@ -731,11 +707,6 @@ extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
   return dtype == DABSN_BF16
              ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st)
              : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st);
-}
-
-extern "C" int dabsn_distill_grad_fits(int dtype, int64_t rows, int64_t V) {
-  if (rows < 0 || V <= 0 || V >= INT32_MAX) return 0;
-  return grad_plan(rows, V, dtype == DABSN_BF16 ? 2 : 4).cl > 0;
 }
 
 extern "C" int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld,

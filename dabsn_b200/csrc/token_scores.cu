@@ -27,6 +27,9 @@ using namespace rowsm;
 typedef unsigned long long u64;
 
 constexpr int TS_THREADS = 256;
+constexpr int TS_FEW_THREADS = 512;
+constexpr int TS_FEW_ROWS = 592;
+constexpr int TS_FEW_BYTES = 16384;
 constexpr int TS_MAX_K = 128;
 constexpr int TS_CAP = 1024;  // candidates of a row
 constexpr int STATUS_BAD_TOKEN = 8;
@@ -314,7 +317,7 @@ __device__ __forceinline__ void token_scores_rows(
       int64_t* ids = top_ids + r * k;
       if (all.s > 0.f) {
         select_top<T, THREADS>(top, row, V, k);
-        rank_found(top, k, [&](int rank, u64 best) {
+        rank_found<THREADS>(top, k, [&](int rank, u64 best) {
           values[rank] = (key_value((unsigned)(best >> 32)) - m) * inv_t - log_s;
           ids[rank] = candidate_index(best);
         });
@@ -329,26 +332,26 @@ __device__ __forceinline__ void token_scores_rows(
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS) token_scores_fwd_kernel(
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) token_scores_fwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits,
     const int64_t* __restrict__ tokens, long long ignore_index, float inv_t,
     float* __restrict__ log_prob, float* __restrict__ entropy, float2* __restrict__ stats,
     int* status) {
-  token_scores_rows<T, TS_THREADS, false>(rows, V, ld, logits, tokens, ignore_index, inv_t, 0,
-                                          log_prob, entropy, stats, nullptr, nullptr, status);
+  token_scores_rows<T, THREADS, false>(rows, V, ld, logits, tokens, ignore_index, inv_t, 0,
+                                       log_prob, entropy, stats, nullptr, nullptr, status);
 }
 
-// Eight CTAs an SM: the selection is a chain of short steps between barriers,
+// 2048 threads an SM: the selection is a chain of short steps between barriers,
 // which only other rows can fill.
-template <typename T>
-__global__ void __launch_bounds__(TS_THREADS, 8) token_scores_top_kernel(
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 2048 / THREADS) token_scores_top_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits,
     const int64_t* __restrict__ tokens, long long ignore_index, float inv_t, int k,
     float* __restrict__ log_prob, float* __restrict__ entropy, float2* __restrict__ stats,
     float* __restrict__ top_values, int64_t* __restrict__ top_ids, int* status) {
-  token_scores_rows<T, TS_THREADS, true>(rows, V, ld, logits, tokens, ignore_index, inv_t, k,
-                                         log_prob, entropy, stats, top_values, top_ids, status);
+  token_scores_rows<T, THREADS, true>(rows, V, ld, logits, tokens, ignore_index, inv_t, k,
+                                      log_prob, entropy, stats, top_values, top_ids, status);
 }
 
 // Rows short enough for one warp: eight a CTA, no barriers.
@@ -439,6 +442,21 @@ int check_rows(const char* what, int dtype, int64_t rows, int64_t V, int64_t ld,
   return DABSN_OK;
 }
 
+template <typename T, int THREADS>
+void launch_rows(int64_t rows, int64_t V, int64_t ld, const void* logits, const int64_t* tokens,
+                 int64_t ignore_index, float inv_t, int64_t k, float* log_prob, float* entropy,
+                 float* stats, float* top_values, int64_t* top_ids, int* status,
+                 cudaStream_t st) {
+  if (k > 0)
+    token_scores_top_kernel<T, THREADS><<<row_grid(rows), THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (int)k, log_prob,
+        entropy, (float2*)stats, top_values, top_ids, status);
+  else
+    token_scores_fwd_kernel<T, THREADS><<<row_grid(rows), THREADS, 0, st>>>(
+        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
+        (float2*)stats, status);
+}
+
 template <typename T>
 int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const int64_t* tokens,
                int64_t ignore_index, float temperature, int64_t k, float* log_prob,
@@ -446,18 +464,16 @@ int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
                cudaStream_t st) {
   const float inv_t = 1.f / temperature;
   int* status = device_status();
-  if (k > 0)
-    token_scores_top_kernel<T><<<row_grid(rows), TS_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (int)k, log_prob,
-        entropy, (float2*)stats, top_values, top_ids, status);
-  else if (V * sizeof(T) <= TS_WARP_BYTES)
+  if (k == 0 && V * sizeof(T) <= TS_WARP_BYTES)
     token_scores_warp_kernel<T><<<warp_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
         (float2*)stats, status);
+  else if (rows <= TS_FEW_ROWS && V * sizeof(T) > TS_FEW_BYTES)
+    launch_rows<T, TS_FEW_THREADS>(rows, V, ld, logits, tokens, ignore_index, inv_t, k,
+                                   log_prob, entropy, stats, top_values, top_ids, status, st);
   else
-    token_scores_fwd_kernel<T><<<row_grid(rows), TS_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
-        (float2*)stats, status);
+    launch_rows<T, TS_THREADS>(rows, V, ld, logits, tokens, ignore_index, inv_t, k, log_prob,
+                               entropy, stats, top_values, top_ids, status, st);
   return launch_status("token_scores_fwd");
 }
 

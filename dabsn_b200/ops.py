@@ -1009,19 +1009,14 @@ def distill_reduce(row_loss: Tensor, lists: Tensor, entries: int, mean: bool) ->
 def distill_gradient(logits: Tensor, lists: Tensor, entries: int, temperature: float,
                      mean: bool):
     """Row losses, statistics and the logits' gradient for the sum (the mean if
-    ``mean``) of the losses, in one pass over the logits; None where a row is
-    too long for it (then :func:`distill_forward` and
-    :func:`distill_backward`)."""
+    ``mean``) of the losses, with one read of the logits from memory."""
     dev = _same_cuda(logits, lists)
     rows, V, ld = _logit_rows(logits)
-    code, lib = act_code(logits.dtype), N.load()
-    if not lib.dabsn_distill_grad_fits(code, rows, V):
-        return None
     loss = torch.empty(rows, device=dev, dtype=torch.float32)
     stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
     dl, ldd = _gradient_rows(logits, ld)
-    _run("distill_grad", dev, lib.dabsn_distill_grad, code, rows, V, ld, logits.data_ptr(),
-         entries, lists.data_ptr(), _temperature(temperature), int(mean), loss.data_ptr(),
+    _run("distill_grad", dev, N.load().dabsn_distill_grad, act_code(logits.dtype), rows, V, ld,
+         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature), int(mean), loss.data_ptr(),
          stats.data_ptr(), dl.data_ptr(), ldd)
     return loss, stats, dl
 

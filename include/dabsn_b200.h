@@ -520,8 +520,8 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  *   at the 16-byte phase of the logits rows, for row weights weight[r *
  *   weight_stride], divided by the same number if `mean`; `unless_one` (one
  *   weight for all rows): dlogits holds the gradient for weight 1 already.
- *   grad: fwd, and the gradient for weight 1, in one pass over the logits, for
- *   rows that dabsn_distill_grad_fits. */
+ *   grad: fwd and the gradient for weight 1 together, with one read of the
+ *   logits from memory. */
 size_t dabsn_distill_list_bytes(int64_t rows, int64_t K);
 int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
                        const int64_t* teacher_tokens, const void* teacher_logits,
@@ -529,7 +529,6 @@ int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
 int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int64_t K, const void* list, float temperature, float* row_loss,
                       float* stats, void* stream);
-int dabsn_distill_grad_fits(int dtype, int64_t rows, int64_t V);
 int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                        int64_t K, const void* list, float temperature, int mean,
                        float* row_loss, float* stats, void* dlogits, int64_t ldd, void* stream);
