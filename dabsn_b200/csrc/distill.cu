@@ -25,7 +25,7 @@ using namespace rowsm;
 
 constexpr int DT_THREADS = 256;
 constexpr int DT_MAX_K = 256;
-constexpr int DT_PREP_THREADS = 256;
+constexpr int DT_PREP_THREADS = 512;
 constexpr int DT_STATUS_BAD_TOKEN = 8;
 
 // Entry of a row's list after preparation: id (-1: absent), q, and q summed
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
     long long rows, int V, int K, const int64_t* __restrict__ ids, const T* __restrict__ logits,
     float inv_t, long long ignore_index, Entries out, int* status) {
   __shared__ int live_rows[DT_PREP_THREADS / 32];
-  constexpr int TABLE = 128 * PER;  // four slots an entry
+  constexpr int TABLE = 64 * PER;  // two slots an entry
   __shared__ int table[DT_PREP_THREADS / 32][TABLE];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long nwarps = (long long)gridDim.x * (DT_PREP_THREADS / 32);
@@ -579,6 +579,7 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(long long rows,
                                                               float* __restrict__ result) {
   __shared__ double sh[32];
   double s = 0.;
+#pragma unroll 8
   for (long long r = threadIdx.x; r < rows; r += 1024) s += (double)loss[r];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);

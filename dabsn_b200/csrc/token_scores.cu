@@ -28,7 +28,7 @@ typedef unsigned long long u64;
 
 constexpr int TS_THREADS = 256;
 constexpr int TS_FEW_THREADS = 512;
-constexpr int TS_FEW_ROWS = 592;
+constexpr int TS_FEW_ROWS = 148;
 constexpr int TS_FEW_BYTES = 16384;
 constexpr int TS_MAX_K = 128;
 constexpr int TS_CAP = 1024;  // candidates of a row
@@ -156,6 +156,38 @@ __device__ __forceinline__ void keep(TopkShared<THREADS>& sh, unsigned key, int 
   if (at < TS_CAP) sh.found[at] = candidate(key, index);
 }
 
+// visit(x, index) for the row's elements from `low` on; four vectors of a
+// thread in flight, those below `low` cost their maximum.
+template <typename T, int THREADS, typename Visit>
+__device__ __forceinline__ void visit_row(const T* p, int n, float low, Visit visit) {
+  constexpr int VW = Vec<T>::N, U = 4;
+  const int t = threadIdx.x;
+  const RowShape r = row_shape(p, n);
+  const uint4* pv = reinterpret_cast<const uint4*>(p + r.head);
+  for (int k0 = t; k0 < r.nv; k0 += U * THREADS) {
+    float top[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * THREADS;
+      constexpr unsigned ni = Vec<T>::kNegInf;
+      const uint4 raw[1] = {k < r.nv ? __ldg(pv + k) : make_uint4(ni, ni, ni, ni)};
+      top[u] = vector_max<T, 1>(raw);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * THREADS;
+      if (k >= r.nv || top[u] < low) continue;
+      for (int j = 0; j < VW; ++j) {
+        const int i = r.head + k * VW + j;
+        const float x = to_f<T>(p[i]);
+        if (x >= low) visit(x, i);
+      }
+    }
+  }
+  if (t < r.head && to_f<T>(p[t]) >= low) visit(to_f<T>(p[t]), t);
+  if (t < r.tail && to_f<T>(p[r.tail0 + t]) >= low) visit(to_f<T>(p[r.tail0 + t]), r.tail0 + t);
+}
+
 // More logits reach the bound than are kept: a flat row, a masked one with
 // fewer than k logits left, one built against the bound.  With the k-th largest
 // key of the threads (or, where too many lie above that too, of the row): what
@@ -169,11 +201,10 @@ __device__ __noinline__ void select_top_slow(TopkShared<THREADS>& sh, const T* p
   unsigned bound = sh.bound;
   auto above = [&](float x, int index) {
     const unsigned key = order_key(x);
-    if (key > bound) keep(sh, key, index);
+    if (key > bound && *(volatile int*)&sh.n_found <= TS_CAP) keep(sh, key, index);
   };
-  const float low = bound == 0u ? -INFINITY : key_value(bound);
   // strictly above, so the next number is where the visit starts
-  visit_parts<T, THREADS>(sh, p, n, sh.n_hot, bound == 0u ? low : key_value(bound + 1u), above);
+  visit_row<T, THREADS>(p, n, bound == 0u ? -INFINITY : key_value(bound + 1u), above);
   __syncthreads();
   if (sh.n_found > TS_CAP) {
     bound = 0;
@@ -192,7 +223,7 @@ __device__ __noinline__ void select_top_slow(TopkShared<THREADS>& sh, const T* p
     __syncthreads();
     if (t == 0) sh.n_found = 0;
     __syncthreads();
-    for (int i = t; i < n; i += THREADS) above(to_f<T>(p[i]), i);
+    visit_row<T, THREADS>(p, n, bound == 0u ? -INFINITY : key_value(bound + 1u), above);
     __syncthreads();
   }
   const int have = sh.n_found, need = k - have;
