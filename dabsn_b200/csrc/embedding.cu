@@ -106,7 +106,10 @@ struct Raw {
 };
 
 // ---------------------------------------------------------------------------
-// Lookup: each CTA copies a group of rows, a thread per vector.
+// Lookup: each CTA copies a group of rows, a thread per unit.  One unit in
+// flight a thread and eight CTAs an SM: 131072 Zipf rows of 2048, FP32 to BF16,
+// in 128 us (100 us of traffic at the copy rate); two or four in flight at fewer
+// CTAs took 158 us.
 // ---------------------------------------------------------------------------
 template <typename TW, typename TO, int W>
 __global__ void __launch_bounds__(EM_THREADS) embedding_fwd_kernel(
@@ -292,12 +295,12 @@ __device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
 
 // ---------------------------------------------------------------------------
 // Sums over runs of equal ids.  Token frequencies are skewed (the first of
-// 32000 Zipf tokens has a tenth of all positions), so the work is cut along
-// the sorted positions, not along the ids: a group of threads sums a chunk of
-// them, one 8-element unit of the columns a thread, and stores every run that
-// lies inside the chunk.  A run that crosses a boundary leaves an FP32 partial
-// sum in each chunk it touches (slot 1 where it begins, slot 0 where it goes
-// on), which the join adds up in order.
+// 32000 Zipf tokens has a seventh of all positions), so the work is cut along
+// the sorted positions, not along the ids: a group of threads sums the runs that
+// begin in a chunk of them, one 16-byte unit of the columns a thread.  A run that
+// ends in the next chunk is summed to its end by the chunk it begins in.  A
+// longer one, which covers a chunk whole, leaves an FP32 partial sum in each
+// chunk it touches, and the join adds those up in order.
 // ---------------------------------------------------------------------------
 struct GradPlan {
   int chunk, chunks;   // sorted positions in a chunk, number of chunks
@@ -308,10 +311,11 @@ struct GradPlan {
   int zero_blocks;
 };
 
-constexpr int GR_CHUNK_MAX = 128;
+constexpr int GR_CHUNK_MAX = 64;
 constexpr int GR_ZERO_ROWS = 32;
-constexpr int GR_JOIN_UNITS = 64;
-constexpr int GR_POSITIONS = 4096;  // of the chunks of a CTA, at most
+constexpr int GR_JOIN_UNITS = 32;
+constexpr int GR_JOIN_CHUNKS = 4;
+constexpr int GR_POSITIONS = 2048;  // of the chunks of a CTA, at most
 
 GradPlan grad_plan(int64_t N, int64_t V, int units) {
   GradPlan g;
@@ -352,50 +356,70 @@ __global__ void __launch_bounds__(EM_THREADS, 4) embedding_grad_kernel(
     }
     return;
   }
-  // the keys and positions of the CTA's chunks, with the keys before and after
-  __shared__ int keys[GR_POSITIONS + 2], places[GR_POSITIONS];
+  // the keys and positions of the CTA's chunks, and of the chunk after them;
+  // the keys from a chunk (and one) before them
+  __shared__ int keys[GR_POSITIONS + 2 * GR_CHUNK_MAX + 2];
+  __shared__ int places[GR_POSITIONS + GR_CHUNK_MAX];
   const int c0 = blockIdx.x * g.groups * g.chunk;
-  const int count = min(g.groups * g.chunk, N - c0);
-  for (int i = t; i < count + 2; i += EM_THREADS) {
-    const int at = c0 + i - 1;
+  const int count = min((g.groups + 1) * g.chunk, N - c0);
+  for (int i = t; i < (g.groups + 2) * g.chunk + 2; i += EM_THREADS) {
+    const int at = c0 - g.chunk - 1 + i;
     keys[i] = at >= 0 && at < N ? key[at] : -1;
-    if (i < count) places[i] = pos[c0 + i];
   }
+  for (int i = t; i < count; i += EM_THREADS) places[i] = pos[c0 + i];
   __syncthreads();
   const int group = t / g.wide;
   const int chunk = blockIdx.x * g.groups + group;
   const int u = blockIdx.y * g.wide + t % g.wide;
   if (group >= g.groups || chunk >= g.chunks || u >= g.units) return;
-  const int i0 = group * g.chunk, i1 = min(i0 + g.chunk, count);
-  const int* k = keys + 1;
-  const int before = k[i0 - 1], after = k[i1];
-  int cur = k[i0];
+  const int C = g.chunk;
+  const int* k = keys + C + 1 + group * C;  // this chunk's keys; from k[-C - 1] to k[2 * C]
+  const int* place = places + group * C;
+  const int end = min(C, N - chunk * C);    // of the chunk
+  // A run that comes in from the chunk before and began there ends there for
+  // this chunk, if it ends here; the same for the run that leaves this chunk.
+  int from = 0, to = end;
+  bool came = k[0] == k[-1], leaves = k[end - 1] == k[end];  // as a partial sum
+  if (came && k[-C - 1] != k[0] && !(k[end - 1] == k[0] && leaves)) {
+    came = false;
+    while (from < end && k[from] == k[-1]) ++from;
+    if (from == end) return;
+  }
+  if (leaves && !(k[0] == k[end - 1] && k[-1] == k[0])) {
+    // it begins here; does it end in the next chunk?
+    const int far = min(2 * C, N - chunk * C);
+    if (k[far - 1] != k[end - 1] || k[far] != k[end - 1]) {
+      leaves = false;
+      while (to < far && k[to] == k[end - 1]) ++to;
+    }
+  }
+  int cur = k[from];
   bool first = true;
   float sum[W];
 #pragma unroll
   for (int j = 0; j < W; ++j) sum[j] = 0.f;
   auto flush = [&](bool last) {
     if (cur >= V) return;
-    const bool began = first && cur == before;
-    const bool goes_on = last && cur == after;
-    if (!began && !goes_on) {
+    if ((first && came) || (last && leaves)) {
+      store_w<W, float>(partial + ((size_t)chunk * 2 + (first && came ? 0 : 1)) * g.units * W +
+                            (size_t)u * W,
+                        sum);
+    } else {
       float out[W];
 #pragma unroll
       for (int j = 0; j < W; ++j) out[j] = sum[j] * scale;
       store_w<W, TW>(dweight + ((size_t)cur * g.units + u) * W, out);
-    } else {
-      store_w<W, float>(partial + (((size_t)chunk * 2 + (began ? 0 : 1)) * g.units + u) * W, sum);
     }
   };
   const TG* column = dout + (size_t)u * W;
-  for (int i = i0; i < i1 && cur < V; i += AHEAD) {
+  for (int i = from; i < to && cur < V; i += AHEAD) {
     Raw<W, TG> v[AHEAD];
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a)
-      if (i + a < i1) v[a].load(column + (size_t)places[i + a] * g.units * W);
+      if (i + a < to) v[a].load(column + (size_t)place[i + a] * g.units * W);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      if (i + a >= i1) break;
+      if (i + a >= to) break;
       if (k[i + a] != cur) {
         flush(false);
         first = false;
@@ -411,61 +435,74 @@ __global__ void __launch_bounds__(EM_THREADS, 4) embedding_grad_kernel(
   flush(true);
 }
 
-// One CTA per chunk and tile of GR_JOIN_UNITS units: where a run begins in the
-// chunk and goes on, adds up its partial sums.  Four threads share a unit, each
-// every fourth partial.
+// One CTA per GR_JOIN_CHUNKS chunks and tile of GR_JOIN_UNITS units: for every
+// run that begins in one of the chunks and covers the next one whole, adds up
+// its partial sums (slot 1 where it begins, slot 0 where it goes on).  Eight
+// threads share a unit, each every eighth partial.
 template <typename TW, int W>
 __global__ void __launch_bounds__(EM_THREADS) embedding_join_kernel(
     int N, int V, GradPlan g, const int* __restrict__ key, const float* __restrict__ partial,
     float scale, TW* __restrict__ dweight) {
   constexpr int SLICES = EM_THREADS / GR_JOIN_UNITS;
   __shared__ float sh[SLICES][GR_JOIN_UNITS * W];
-  const int chunk = blockIdx.x;
-  const int i0 = chunk * g.chunk, i1 = min(i0 + g.chunk, N);
-  if (i1 >= N) return;
-  // read together: a CTA that finds nothing to do costs one round trip
-  const int id = key[i1 - 1], next = key[i1], first = key[i0];
-  const int before = key[max(i0 - 1, 0)], far = key[min(i1 + g.chunk, N) - 1];
-  if (id >= V || next != id) return;                       // nothing goes on
-  if (first == id && i0 > 0 && before == id) return;       // begun earlier
-  // chunks it goes on into (mostly the next one alone): those that begin with
-  // its id, EM_THREADS of them looked at in one round trip
-  int n = 1;
-  if (i1 + g.chunk <= N && far == id) {
-    n = 0;
+  __shared__ int begins[GR_JOIN_CHUNKS];  // id of the long run that begins there, or -1
+  if (threadIdx.x < GR_JOIN_CHUNKS) {
+    const int chunk = blockIdx.x * GR_JOIN_CHUNKS + threadIdx.x;
+    int id = -1;
+    if (chunk < g.chunks) {
+      const long long i0 = (long long)chunk * g.chunk, i1 = i0 + g.chunk, i2 = i1 + g.chunk;
+      if (i2 < N) {
+        const int first = key[i0], before = i0 > 0 ? key[i0 - 1] : -1;
+        const int last = key[i1 - 1], next = key[i1], far = key[i2 - 1], over = key[i2];
+        // leaves this chunk, covers the next and goes on, and began here
+        if (last < V && last == next && last == far && last == over &&
+            !(first == last && before == last))
+          id = last;
+      }
+    }
+    begins[threadIdx.x] = id;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % GR_JOIN_UNITS, slice = threadIdx.x / GR_JOIN_UNITS;
+  const int u = blockIdx.y * GR_JOIN_UNITS + lane;
+  const bool in = u < g.units;
+  for (int b = 0; b < GR_JOIN_CHUNKS; ++b) {
+    const int id = begins[b], chunk = blockIdx.x * GR_JOIN_CHUNKS + b;
+    if (id < 0) continue;
+    // chunks it goes on into: those that begin with its id, EM_THREADS of them
+    // looked at in one round trip
+    int n = 0;
     for (int c = chunk + 1;; c += EM_THREADS) {
       const long long at = ((long long)c + threadIdx.x) * g.chunk;
       const int found = __syncthreads_count(at < N && key[at] == id);
       n += found;
       if (found < EM_THREADS) break;
     }
-  }
-  const int lane = threadIdx.x % GR_JOIN_UNITS, slice = threadIdx.x / GR_JOIN_UNITS;
-  const int u = blockIdx.y * GR_JOIN_UNITS + lane;
-  const bool in = u < g.units;
-  float sum[W];
+    float sum[W];
 #pragma unroll
-  for (int k = 0; k < W; ++k) sum[k] = 0.f;
-  if (in) {
+    for (int k = 0; k < W; ++k) sum[k] = 0.f;
+    if (in) {
 #pragma unroll 8
-    for (int j = slice; j <= n; j += SLICES) {
-      float v[W];
-      load_w<W, float>(
-          partial + (((size_t)(chunk + j) * 2 + (j == 0 ? 1 : 0)) * g.units + u) * W, v);
+      for (int j = slice; j <= n; j += SLICES) {
+        float v[W];
+        load_w<W, float>(
+            partial + (((size_t)(chunk + j) * 2 + (j == 0 ? 1 : 0)) * g.units + u) * W, v);
 #pragma unroll
-      for (int k = 0; k < W; ++k) sum[k] += v[k];
+        for (int k = 0; k < W; ++k) sum[k] += v[k];
+      }
     }
-  }
 #pragma unroll
-  for (int k = 0; k < W; ++k) sh[slice][k * GR_JOIN_UNITS + lane] = sum[k];
-  __syncthreads();
-  if (slice == 0 && in) {
+    for (int k = 0; k < W; ++k) sh[slice][k * GR_JOIN_UNITS + lane] = sum[k];
+    __syncthreads();
+    if (slice == 0 && in) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      for (int o = 1; o < SLICES; ++o) sum[k] += sh[o][k * GR_JOIN_UNITS + lane];
-      sum[k] *= scale;
+      for (int k = 0; k < W; ++k) {
+        for (int o = 1; o < SLICES; ++o) sum[k] += sh[o][k * GR_JOIN_UNITS + lane];
+        sum[k] *= scale;
+      }
+      store_w<W, TW>(dweight + ((size_t)id * g.units + u) * W, sum);
     }
-    store_w<W, TW>(dweight + ((size_t)id * g.units + u) * W, sum);
+    __syncthreads();
   }
 }
 
@@ -490,7 +527,10 @@ int launch_lookup(int64_t N, int64_t V, int64_t D, const int64_t* tokens, const 
                   int64_t ldw, float scale, void* out, cudaStream_t st) {
   const bool vec = D % 8 == 0 && ldw % 8 == 0 && aligned16(weight) && aligned16(out);
   const int units = (int)(vec ? D / 8 : D);
-  const int group = std::max(1, 4 * EM_THREADS / units);
+  // four units a thread where that still fills the SMs, else one row a CTA
+  const bool fills = N * units >= (int64_t)148 * 8 * 4 * EM_THREADS;
+  const int group = fills ? std::max(1, 4 * EM_THREADS / units)
+                          : std::max(1, EM_THREADS / units);
   const unsigned grid = (unsigned)((N + group - 1) / group);
   if (vec)
     embedding_fwd_kernel<TW, TO, 8><<<grid, EM_THREADS, 0, st>>>(
@@ -521,10 +561,11 @@ int launch_grad_w(int64_t N, int64_t V, int units, const int* key, const int* po
   const GradPlan g = grad_plan(N, V, units);
   embedding_grad_kernel<TG, TW, W><<<dim3(g.blocks + g.zero_blocks, g.tiles), EM_THREADS, 0, st>>>(
       (int)N, (int)V, g, key, pos, (const TG*)dout, scale, (TW*)dweight, partial);
-  if (g.chunks > 1)
+  if (g.chunks > 2)  // a run covers a chunk whole and goes on on both sides
     embedding_join_kernel<TW, W>
-        <<<dim3(g.chunks, (units + GR_JOIN_UNITS - 1) / GR_JOIN_UNITS), EM_THREADS, 0, st>>>(
-            (int)N, (int)V, g, key, partial, scale, (TW*)dweight);
+        <<<dim3((g.chunks + GR_JOIN_CHUNKS - 1) / GR_JOIN_CHUNKS,
+                (units + GR_JOIN_UNITS - 1) / GR_JOIN_UNITS),
+           EM_THREADS, 0, st>>>((int)N, (int)V, g, key, partial, scale, (TW*)dweight);
   return launch_status("embedding_bwd");
 }
 

@@ -376,6 +376,33 @@ def test_embedding(lib, N, V, D, wdtype, odtype):
     _near(dw, want, _half_step(wdtype) * 1.01 * want.abs() + U * (n + 1) * size)
 
 
+RUNS = [
+    [1], [64], [65, 1], [32, 32, 32], [31, 1, 64, 2, 95, 33], [1, 63, 1, 64, 1, 65],
+    [16, 32, 16, 32, 64], [200], [31, 97, 1, 1, 30], [5] * 41, [128, 128, 127, 129],
+    [40000], [63, 1, 40000, 64, 65, 127, 129, 192, 2], [33] * 1200, [64] * 520 + [1],
+    [1, 62, 2, 62, 130] * 140,
+]
+
+
+@pytest.mark.parametrize("D", [8, 21, 72])
+@pytest.mark.parametrize("runs", RUNS, ids=lambda r: f"{len(r)}runs{sum(r)}")
+def test_embedding_runs(lib, runs, D):
+    """Numbers of positions per token that begin and end at every place of the
+    pieces that the sums are cut into, absent tokens between them; the sums of
+    small whole numbers are exact."""
+    g = torch.Generator().manual_seed(len(runs))
+    V = 2 * len(runs) + 1
+    tokens = torch.cat([torch.full((n,), 2 * i + 1) for i, n in enumerate(runs)])
+    tokens = tokens[torch.randperm(len(tokens), generator=g)]
+    go = torch.randint(-8, 9, (len(tokens), D), generator=g).float()
+    for dtype in (F32, BF16):
+        w = torch.zeros(V, D, device="cuda", requires_grad=True)
+        out = lib.embedding(tokens.cuda(), w, dtype=dtype)
+        (dw,) = torch.autograd.grad(out, w, go.cuda().to(dtype))
+        want = torch.zeros(V, D).index_add_(0, tokens, go)
+        assert torch.equal(dw.cpu(), want)
+
+
 def test_embedding_views_and_shapes(lib):
     table = torch.randn(50, 40, device="cuda")
     t = torch.randint(0, 50, (3, 4), device="cuda")
