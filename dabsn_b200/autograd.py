@@ -622,12 +622,13 @@ def make_ce_from_logits(original):
 
 class TokenLogProbs(NamedTuple):
     """What :func:`token_log_probs` returns: FP32 numbers shaped like the
-    tokens, and the alternatives with one more axis (int64 ids)."""
+    tokens, and the alternatives with one more axis (int64 ids), None where
+    none were asked for."""
 
     log_prob: Tensor
     entropy: Tensor
-    top_log_probs: Tensor
-    top_tokens: Tensor
+    top_log_probs: Tensor | None
+    top_tokens: Tensor | None
 
 
 def _differentiates(t: Tensor) -> bool:
@@ -682,10 +683,10 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     """Log-probabilities of given tokens under ``softmax(logits / temperature)``.
 
     ``logits`` [..., V] (CUDA, FP32 or BF16; any row stride), ``tokens`` [...]
-    (int64 or int32).  Returns a :class:`TokenLogProbs`: ``log_prob`` and
+    (int64 or int32), ``temperature`` in [1e-6, 1e6].  Returns a :class:`TokenLogProbs`: ``log_prob`` and
     ``entropy`` [...] in FP32, and the ``top_k`` (0 to 128) most likely tokens
-    of every row as ``top_log_probs`` / ``top_tokens`` [..., top_k], most
-    likely first, equal logits by the lower id.  ``log_prob`` and ``entropy``
+    of every row as ``top_log_probs`` / ``top_tokens`` [..., top_k] (None for
+    0), most likely first, equal logits by the lower id.  ``log_prob`` and ``entropy``
     are differentiable in the logits; the alternatives are not.
 
     A row whose token is ``ignore_index`` is not read: log-probability and
@@ -706,15 +707,12 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     else:
         out = ops.token_scores_forward(rows, flat, top_k, temperature, int(ignore_index), False)
     log_prob, entropy = out[:2]
-    if top_k:
-        top_values, top_ids = out[2:4]
-    else:
-        top_values = log_prob.new_empty((flat.shape[0], 0))
-        top_ids = flat.new_empty((flat.shape[0], 0), dtype=torch.int64)
+    top_values, top_ids = out[2:4] if top_k else (None, None)
     if tokens.dim() != 1:
         log_prob, entropy = log_prob.reshape(shape), entropy.reshape(shape)
-        top_values = top_values.reshape(*shape, top_k)
-        top_ids = top_ids.reshape(*shape, top_k)
+        if top_k:
+            top_values = top_values.reshape(*shape, top_k)
+            top_ids = top_ids.reshape(*shape, top_k)
     return TokenLogProbs(log_prob, entropy, top_values, top_ids)
 
 
@@ -728,19 +726,19 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, ignore_index,
                 reduction):
-        entries, mean = teacher_tokens.shape[1], reduction == "mean"
+        entries = teacher_tokens.shape[1]
         lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
                                  ignore_index)
         if reduction == "none":
-            loss, stats = ops.distill_forward(logits, lists, entries, temperature)
+            loss, stats = ops.distill_forward(logits, lists, entries, temperature, reduction)
             ctx.ready = None
         else:
             loss, stats, ctx.ready = ops.distill_gradient(logits, lists, entries, temperature,
-                                                          mean)
+                                                          reduction == "mean")
             ctx.capture = ops.capture_id(logits.device)
         ctx.save_for_backward(logits, lists, stats)
         ctx.meta = (entries, temperature, reduction)
-        return loss if reduction == "none" else ops.distill_reduce(loss, lists, entries, mean)
+        return loss
 
     @staticmethod
     @once_differentiable
@@ -765,7 +763,7 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     ``logits`` [..., V] (CUDA, FP32 or BF16; any row stride),
     ``teacher_tokens`` [..., K] ids (int64 or int32, 1 to 256 a row) and
     ``teacher_logits`` [..., K] (FP32 or BF16; logits or log-probabilities:
-    only their differences count).  Entries whose id is ``ignore_index`` are
+    only their differences count); ``temperature`` in [1e-6, 1e6].  Entries whose id is ``ignore_index`` are
     absent; an id listed twice counts with both its entries.  ``reduction`` is
     "mean" (over the rows that list anything; 0 if none does), "sum" or "none".
     The loss is FP32; the gradient goes to ``logits`` alone, in their dtype.
@@ -798,9 +796,7 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     else:
         lists = ops.distill_prep(teacher_tokens, teacher_logits, rows.shape[1], temperature,
                                  ignore_index)
-        loss, _ = ops.distill_forward(rows, lists, entries, temperature)
-        if reduction != "none":
-            loss = ops.distill_reduce(loss, lists, entries, reduction == "mean")
+        loss, _ = ops.distill_forward(rows, lists, entries, temperature, reduction)
     return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 

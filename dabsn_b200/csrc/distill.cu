@@ -197,6 +197,46 @@ __device__ __forceinline__ float list_loss(const T* row, const int* id, const fl
   return loss;
 }
 
+// 1 / the number of rows with a loss.
+__device__ __forceinline__ float mean_scale(const int* counts, int blocks) {
+  int n = 0;
+  for (int i = threadIdx.x & 31; i < blocks; i += 32) n += counts[i];
+  n = __reduce_add_sync(0xffffffffu, n);
+  return 1.f / (float)max(n, 1);
+}
+
+// result = sum of the row losses, in a fixed order and in 64 bits, or their mean
+// over the live rows if mean_blocks.  A launch of its own: at the end of the
+// persistent kernel below, in its last CTA, the same sum cost that kernel's main
+// loop 100 us of 705.
+__global__ void __launch_bounds__(1024) distill_reduce_kernel(long long rows,
+                                                              const float* __restrict__ loss,
+                                                              const int* __restrict__ counts,
+                                                              int mean_blocks,
+                                                              float* __restrict__ result) {
+  __shared__ double sums[32];
+  const int t = threadIdx.x;
+  double s = 0.;
+  for (long long r = t; r < rows; r += 8 * 1024) {
+    float v[8];
+#pragma unroll
+    for (int a = 0; a < 8; ++a) v[a] = r + a * 1024 < rows ? loss[r + a * 1024] : 0.f;
+#pragma unroll
+    for (int a = 0; a < 8; ++a) s += (double)v[a];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((t & 31) == 0) sums[t >> 5] = s;
+  __syncthreads();
+  if (t < 32) {
+    s = sums[t];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float scale = mean_blocks ? mean_scale(counts, mean_blocks) : 1.f;
+    if (t == 0) *result = (float)(s * (double)scale);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
@@ -226,14 +266,6 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     }
     __syncthreads();
   }
-}
-
-// weight[r * wstride] * (1 / live rows if `mean`) is the weight of row r.
-__device__ __forceinline__ float mean_scale(const int* counts, int blocks) {
-  int n = 0;
-  for (int i = threadIdx.x & 31; i < blocks; i += 32) n += counts[i];
-  n = __reduce_add_sync(0xffffffffu, n);
-  return 1.f / (float)max(n, 1);
 }
 
 // `unless_one`: dlogits holds the gradient for weight 1 already, and a weight of
@@ -280,18 +312,11 @@ constexpr int warp_row() {
 }
 
 template <typename T, bool GRAD>
-__global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
-    long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
-    T* __restrict__ dlogits, long long ldd) {
+__device__ __forceinline__ void distill_warp_row(long long r, int V, const T* row, int K,
+                                                 const Entries& list, float temperature, float w,
+                                                 float* loss, float2* stats, T* drow) {
   const int lane = threadIdx.x & 31;
-  const long long r = (long long)blockIdx.x * (DT_THREADS / 32) + (threadIdx.x >> 5);
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
-  const float w =
-      GRAD ? temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f) : 0.f;
-  if (r >= rows) return;
-  const T* row = logits + (size_t)r * ld;
-  T* drow = GRAD ? dlogits + (size_t)r * ldd : nullptr;
   if (!list.live[r]) {
     if (GRAD) zero_row<T, 32>(drow, V, lane);
     if (lane == 0) {
@@ -341,6 +366,19 @@ __global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
     if (id >= 0 && q > 0.f)
       drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
   }
+}
+
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
+    long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
+    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
+    T* __restrict__ dlogits, long long ldd) {
+  const long long r = (long long)blockIdx.x * (DT_THREADS / 32) + (threadIdx.x >> 5);
+  const float w =
+      GRAD ? temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f) : 0.f;
+  if (r < rows)
+    distill_warp_row<T, GRAD>(r, V, logits + (size_t)r * ld, K, list, temperature, w, loss,
+                              stats, GRAD ? dlogits + (size_t)r * ldd : nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -570,30 +608,6 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
   }
 }
 
-// result = sum of the row losses (times 1 / live rows if mean_blocks), in a
-// fixed order.
-__global__ void __launch_bounds__(1024) distill_reduce_kernel(long long rows,
-                                                              const float* __restrict__ loss,
-                                                              const int* __restrict__ counts,
-                                                              int mean_blocks,
-                                                              float* __restrict__ result) {
-  __shared__ double sh[32];
-  double s = 0.;
-#pragma unroll 8
-  for (long long r = threadIdx.x; r < rows; r += 1024) s += (double)loss[r];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    s = sh[threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float scale = mean_blocks ? mean_scale(counts, mean_blocks) : 1.f;
-    if (threadIdx.x == 0) *result = (float)(s * (double)scale);
-  }
-}
-
 int check_distill(const char* what, int dtype, int64_t rows, int64_t V, int64_t ld, int64_t K,
                   float temperature) {
   if (rows < 0 || rows > INT32_MAX || V <= 0 || V >= INT32_MAX || ld < V) {
@@ -609,8 +623,8 @@ int check_distill(const char* what, int dtype, int64_t rows, int64_t V, int64_t 
     set_error("%s: logits must be FP32 or BF16", what);
     return DABSN_ERR_DTYPE;
   }
-  if (!(temperature > 0.f) || temperature == INFINITY) {
-    set_error("%s: the temperature must be positive and finite", what);
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) {
+    set_error("%s: the temperature must lie in [1e-6, 1e6]", what);
     return DABSN_ERR_UNSUPPORTED;
   }
   return DABSN_OK;
@@ -634,11 +648,7 @@ extern "C" int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, in
                                   void* stream) {
   const int bad = check_distill("distill_prep", teacher_dtype, rows, V, V, K, temperature);
   if (bad) return bad;
-  if (rows == 0) {
-    const Entries e = entries_of(list, 0, K);
-    cudaMemsetAsync(e.counts, 0, sizeof(int), (cudaStream_t)stream);
-    return launch_status("distill_prep");
-  }
+  if (rows == 0) return DABSN_OK;
   const Entries e = entries_of(list, rows, K);
   cudaStream_t st = (cudaStream_t)stream;
   if (teacher_dtype == DABSN_BF16)
@@ -651,6 +661,12 @@ extern "C" int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, in
 }
 
 namespace {
+
+int reduce(int64_t rows, const float* row_loss, const Entries& e, int mean_blocks, float* result,
+           cudaStream_t st) {
+  distill_reduce_kernel<<<1, 1024, 0, st>>>(rows, row_loss, e.counts, mean_blocks, result);
+  return launch_status("distill_reduce");
+}
 
 template <typename T>
 int fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
@@ -699,33 +715,46 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
 
 extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
                                  const void* logits, int64_t K, const void* list,
-                                 float temperature, float* row_loss, float* stats, void* stream) {
+                                 float temperature, int mean, float* row_loss, float* stats,
+                                 float* result, void* stream) {
   const int bad = check_distill("distill_fwd", dtype, rows, V, ld, K, temperature);
   if (bad) return bad;
-  if (rows == 0) return DABSN_OK;
-  const Entries e = entries_of(const_cast<void*>(list), rows, K);
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == DABSN_BF16
-             ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st)
-             : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st);
+  if (rows == 0) {
+    if (result) cudaMemsetAsync(result, 0, sizeof(float), st);
+    return result ? launch_status("distill_fwd") : DABSN_OK;
+  }
+  const Entries e = entries_of(const_cast<void*>(list), rows, K);
+  const int mb = mean ? prep_blocks(rows) : 0;
+  const int status =
+      dtype == DABSN_BF16
+          ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st)
+          : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st);
+  if (status || !result) return status;
+  return reduce(rows, row_loss, e, mb, result, st);
 }
 
 extern "C" int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld,
                                   const void* logits, int64_t K, const void* list,
                                   float temperature, int mean, float* row_loss, float* stats,
-                                  void* dlogits, int64_t ldd, void* stream) {
+                                  float* result, void* dlogits, int64_t ldd, void* stream) {
   int bad = check_distill("distill_grad", dtype, rows, V, ld, K, temperature);
   if (!bad)
     bad = check_gradient_rows("distill_grad", dtype, rows, V, ld, logits, ldd, dlogits);
   if (bad) return bad;
-  if (rows == 0) return DABSN_OK;
-  const Entries e = entries_of(const_cast<void*>(list), rows, K);
   cudaStream_t st = (cudaStream_t)stream;
+  if (rows == 0) {
+    cudaMemsetAsync(result, 0, sizeof(float), st);
+    return launch_status("distill_grad");
+  }
+  const Entries e = entries_of(const_cast<void*>(list), rows, K);
   const int mb = mean ? prep_blocks(rows) : 0;
-  return dtype == DABSN_BF16 ? grad<bf16>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
-                                          stats, dlogits, ldd, st)
-                             : grad<float>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
-                                           stats, dlogits, ldd, st);
+  const int status = dtype == DABSN_BF16
+                         ? grad<bf16>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
+                                      stats, dlogits, ldd, st)
+                         : grad<float>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
+                                       stats, dlogits, ldd, st);
+  return status ? status : reduce(rows, row_loss, e, mb, result, st);
 }
 
 extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
@@ -756,16 +785,4 @@ extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
         rows, (int)V, ld, (const float*)logits, (int)K, e, mb, temperature, (const float2*)stats,
         weight, weight_stride, unless_one != 0, (float*)dlogits, ldd);
   return launch_status("distill_bwd");
-}
-
-extern "C" int dabsn_distill_reduce(int64_t rows, int64_t K, const float* row_loss,
-                                    const void* list, int mean, float* result, void* stream) {
-  if (rows < 0 || K < 1 || K > DT_MAX_K) {
-    set_error("distill_reduce: bad sizes rows=%lld K=%lld", (long long)rows, (long long)K);
-    return DABSN_ERR_SHAPE;
-  }
-  const Entries e = entries_of(const_cast<void*>(list), rows, K);
-  distill_reduce_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(
-      rows, row_loss, e.counts, mean ? prep_blocks(rows) : 0, result);
-  return launch_status("distill_reduce");
 }

@@ -280,6 +280,111 @@ __global__ void __launch_bounds__(EM_THREADS) sort_place_kernel(
   }
 }
 
+// The whole sort of up to RS_SMALL tokens in one CTA and one launch, passes
+// through shared memory: 4099 tokens of 1009 in 6 us, against 13 us in the four
+// launches of two passes.
+constexpr int RS_SMALL_THREADS = 1024;
+constexpr int RS_SMALL_ITEMS = 8;
+constexpr int RS_SMALL = RS_SMALL_THREADS * RS_SMALL_ITEMS;
+constexpr int RS_SMALL_WARPS = RS_SMALL_THREADS / 32;
+constexpr int RS_SMALL_ROW = RS_DIGITS + 1;  // the rows of counts start in other banks
+constexpr int RS_SMALL_SMEM = (2 * RS_SMALL + RS_SMALL_WARPS * RS_SMALL_ROW) * (int)sizeof(int);
+
+__global__ void __launch_bounds__(RS_SMALL_THREADS) sort_small_kernel(
+    int N, int V, long long padding, int passes, int bits, const int64_t* __restrict__ tokens,
+    int* __restrict__ key_out, int* __restrict__ pos_out) {
+  extern __shared__ int small[];
+  int* key = small;                    // [RS_SMALL]
+  int* pos = small + RS_SMALL;         // [RS_SMALL]
+  int* offset = small + 2 * RS_SMALL;  // [RS_SMALL_WARPS][RS_SMALL_ROW]
+  static_assert(RS_SMALL_THREADS == 4 * RS_DIGITS, "four threads a digit");
+  __shared__ int warp_total[RS_SMALL_WARPS];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  // as few items a thread as hold the input, a warp's consecutive
+  const int items = (N + RS_SMALL_THREADS - 1) / RS_SMALL_THREADS;
+  int* mine = offset + warp * RS_SMALL_ROW;
+  int k[RS_SMALL_ITEMS], p[RS_SMALL_ITEMS], rank[RS_SMALL_ITEMS];
+#pragma unroll
+  for (int j = 0; j < RS_SMALL_ITEMS; ++j) {
+    p[j] = (warp * items + j) * 32 + lane;
+    k[j] = j < items && p[j] < N ? sort_key(tokens[p[j]], V, padding) : -1;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits, mask = (1 << bits) - 1;
+    for (int d = t; d < RS_SMALL_WARPS * RS_SMALL_ROW; d += RS_SMALL_THREADS) offset[d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < RS_SMALL_ITEMS; ++j) {
+      if (j >= items) break;
+      const bool in = k[j] >= 0;
+      const int digit = in ? (k[j] >> shift) & mask : RS_DIGITS;
+      const unsigned peers = __match_any_sync(0xffffffffu, digit);
+      const int seen = in ? mine[digit] : 0;
+      rank[j] = seen + __popc(peers & ((1u << lane) - 1));
+      __syncwarp();
+      if (in && (peers >> lane) == 1u) mine[digit] = seen + __popc(peers);
+      __syncwarp();
+    }
+    __syncthreads();
+    // four threads a digit, each a quarter of the warps
+    constexpr int QUARTER = RS_SMALL_WARPS / 4;
+    int* column = offset + (t & 3) * QUARTER * RS_SMALL_ROW + (t >> 2);
+    int n[QUARTER], sum = 0;
+#pragma unroll
+    for (int w = 0; w < QUARTER; ++w) {
+      n[w] = column[w * RS_SMALL_ROW];
+      sum += n[w];
+    }
+    int scan = sum;  // over the digits and quarters before this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) warp_total[warp] = scan;
+    __syncthreads();
+    if (warp == 0) {
+      int all = warp_total[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, all, o);
+        if (lane >= o) all += v;
+      }
+      warp_total[lane] = all;
+    }
+    __syncthreads();
+    int at = scan - sum + (warp > 0 ? warp_total[warp - 1] : 0);
+#pragma unroll
+    for (int w = 0; w < QUARTER; ++w) {
+      column[w * RS_SMALL_ROW] = at;
+      at += n[w];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < RS_SMALL_ITEMS; ++j) {
+      if (j >= items || k[j] < 0) continue;
+      const int dst = mine[(k[j] >> shift) & mask] + rank[j];
+      key[dst] = k[j];
+      pos[dst] = p[j];
+    }
+    __syncthreads();
+    if (pass + 1 < passes) {
+#pragma unroll
+      for (int j = 0; j < RS_SMALL_ITEMS; ++j) {
+        const int i = (warp * items + j) * 32 + lane;
+        const bool in = j < items && i < N;
+        k[j] = in ? key[i] : -1;
+        p[j] = in ? pos[i] : 0;
+      }
+      __syncthreads();
+    }
+  }
+  for (int i = t; i < N; i += RS_SMALL_THREADS) {
+    key_out[i] = key[i];
+    pos_out[i] = pos[i];
+  }
+}
+
 // First sorted element whose key is not below v.
 __device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
   int lo = 0, hi = N;
@@ -625,8 +730,14 @@ extern "C" int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, i
   const SortPlan plan = sort_plan(N, V);
   const SortSpace s = sort_space(workspace, N);
   const int mask = (1 << plan.bits) - 1;
-  const int n = (int)N, v = (int)V;
-  for (int pass = 0; pass < plan.passes && N > 0; ++pass) {
+  const int n = (int)N, v = (int)V, out = (plan.passes - 1) & 1;
+  const bool small = N <= RS_SMALL;
+  if (small && N > 0) {
+    if (!kernel_prepared((const void*)sort_small_kernel, RS_SMALL_SMEM)) return DABSN_ERR_LAUNCH;
+    sort_small_kernel<<<1, RS_SMALL_THREADS, RS_SMALL_SMEM, st>>>(
+        n, v, padding_idx, plan.passes, plan.bits, tokens, s.key[out], s.pos[out]);
+  }
+  for (int pass = 0; pass < plan.passes && !small; ++pass) {
     const int shift = pass * plan.bits, to = pass & 1, from = to ^ 1;
     if (pass == 0) {
       sort_count_kernel<true><<<plan.blocks, EM_THREADS, 0, st>>>(
@@ -642,8 +753,8 @@ extern "C" int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, i
           s.key[to], s.pos[to]);
     }
   }
-  const int* key = s.key[(plan.passes - 1) & 1];
-  const int* pos = s.pos[(plan.passes - 1) & 1];
+  const int* key = s.key[out];
+  const int* pos = s.pos[out];
   float* partial = (float*)((char*)workspace + sort_bytes(N, V));
   if (out_dtype == DABSN_BF16)
     return weight_dtype == DABSN_BF16

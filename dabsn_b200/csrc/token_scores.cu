@@ -466,8 +466,8 @@ int check_rows(const char* what, int dtype, int64_t rows, int64_t V, int64_t ld,
     set_error("%s: logits must be FP32 or BF16", what);
     return DABSN_ERR_DTYPE;
   }
-  if (!(temperature > 0.f) || temperature == INFINITY) {
-    set_error("%s: the temperature must be positive and finite", what);
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) {
+    set_error("%s: the temperature must lie in [1e-6, 1e6]", what);
     return DABSN_ERR_UNSUPPORTED;
   }
   return DABSN_OK;

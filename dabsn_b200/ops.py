@@ -899,8 +899,8 @@ def _gradient_rows(logits: Tensor, ld: int) -> tuple[Tensor, int]:
 
 def _temperature(temperature: float) -> float:
     t = float(temperature)
-    if not (0.0 < t < float("inf")) or not ctypes.c_float(1.0 / t).value < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= t <= 1e6:  # its square and its inverse stay well inside FP32
+        raise ValueError(f"temperature must lie in [1e-6, 1e6], got {temperature}")
     return t
 
 
@@ -984,41 +984,40 @@ def distill_prep(teacher_tokens: Tensor, teacher_logits: Tensor, vocab: int, tem
     return lists
 
 
-def distill_forward(logits: Tensor, lists: Tensor, entries: int, temperature: float):
-    """(row losses [rows] FP32, statistics [rows, 2]) of the student's logits
-    [rows, V] against prepared lists."""
+def distill_forward(logits: Tensor, lists: Tensor, entries: int, temperature: float,
+                    reduction: str):
+    """(loss, statistics [rows, 2]) of the student's logits [rows, V] against
+    prepared lists: FP32 row losses [rows] for
+    reduction "none", else their "sum" or their "mean" over the rows that have
+    one, []."""
     dev = _same_cuda(logits, lists)
     rows, V, ld = _logit_rows(logits)
     loss = torch.empty(rows, device=dev, dtype=torch.float32)
     stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    result = None
+    if reduction != "none":
+        result = torch.empty((), device=dev, dtype=torch.float32)
     _run("distill_fwd", dev, N.load().dabsn_distill_fwd, act_code(logits.dtype), rows, V, ld,
          logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature),
-         loss.data_ptr(), stats.data_ptr())
-    return loss, stats
-
-
-def distill_reduce(row_loss: Tensor, lists: Tensor, entries: int, mean: bool) -> Tensor:
-    """Sum of the row losses, or their mean over the rows that have one; FP32 []."""
-    dev = _same_cuda(row_loss, lists)
-    out = torch.empty((), device=dev, dtype=torch.float32)
-    _run("distill_reduce", dev, N.load().dabsn_distill_reduce, row_loss.shape[0], entries,
-         row_loss.data_ptr(), lists.data_ptr(), int(mean), out.data_ptr())
-    return out
+         int(reduction == "mean"), loss.data_ptr(), stats.data_ptr(), _addr(result),
+         launches=1 if result is None else 2)
+    return (loss if result is None else result), stats
 
 
 def distill_gradient(logits: Tensor, lists: Tensor, entries: int, temperature: float,
                      mean: bool):
-    """Row losses, statistics and the logits' gradient for the sum (the mean if
-    ``mean``) of the losses, with one read of the logits from memory."""
+    """(sum or mean of the row losses, statistics, the logits' gradient of it),
+    with one read of the logits from memory."""
     dev = _same_cuda(logits, lists)
     rows, V, ld = _logit_rows(logits)
     loss = torch.empty(rows, device=dev, dtype=torch.float32)
     stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
+    result = torch.empty((), device=dev, dtype=torch.float32)
     dl, ldd = _gradient_rows(logits, ld)
     _run("distill_grad", dev, N.load().dabsn_distill_grad, act_code(logits.dtype), rows, V, ld,
-         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature), int(mean), loss.data_ptr(),
-         stats.data_ptr(), dl.data_ptr(), ldd)
-    return loss, stats, dl
+         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature), int(mean),
+         loss.data_ptr(), stats.data_ptr(), result.data_ptr(), dl.data_ptr(), ldd, launches=2)
+    return result, stats, dl
 
 
 def distill_backward(logits: Tensor, lists: Tensor, entries: int, temperature: float,
@@ -1077,7 +1076,7 @@ def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: floa
     ws = torch.empty(need, device=dev, dtype=torch.uint8)
     _run("embedding_bwd", dev, lib.dabsn_embedding_bwd, act_code(g.dtype), act_code(dtype), n,
          vocab, D, ids.data_ptr(), -1 if padding_idx is None else padding_idx, g.data_ptr(),
-         scale, dw.data_ptr(), ws.data_ptr(), need)
+         scale, dw.data_ptr(), ws.data_ptr(), need, launches=3 if n <= 8192 else 6)
     return dw
 
 

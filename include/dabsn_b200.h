@@ -490,7 +490,7 @@ uint64_t dabsn_capture_id(void* stream);
 /* Log-probabilities of given tokens, with entropy and top alternatives.
  *   logits [rows, V] FP32/BF16, rows contiguous and `ld` elements apart, any
  *   alignment; tokens [rows] int64 (rows of ignore_index are not read);
- *   temperature > 0; 0 <= top_k <= min(128, V).
+ *   temperature in [1e-6, 1e6]; 0 <= top_k <= min(128, V).
  *   log_prob, entropy [rows] FP32; stats FP32 [rows, 2] (maximum, sum of
  *   exponentials; for the reverse, may be null); top_values FP32 and top_ids
  *   int64 [rows, top_k], most likely first, equal logits by the lower id.
@@ -512,32 +512,31 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  * entries that a row lists (1 <= K <= 256; entries of ignore_index are absent).
  *   prep: teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K] ->
  *   `list`, dabsn_distill_list_bytes(rows, K) bytes, 8-byte aligned, which the
- *   other three read; an id outside [0, V) gives a NaN loss and status 8.
+ *   others read; an id outside [0, V) gives a NaN loss and status 8.
  *   fwd: row_loss [rows], stats [rows, 2] FP32 (stats for the reverse, may be
- *   null).  reduce: result FP32 [1], the sum of the row losses, divided by the
- *   number of rows that list anything if `mean`.
- *   bwd: dlogits [rows, V] in the logits' dtype, rows `ldd` elements apart and
- *   at the 16-byte phase of the logits rows, for row weights weight[r *
- *   weight_stride], divided by the same number if `mean`; `unless_one` (one
- *   weight for all rows): dlogits holds the gradient for weight 1 already.
- *   grad: fwd and the gradient for weight 1 together, with one read of the
- *   logits from memory. */
+ *   null); result FP32 [1] (may be null): the sum of the row losses, divided by
+ *   the number of rows that list anything if `mean`.
+ *   grad: fwd with a result, and its gradient, with one read of the logits from
+ *   memory.  dlogits [rows, V] in the logits' dtype, rows `ldd` elements apart
+ *   and at the 16-byte phase of the logits rows.
+ *   bwd: dlogits for row weights weight[r * weight_stride], divided by the same
+ *   number if `mean`; `unless_one` (one weight for all rows): dlogits holds the
+ *   gradient for weight 1 already. */
 size_t dabsn_distill_list_bytes(int64_t rows, int64_t K);
 int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
                        const int64_t* teacher_tokens, const void* teacher_logits,
                        float temperature, int64_t ignore_index, void* list, void* stream);
 int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
-                      int64_t K, const void* list, float temperature, float* row_loss,
-                      float* stats, void* stream);
+                      int64_t K, const void* list, float temperature, int mean, float* row_loss,
+                      float* stats, float* result, void* stream);
 int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                        int64_t K, const void* list, float temperature, int mean,
-                       float* row_loss, float* stats, void* dlogits, int64_t ldd, void* stream);
+                       float* row_loss, float* stats, float* result, void* dlogits, int64_t ldd,
+                       void* stream);
 int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int64_t K, const void* list, float temperature, const float* stats,
                       int mean, const float* weight, int64_t weight_stride, int unless_one,
                       void* dlogits, int64_t ldd, void* stream);
-int dabsn_distill_reduce(int64_t rows, int64_t K, const float* row_loss, const void* list,
-                         int mean, float* result, void* stream);
 
 /* Scaled embedding lookup: out [N, D] = scale * weight[tokens], weight [V, D]
  * with rows `ldw` elements apart; tables and outputs FP32 or BF16.  A token

@@ -201,7 +201,7 @@ def test_token_log_probs_shapes_and_int32(lib):
     assert a.log_prob.shape == (3, 4) and a.top_tokens.shape == (3, 4, 2)
     assert torch.equal(a.log_prob, b.log_prob) and torch.equal(a.top_tokens, b.top_tokens)
     one = lib.token_log_probs(x[1, 2], t[1, 2])
-    assert one.log_prob.shape == () and one.top_tokens.shape == (0,)
+    assert one.log_prob.shape == () and one.top_tokens is None and one.top_log_probs is None
     assert torch.equal(one.log_prob, a.log_prob[1, 2])
     none = lib.token_log_probs(x[:0], t[:0], top_k=2)
     assert none.log_prob.shape == (0, 4) and none.top_tokens.shape == (0, 4, 2)
@@ -250,6 +250,7 @@ DISTILL_CASES = [
     (7, 4099, 100, "far", 5, 0), (3, 32000, 64, "normal", 0, 0), (2, 32771, 256, "flat", 0, 1),
     (300, 4096, 16, "normal", 0, 0), (1, 128003, 128, "normal", 0, 0), (900, 70, 5, "ties", 0, 0),
     (2, 700001, 4, "normal", 0, 0), (500, 33000, 3, "normal", 0, 0),
+    (301, 4099, 7, "normal", 5, 3), (460, 8191, 5, "masked", 1, 1), (451, 1025, 40, "ties", 0, 0),
 ]
 
 
@@ -542,6 +543,84 @@ def test_on_another_stream_and_in_a_graph(lib):
         for a, b in zip(outs, want2):
             assert torch.equal(a, b)
     assert not torch.equal(want[0], want2[0])
+
+
+def test_reverse_captured_without_its_forward(lib):
+    """A graph that holds a reverse alone, replayed with other upstream
+    gradients: every replay starts from the saved logits, whatever the replay
+    before it left behind."""
+    x = _logits(400, 2000, BF16, 4)
+    ids, tl = _teacher(400, 2000, 6, 4)
+    # a reverse runs on its forward's stream, so that one is the capture's
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaf = x.detach().requires_grad_()
+        loss = lib.distillation_loss(leaf, ids, tl)
+    up = torch.ones((), device="cuda")
+    want = {}
+    for w in (1.0, 0.5, -3.0):
+        a = x.detach().requires_grad_()
+        (want[w],) = torch.autograd.grad(lib.distillation_loss(a, ids, tl), a,
+                                         torch.tensor(w, device="cuda"))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        (dx,) = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+    for w in (1.0, 0.5, 1.0, -3.0, 1.0):
+        up.fill_(w)
+        graph.replay()
+        assert torch.equal(dx, want[w]), w
+    # the eager graph still has its reverse
+    torch.cuda.synchronize()
+    (again,) = torch.autograd.grad(loss, leaf)
+    torch.cuda.synchronize()
+    assert torch.equal(again, want[1.0])
+
+
+def test_changed_logits_are_refused_in_the_reverse(lib):
+    x = _logits(3, 50, F32, 1)
+    for loss in (lambda z: lib.token_log_probs(z, _tokens(3, 50, 1)).log_prob.sum(),
+                 lambda z: lib.distillation_loss(z, *_teacher(3, 50, 2, 1))):
+        base = x.detach().requires_grad_()
+        z = base * 1.0
+        out = loss(z)
+        z.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified"):
+            torch.autograd.grad(out, base)
+
+
+def test_calls_on_two_streams_at_once(lib):
+    """Calls that overlap share nothing: their results are those of calls in a
+    row."""
+    xs = [_logits(300, 9000, BF16, s) for s in (1, 2)]
+    tokens = _tokens(300, 9000, 1)
+    ids, tl = _teacher(300, 9000, 5, 1)
+    w = torch.randn(500, 64, device="cuda")
+    words = torch.randint(0, 500, (20000,), device="cuda")
+    go = torch.randn(20000, 64, device="cuda")
+
+    def step(x):
+        leaf = x.detach().requires_grad_()
+        s = lib.token_log_probs(leaf, tokens, top_k=30)
+        loss = lib.distillation_loss(leaf, ids, tl)
+        (dx,) = torch.autograd.grad(s.entropy.sum() + loss, leaf)
+        table = w.detach().requires_grad_()
+        (dw,) = torch.autograd.grad(lib.embedding(words, table), table, go * x[0, 0].float())
+        return [s.log_prob.detach(), s.top_tokens, loss.detach(), dx, dw]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(3):
+        for i, (x, stream) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(stream):
+                got[i] = step(x)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
 
 
 def test_second_derivatives_are_refused(lib):

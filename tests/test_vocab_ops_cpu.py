@@ -48,7 +48,7 @@ def test_cpu_tensors_are_refused():
         dabsn_b200.embedding(ids, torch.zeros(5, 4))
 
 
-@pytest.mark.parametrize("t", [0.0, -1.0, float("inf"), float("nan"), 1e-45])
+@pytest.mark.parametrize("t", [0.0, -1.0, float("inf"), float("nan"), 1e-45, 1e39, 9e-7, 1.1e6])
 def test_temperatures(t):
     with pytest.raises(ValueError, match="temperature"):
         ops._temperature(t)
@@ -79,19 +79,19 @@ def test_entry_points_check_sizes_before_launching():
     assert scores(k=11) and scores(V=1000, ld=1000, k=129) and scores(k=-1)
 
     def distill(dtype=0, rows=4, V=10, ld=10, K=2, t=1.0):
-        return lib.dabsn_distill_fwd(dtype, rows, V, ld, NULL, K, NULL, f(t), *([NULL] * 3))
+        return lib.dabsn_distill_fwd(dtype, rows, V, ld, NULL, K, NULL, f(t), 1, *([NULL] * 4))
 
     assert distill(rows=0) == 0
     assert distill(K=0) and distill(K=257) and distill(dtype=7) and distill(t=float("inf"))
     assert lib.dabsn_distill_prep(0, 4, 0, 2, NULL, NULL, f(1.0), -100, NULL, NULL)
-    assert lib.dabsn_distill_reduce(-1, 2, NULL, NULL, 1, NULL, NULL)
     def reverse(ld=10, ldd=10, x=0, dx=0, unless_one=0, stride=0):
         return lib.dabsn_distill_bwd(0, 4, 10, ld, x, 2, NULL, f(1.0), NULL, 1, NULL, stride,
                                      unless_one, dx, ldd, NULL)
 
     assert reverse(ld=9) and reverse(ldd=9) and reverse(ldd=11) and reverse(x=16, dx=4)
     assert reverse(unless_one=1, stride=1)
-    assert lib.dabsn_distill_grad(0, 4, 10, 10, 16, 2, NULL, f(1.0), 1, NULL, NULL, 8, 10, NULL)
+    assert lib.dabsn_distill_grad(0, 4, 10, 10, 16, 2, NULL, f(1.0), 1, NULL, NULL, NULL, 8, 10,
+                                  NULL)
     assert b"phase" in lib.dabsn_last_error()
     assert lib.dabsn_token_scores_bwd(0, 4, 10, 10, 16, NULL, -100, f(1.0), *([NULL] * 4), 4, 10,
                                       NULL)
