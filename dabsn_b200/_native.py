@@ -124,17 +124,13 @@ _SIGNATURES = {
     "dabsn_token_scores_bwd": (
         [_i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float] + [_vp] * 5 + [_i64, _vp],
         _i32),
-    "dabsn_distill_list_bytes": ([_i64, _i64], ctypes.c_size_t),
-    "dabsn_distill_prep": (
-        [_i32, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _i64, _vp, _vp], _i32),
+    "dabsn_distill_workspace": ([_i64, _i64], ctypes.c_size_t),
     "dabsn_distill_fwd": (
-        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _i32] + [_vp] * 4, _i32),
+        [_i32, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, ctypes.c_float, _i32]
+        + [_vp] * 4 + [_i64, _vp], _i32),
     "dabsn_distill_bwd": (
-        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _vp, _i32, _vp, _i64, _i32, _vp,
-         _i64, _vp], _i32),
-    "dabsn_distill_grad": (
-        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _i32] + [_vp] * 4
-        + [_i64, _vp], _i32),
+        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _i32, _vp, _i64, _i32, _vp, _i64,
+         _vp], _i32),
     "dabsn_capture_id": ([_vp], ctypes.c_uint64),
     "dabsn_embedding_fwd": (
         [_i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _vp], _i32),

@@ -631,6 +631,18 @@ class TokenLogProbs(NamedTuple):
     top_tokens: Tensor | None
 
 
+def _once_differentiable(backward):
+    """``torch.autograd.function.once_differentiable`` where a graph of the
+    reverse is being recorded; without one there is nothing to guard, and the
+    reverse runs as it is."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 def _differentiates(t: Tensor) -> bool:
     """Whether a call has to record its reverse; without one the operators
     below run their forward directly (a node costs a single token's call more
@@ -655,7 +667,7 @@ class _TokenScores(torch.autograd.Function):
         return log_prob, entropy, top_values, top_ids
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, g_log_prob, g_entropy, *_):
         if g_log_prob is None and g_entropy is None:
             return None, None, None, None, None
@@ -726,30 +738,23 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, ignore_index,
                 reduction):
-        entries = teacher_tokens.shape[1]
-        lists = ops.distill_prep(teacher_tokens, teacher_logits, logits.shape[1], temperature,
-                                 ignore_index)
-        if reduction == "none":
-            loss, stats = ops.distill_forward(logits, lists, entries, temperature, reduction)
-            ctx.ready = None
-        else:
-            loss, stats, ctx.ready = ops.distill_gradient(logits, lists, entries, temperature,
-                                                          reduction == "mean")
-            ctx.capture = ops.capture_id(logits.device)
-        ctx.save_for_backward(logits, lists, stats)
-        ctx.meta = (entries, temperature, reduction)
+        loss, ws, ctx.ready = ops.distill_forward(logits, teacher_tokens, teacher_logits,
+                                                  temperature, ignore_index, reduction,
+                                                  reduction != "none")
+        ctx.save_for_backward(logits, ws)
+        ctx.meta = (teacher_tokens.shape[1], temperature, reduction == "mean",
+                    ops.capture_id(logits.device))
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, grad):
-        logits, lists, stats = ctx.saved_tensors
-        entries, temperature, reduction = ctx.meta
+        logits, ws = ctx.saved_tensors
+        entries, temperature, mean, capture = ctx.meta
         ready, ctx.ready = ctx.ready, None
-        if ready is not None and ctx.capture != ops.capture_id(logits.device):
+        if ready is not None and capture != ops.capture_id(logits.device):
             ready = None
-        dl = ops.distill_backward(logits, lists, entries, temperature, stats,
-                                  reduction == "mean", grad, ready)
+        dl = ops.distill_backward(logits, ws, entries, temperature, mean, grad, ready)
         return dl, None, None, None, None, None
 
 
@@ -794,9 +799,8 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
         loss = _Distillation.apply(rows, teacher_tokens, teacher_logits.detach(), temperature,
                                    ignore_index, reduction)
     else:
-        lists = ops.distill_prep(teacher_tokens, teacher_logits, rows.shape[1], temperature,
-                                 ignore_index)
-        loss, _ = ops.distill_forward(rows, lists, entries, temperature, reduction)
+        loss = ops.distill_forward(rows, teacher_tokens, teacher_logits, temperature,
+                                   ignore_index, reduction)[0]
     return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 
@@ -810,7 +814,7 @@ class _Embedding(torch.autograd.Function):
         return ops.embedding_forward(tokens, weight, scale, dtype)
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
         vocab, scale, padding_idx, wdtype = ctx.meta

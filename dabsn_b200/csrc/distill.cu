@@ -33,8 +33,9 @@ constexpr int DT_STATUS_BAD_TOKEN = 8;
 struct Entries {
   int* id;
   float2* q;
-  int* live;    // [rows] 1 where the row has a loss
-  int* counts;  // [blocks] live rows of each preparation block
+  float2* stats;  // [rows] maximum and sum of exponentials of the student's row
+  int* live;      // [rows] 1 where the row has a loss
+  int* counts;    // [blocks] live rows of each preparation block
 };
 
 int prep_blocks(int64_t rows) {
@@ -42,10 +43,12 @@ int prep_blocks(int64_t rows) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + warps - 1) / warps, 148 * 4));
 }
 
+// The workspace of a call, read again by its reverse.
 Entries entries_of(void* ws, int64_t rows, int64_t K) {
   Entries e;
   e.q = (float2*)ws;
-  e.id = (int*)(e.q + rows * K);
+  e.stats = e.q + rows * K;
+  e.id = (int*)(e.stats + rows);
   e.live = e.id + rows * K;
   e.counts = e.live + rows;
   return e;
@@ -240,14 +243,14 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(long long rows,
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    float temperature, float* __restrict__ loss, float2* __restrict__ stats) {
+    float temperature, float* __restrict__ loss) {
   __shared__ float part[DT_THREADS / 32][3];
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     if (!list.live[r]) {
       if (threadIdx.x == 0) {
         loss[r] = 0.f;
-        if (stats) stats[r] = make_float2(0.f, 0.f);
+        list.stats[r] = make_float2(0.f, 0.f);
       }
       continue;
     }
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
                                                 all.s == 0.f));
       if (threadIdx.x == 0) {
         loss[r] = temperature * temperature * l;
-        if (stats) stats[r] = make_float2(m, all.s);
+        list.stats[r] = make_float2(m, all.s);
       }
     }
     __syncthreads();
@@ -275,8 +278,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, const float2* __restrict__ stats,
-    const float* __restrict__ weight, long long wstride, bool unless_one,
+    int mean_blocks, float temperature, const float* __restrict__ weight, long long wstride, bool unless_one,
     T* __restrict__ dlogits, long long ldd) {
   if (unless_one && *weight == 1.f) return;
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = logits + (size_t)r * ld;
     T* drow = dlogits + (size_t)r * ldd;
-    const float2 ms = stats[r];
+    const float2 ms = list.stats[r];
     if (!list.live[r] || ms.y == 0.f) {
       zero_row<T, DT_THREADS>(drow, V, threadIdx.x);
       continue;
@@ -314,14 +316,14 @@ constexpr int warp_row() {
 template <typename T, bool GRAD>
 __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* row, int K,
                                                  const Entries& list, float temperature, float w,
-                                                 float* loss, float2* stats, T* drow) {
+                                                 float* loss, T* drow) {
   const int lane = threadIdx.x & 31;
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
   if (!list.live[r]) {
     if (GRAD) zero_row<T, 32>(drow, V, lane);
     if (lane == 0) {
       loss[r] = 0.f;
-      if (stats) stats[r] = make_float2(0.f, 0.f);
+      list.stats[r] = make_float2(0.f, 0.f);
     }
     return;
   }
@@ -347,7 +349,7 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
                                             inv_t, logf(st.s), empty));
   if (lane == 0) {
     loss[r] = temperature * temperature * l;
-    if (stats) stats[r] = make_float2(m, st.s);
+    list.stats[r] = make_float2(m, st.s);
   }
   if (!GRAD) return;
   const float A = empty ? 0.f : w / st.s;
@@ -371,14 +373,14 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
-    T* __restrict__ dlogits, long long ldd) {
+    int mean_blocks, float temperature, float* __restrict__ loss, T* __restrict__ dlogits,
+    long long ldd) {
   const long long r = (long long)blockIdx.x * (DT_THREADS / 32) + (threadIdx.x >> 5);
   const float w =
       GRAD ? temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f) : 0.f;
   if (r < rows)
     distill_warp_row<T, GRAD>(r, V, logits + (size_t)r * ld, K, list, temperature, w, loss,
-                              stats, GRAD ? dlogits + (size_t)r * ldd : nullptr);
+                              GRAD ? dlogits + (size_t)r * ldd : nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -425,8 +427,8 @@ __device__ __forceinline__ void cp_async_wait_for(int pending) {
 template <typename T>
 __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
-    T* __restrict__ dlogits, long long ldd) {
+    int mean_blocks, float temperature, float* __restrict__ loss, T* __restrict__ dlogits,
+    long long ldd) {
   extern __shared__ uint4 slots[];  // [vectors of a thread][DF_THREADS]
   __shared__ float part[DF_THREADS / 32][3];
   __shared__ float loss_part[DF_THREADS / 32];
@@ -446,7 +448,7 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
       zero_row<T, DF_THREADS>(dlogits + (size_t)r * ldd, V, t);
       if (t == 0) {
         loss[r] = 0.f;
-        stats[r] = make_float2(0.f, 0.f);
+        list.stats[r] = make_float2(0.f, 0.f);
       }
       r += stride;
     }
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
       l = 0.f;
       for (int i = 0; i < DF_THREADS / 32; ++i) l += loss_part[i];
       loss[r] = temperature * temperature * l;
-      stats[r] = make_float2(m, st.s);
+      list.stats[r] = make_float2(m, st.s);
     }
     r = rn;
   }
@@ -568,8 +570,8 @@ constexpr int DF_LONG_THREADS = 1024;
 template <typename T>
 __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, float2* __restrict__ stats,
-    T* __restrict__ dlogits, long long ldd) {
+    int mean_blocks, float temperature, float* __restrict__ loss, T* __restrict__ dlogits,
+    long long ldd) {
   __shared__ float part[DF_LONG_THREADS / 32][3];
   const int t = threadIdx.x;
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
     zero_row<T, DF_LONG_THREADS>(drow, V, t);
     if (t == 0) {
       loss[r] = 0.f;
-      stats[r] = make_float2(0.f, 0.f);
+      list.stats[r] = make_float2(0.f, 0.f);
     }
     return;
   }
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
                                               inv_t, logf(all.s), empty));
     if (t == 0) {
       loss[r] = temperature * temperature * l;
-      stats[r] = make_float2(m, all.s);
+      list.stats[r] = make_float2(m, all.s);
     }
   }
   __syncthreads();  // listed elements are rounded once, with their own term
@@ -637,61 +639,31 @@ unsigned row_grid(long long rows) { return (unsigned)std::min<long long>(rows, 0
 
 using namespace dabsn;
 
-extern "C" size_t dabsn_distill_list_bytes(int64_t rows, int64_t K) {
-  if (rows < 0 || K < 1) return 0;
-  return (size_t)rows * K * 12 + (size_t)rows * 4 + (size_t)prep_blocks(rows) * 4;
-}
-
-extern "C" int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
-                                  const int64_t* teacher_tokens, const void* teacher_logits,
-                                  float temperature, int64_t ignore_index, void* list,
-                                  void* stream) {
-  const int bad = check_distill("distill_prep", teacher_dtype, rows, V, V, K, temperature);
-  if (bad) return bad;
-  if (rows == 0) return DABSN_OK;
-  const Entries e = entries_of(list, rows, K);
-  cudaStream_t st = (cudaStream_t)stream;
-  if (teacher_dtype == DABSN_BF16)
-    launch_prep<bf16>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
-                      ignore_index, e, st);
-  else
-    launch_prep<float>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
-                       ignore_index, e, st);
-  return launch_status("distill_prep");
-}
-
 namespace {
-
-int reduce(int64_t rows, const float* row_loss, const Entries& e, int mean_blocks, float* result,
-           cudaStream_t st) {
-  distill_reduce_kernel<<<1, 1024, 0, st>>>(rows, row_loss, e.counts, mean_blocks, result);
-  return launch_status("distill_reduce");
-}
 
 template <typename T>
 int fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
-        float temperature, float* row_loss, float* stats, cudaStream_t st) {
+        float temperature, float* row_loss, cudaStream_t st) {
   if (V <= warp_row<T>()) {
     const int64_t grid = (rows + DT_THREADS / 32 - 1) / (DT_THREADS / 32);
     distill_warp_kernel<T, false><<<(unsigned)grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, (int)K, e, 0, temperature, row_loss, (float2*)stats,
-        nullptr, 0);
+        rows, (int)V, ld, (const T*)logits, (int)K, e, 0, temperature, row_loss, nullptr, 0);
   } else {
     distill_fwd_kernel<T><<<row_grid(rows), DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, (int)K, e, temperature, row_loss, (float2*)stats);
+        rows, (int)V, ld, (const T*)logits, (int)K, e, temperature, row_loss);
   }
   return launch_status("distill_fwd");
 }
 
 template <typename T>
 int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
-         float temperature, int mean_blocks, float* row_loss, float* stats, void* dlogits,
-         int64_t ldd, cudaStream_t st) {
+         float temperature, int mean_blocks, float* row_loss, void* dlogits, int64_t ldd,
+         cudaStream_t st) {
   if (V <= warp_row<T>()) {
     const int64_t grid = (rows + DT_THREADS / 32 - 1) / (DT_THREADS / 32);
     distill_warp_kernel<T, true><<<(unsigned)grid, DT_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
-        (float2*)stats, (T*)dlogits, ldd);
+        (T*)dlogits, ldd);
     return launch_status("distill_grad");
   }
   const int64_t unit = DF_THREADS * 16;
@@ -699,7 +671,7 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
   if (smem > DF_ROW_BYTES || rows <= 2 * 148) {
     distill_long_kernel<T><<<row_grid(rows), DF_LONG_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
-        (float2*)stats, (T*)dlogits, ldd);
+        (T*)dlogits, ldd);
     return launch_status("distill_grad");
   }
   if (!kernel_prepared((const void*)distill_grad_kernel<T>, DF_ROW_BYTES))
@@ -707,60 +679,67 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
   const int64_t grid = std::min<int64_t>(rows, 3 * 148);
   distill_grad_kernel<T><<<(unsigned)grid, DF_THREADS, smem, st>>>(
       rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
-      (float2*)stats, (T*)dlogits, ldd);
+      (T*)dlogits, ldd);
   return launch_status("distill_grad");
 }
 
 }  // namespace
 
+extern "C" size_t dabsn_distill_workspace(int64_t rows, int64_t K) {
+  if (rows < 0 || K < 1) return 0;
+  return (size_t)rows * K * 12 + (size_t)rows * 12 + (size_t)prep_blocks(rows) * 4;
+}
+
 extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
-                                 const void* logits, int64_t K, const void* list,
-                                 float temperature, int mean, float* row_loss, float* stats,
-                                 float* result, void* stream) {
-  const int bad = check_distill("distill_fwd", dtype, rows, V, ld, K, temperature);
+                                 const void* logits, int teacher_dtype, int64_t K,
+                                 const int64_t* teacher_tokens, const void* teacher_logits,
+                                 int64_t ignore_index, float temperature, int mean,
+                                 void* workspace, float* row_loss, float* result, void* dlogits,
+                                 int64_t ldd, void* stream) {
+  int bad = check_distill("distill_fwd", dtype, rows, V, ld, K, temperature);
+  if (!bad && teacher_dtype != DABSN_F32 && teacher_dtype != DABSN_BF16) {
+    set_error("distill_fwd: the teacher's logits must be FP32 or BF16");
+    bad = DABSN_ERR_DTYPE;
+  }
+  if (!bad && dlogits) {
+    bad = check_gradient_rows("distill_fwd", dtype, rows, V, ld, logits, ldd, dlogits);
+    if (!bad && !result) {
+      set_error("distill_fwd: a gradient needs the result it belongs to");
+      bad = DABSN_ERR_UNSUPPORTED;
+    }
+  }
   if (bad) return bad;
   cudaStream_t st = (cudaStream_t)stream;
   if (rows == 0) {
     if (result) cudaMemsetAsync(result, 0, sizeof(float), st);
     return result ? launch_status("distill_fwd") : DABSN_OK;
   }
-  const Entries e = entries_of(const_cast<void*>(list), rows, K);
+  const Entries e = entries_of(workspace, rows, K);
+  if (teacher_dtype == DABSN_BF16)
+    launch_prep<bf16>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
+                      ignore_index, e, st);
+  else
+    launch_prep<float>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
+                       ignore_index, e, st);
+  int status = launch_status("distill_prep");
+  if (status) return status;
   const int mb = mean ? prep_blocks(rows) : 0;
-  const int status =
-      dtype == DABSN_BF16
-          ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st)
-          : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, stats, st);
+  const bool bf = dtype == DABSN_BF16;
+  if (dlogits)
+    status = bf ? grad<bf16>(rows, V, ld, logits, K, e, temperature, mb, row_loss, dlogits, ldd, st)
+                : grad<float>(rows, V, ld, logits, K, e, temperature, mb, row_loss, dlogits, ldd,
+                              st);
+  else
+    status = bf ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, st)
+                : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, st);
   if (status || !result) return status;
-  return reduce(rows, row_loss, e, mb, result, st);
-}
-
-extern "C" int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld,
-                                  const void* logits, int64_t K, const void* list,
-                                  float temperature, int mean, float* row_loss, float* stats,
-                                  float* result, void* dlogits, int64_t ldd, void* stream) {
-  int bad = check_distill("distill_grad", dtype, rows, V, ld, K, temperature);
-  if (!bad)
-    bad = check_gradient_rows("distill_grad", dtype, rows, V, ld, logits, ldd, dlogits);
-  if (bad) return bad;
-  cudaStream_t st = (cudaStream_t)stream;
-  if (rows == 0) {
-    cudaMemsetAsync(result, 0, sizeof(float), st);
-    return launch_status("distill_grad");
-  }
-  const Entries e = entries_of(const_cast<void*>(list), rows, K);
-  const int mb = mean ? prep_blocks(rows) : 0;
-  const int status = dtype == DABSN_BF16
-                         ? grad<bf16>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
-                                      stats, dlogits, ldd, st)
-                         : grad<float>(rows, V, ld, logits, K, e, temperature, mb, row_loss,
-                                       stats, dlogits, ldd, st);
-  return status ? status : reduce(rows, row_loss, e, mb, result, st);
+  distill_reduce_kernel<<<1, 1024, 0, st>>>(rows, row_loss, e.counts, mb, result);
+  return launch_status("distill_reduce");
 }
 
 extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
-                                 const void* logits, int64_t K, const void* list,
-                                 float temperature, const float* stats, int mean,
-                                 const float* weight, int64_t weight_stride, int unless_one,
+                                 const void* logits, int64_t K, const void* workspace,
+                                 float temperature, int mean, const float* weight, int64_t weight_stride, int unless_one,
                                  void* dlogits, int64_t ldd, void* stream) {
   int bad = check_distill("distill_bwd", dtype, rows, V, ld, K, temperature);
   if (!bad) bad = check_gradient_rows("distill_bwd", dtype, rows, V, ld, logits, ldd, dlogits);
@@ -770,7 +749,7 @@ extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
     return DABSN_ERR_UNSUPPORTED;
   }
   if (rows == 0) return DABSN_OK;
-  const Entries e = entries_of(const_cast<void*>(list), rows, K);
+  const Entries e = entries_of(const_cast<void*>(workspace), rows, K);
   cudaStream_t st = (cudaStream_t)stream;
   const int mb = mean ? prep_blocks(rows) : 0;
   // a launch that mostly finds nothing to do stays one wave of CTAs
@@ -778,11 +757,9 @@ extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
       unless_one ? (unsigned)std::min<int64_t>(rows, 148 * 8) : row_grid(rows);
   if (dtype == DABSN_BF16)
     distill_bwd_kernel<bf16><<<grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const bf16*)logits, (int)K, e, mb, temperature, (const float2*)stats,
-        weight, weight_stride, unless_one != 0, (bf16*)dlogits, ldd);
+        rows, (int)V, ld, (const bf16*)logits, (int)K, e, mb, temperature, weight, weight_stride, unless_one != 0, (bf16*)dlogits, ldd);
   else
     distill_bwd_kernel<float><<<grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const float*)logits, (int)K, e, mb, temperature, (const float2*)stats,
-        weight, weight_stride, unless_one != 0, (float*)dlogits, ldd);
+        rows, (int)V, ld, (const float*)logits, (int)K, e, mb, temperature, weight, weight_stride, unless_one != 0, (float*)dlogits, ldd);
   return launch_status("distill_bwd");
 }

@@ -960,15 +960,17 @@ def token_scores_backward(logits: Tensor, tokens: Tensor, temperature: float, ig
     return dl
 
 
-def distill_prep(teacher_tokens: Tensor, teacher_logits: Tensor, vocab: int, temperature: float,
-                 ignore_index: int) -> Tensor:
-    """The teacher's lists [rows, K] as probabilities, in the buffer that the
-    distillation kernels read: ids, probabilities, equal ids merged, which rows
-    have a loss, and how many."""
-    dev = _same_cuda(teacher_tokens, teacher_logits)
-    if teacher_tokens.dim() != 2:
-        raise ValueError("teacher_tokens must be [rows, entries]")
-    rows, K = teacher_tokens.shape
+def distill_forward(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor,
+                    temperature: float, ignore_index: int, reduction: str,
+                    gradient: bool = False):
+    """Student's logits [rows, V] against a teacher's lists [rows, K].  Returns
+    (loss, workspace for :func:`distill_backward`, dlogits or None): FP32 row
+    losses [rows] for reduction "none", else their "sum" or their "mean" over
+    the rows that list anything, []; with ``gradient`` (not for "none") the
+    logits' gradient of it too, with one read of the logits from memory."""
+    dev = _same_cuda(logits, teacher_tokens, teacher_logits)
+    rows, V, ld = _logit_rows(logits)
+    K = teacher_tokens.shape[-1]
     if not 1 <= K <= TEACHER_ENTRIES_MAX:
         raise ValueError(f"a teacher's list holds 1 to {TEACHER_ENTRIES_MAX} entries, got {K}")
     ids = _int_rows(teacher_tokens, (rows, K), "teacher_tokens")
@@ -976,70 +978,43 @@ def distill_prep(teacher_tokens: Tensor, teacher_logits: Tensor, vocab: int, tem
         raise ValueError(f"teacher_logits has shape {tuple(teacher_logits.shape)}, expected "
                          f"{(rows, K)}")
     tl = teacher_logits if teacher_logits.is_contiguous() else teacher_logits.contiguous()
-    code, temperature = act_code(tl.dtype), _temperature(temperature)
+    code, teacher, temperature = act_code(logits.dtype), act_code(tl.dtype), _temperature(
+        temperature)
     lib = N.load()
-    lists = torch.empty(lib.dabsn_distill_list_bytes(rows, K), device=dev, dtype=torch.uint8)
-    _run("distill_prep", dev, lib.dabsn_distill_prep, code, rows, vocab, K, ids.data_ptr(),
-         tl.data_ptr(), temperature, ignore_index, lists.data_ptr())
-    return lists
-
-
-def distill_forward(logits: Tensor, lists: Tensor, entries: int, temperature: float,
-                    reduction: str):
-    """(loss, statistics [rows, 2]) of the student's logits [rows, V] against
-    prepared lists: FP32 row losses [rows] for
-    reduction "none", else their "sum" or their "mean" over the rows that have
-    one, []."""
-    dev = _same_cuda(logits, lists)
-    rows, V, ld = _logit_rows(logits)
-    loss = torch.empty(rows, device=dev, dtype=torch.float32)
-    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
-    result = None
+    ws = torch.empty(lib.dabsn_distill_workspace(rows, K), device=dev, dtype=torch.uint8)
+    row_loss = torch.empty(rows, device=dev, dtype=torch.float32)
+    result, dl, ldd = None, None, 0
     if reduction != "none":
         result = torch.empty((), device=dev, dtype=torch.float32)
-    _run("distill_fwd", dev, N.load().dabsn_distill_fwd, act_code(logits.dtype), rows, V, ld,
-         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature),
-         int(reduction == "mean"), loss.data_ptr(), stats.data_ptr(), _addr(result),
-         launches=1 if result is None else 2)
-    return (loss if result is None else result), stats
+        if gradient:
+            dl, ldd = _gradient_rows(logits, ld)
+    _run("distill_grad" if gradient else "distill_fwd", dev, lib.dabsn_distill_fwd, code, rows, V,
+         ld, logits.data_ptr(), teacher, K, ids.data_ptr(), tl.data_ptr(), ignore_index,
+         temperature, reduction == "mean", ws.data_ptr(), row_loss.data_ptr(), _addr(result),
+         _addr(dl), ldd, launches=2 if result is None else 3)
+    return (row_loss if result is None else result), ws, dl
 
 
-def distill_gradient(logits: Tensor, lists: Tensor, entries: int, temperature: float,
-                     mean: bool):
-    """(sum or mean of the row losses, statistics, the logits' gradient of it),
-    with one read of the logits from memory."""
-    dev = _same_cuda(logits, lists)
-    rows, V, ld = _logit_rows(logits)
-    loss = torch.empty(rows, device=dev, dtype=torch.float32)
-    stats = torch.empty((rows, 2), device=dev, dtype=torch.float32)
-    result = torch.empty((), device=dev, dtype=torch.float32)
-    dl, ldd = _gradient_rows(logits, ld)
-    _run("distill_grad", dev, N.load().dabsn_distill_grad, act_code(logits.dtype), rows, V, ld,
-         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature), int(mean),
-         loss.data_ptr(), stats.data_ptr(), result.data_ptr(), dl.data_ptr(), ldd, launches=2)
-    return result, stats, dl
-
-
-def distill_backward(logits: Tensor, lists: Tensor, entries: int, temperature: float,
-                     stats: Tensor, mean: bool, weight: Tensor,
-                     ready: Tensor | None = None) -> Tensor:
+def distill_backward(logits: Tensor, workspace: Tensor, entries: int, temperature: float,
+                     mean: bool, weight: Tensor, ready: Tensor | None = None) -> Tensor:
     """dlogits [rows, V] for row weights ``weight`` ([rows], or [] for all
     rows), divided by the number of rows with a loss if ``mean``.  ``ready``
     holds the gradient for weight 1; it is returned, and written again where
     the (one) weight is another."""
-    dev = _same_cuda(logits, lists, stats, weight)
+    dev = _same_cuda(logits, workspace, weight)
     rows, V, ld = _logit_rows(logits)
     w = _dense_f32(weight)
     dl, ldd = _gradient_rows(logits, ld) if ready is None else (ready, _logit_rows(ready)[2])
     _run("distill_bwd", dev, N.load().dabsn_distill_bwd, act_code(logits.dtype), rows, V, ld,
-         logits.data_ptr(), entries, lists.data_ptr(), _temperature(temperature),
-         stats.data_ptr(), int(mean), w.data_ptr(), int(w.dim() > 0), int(ready is not None),
-         dl.data_ptr(), ldd)
+         logits.data_ptr(), entries, workspace.data_ptr(), temperature, mean, w.data_ptr(),
+         w.dim() > 0, ready is not None, dl.data_ptr(), ldd)
     return dl
 
 
 def capture_id(device: torch.device) -> int:
     """Identity of the CUDA graph capture that the current stream is in (0: none)."""
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
     return N.load().dabsn_capture_id(torch._C._cuda_getCurrentRawStream(device.index))
 
 

@@ -510,33 +510,27 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
 /* Distillation from a teacher's top logits: temperature^2 KL(q || softmax(
  * logits / temperature)), q the softmax of the teacher's logits over the
  * entries that a row lists (1 <= K <= 256; entries of ignore_index are absent).
- *   prep: teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K] ->
- *   `list`, dabsn_distill_list_bytes(rows, K) bytes, 8-byte aligned, which the
- *   others read; an id outside [0, V) gives a NaN loss and status 8.
- *   fwd: row_loss [rows], stats [rows, 2] FP32 (stats for the reverse, may be
- *   null); result FP32 [1] (may be null): the sum of the row losses, divided by
- *   the number of rows that list anything if `mean`.
- *   grad: fwd with a result, and its gradient, with one read of the logits from
- *   memory.  dlogits [rows, V] in the logits' dtype, rows `ldd` elements apart
- *   and at the 16-byte phase of the logits rows.
- *   bwd: dlogits for row weights weight[r * weight_stride], divided by the same
- *   number if `mean`; `unless_one` (one weight for all rows): dlogits holds the
- *   gradient for weight 1 already. */
-size_t dabsn_distill_list_bytes(int64_t rows, int64_t K);
-int dabsn_distill_prep(int teacher_dtype, int64_t rows, int64_t V, int64_t K,
-                       const int64_t* teacher_tokens, const void* teacher_logits,
-                       float temperature, int64_t ignore_index, void* list, void* stream);
+ *   teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K]; an id outside
+ *   [0, V) gives a NaN loss and status 8.
+ *   fwd: row_loss FP32 [rows]; result FP32 [1] (may be null): the sum of the row
+ *   losses, divided by the number of rows that list anything if `mean`; dlogits
+ *   (may be null): the gradient of result, with one read of the logits from
+ *   memory: [rows, V] in the logits' dtype, rows `ldd` elements apart and at the
+ *   16-byte phase of the logits rows.
+ *   bwd, with the fwd's workspace: dlogits for row weights weight[r *
+ *   weight_stride], divided by the same number if `mean`; `unless_one` (one
+ *   weight for all rows): dlogits holds the gradient for weight 1 already.
+ *   `workspace` holds dabsn_distill_workspace(rows, K) bytes, 8-byte aligned. */
+size_t dabsn_distill_workspace(int64_t rows, int64_t K);
 int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
-                      int64_t K, const void* list, float temperature, int mean, float* row_loss,
-                      float* stats, float* result, void* stream);
-int dabsn_distill_grad(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
-                       int64_t K, const void* list, float temperature, int mean,
-                       float* row_loss, float* stats, float* result, void* dlogits, int64_t ldd,
-                       void* stream);
+                      int teacher_dtype, int64_t K, const int64_t* teacher_tokens,
+                      const void* teacher_logits, int64_t ignore_index, float temperature,
+                      int mean, void* workspace, float* row_loss, float* result, void* dlogits,
+                      int64_t ldd, void* stream);
 int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
-                      int64_t K, const void* list, float temperature, const float* stats,
-                      int mean, const float* weight, int64_t weight_stride, int unless_one,
-                      void* dlogits, int64_t ldd, void* stream);
+                      int64_t K, const void* workspace, float temperature, int mean,
+                      const float* weight, int64_t weight_stride, int unless_one, void* dlogits,
+                      int64_t ldd, void* stream);
 
 /* Scaled embedding lookup: out [N, D] = scale * weight[tokens], weight [V, D]
  * with rows `ldw` elements apart; tables and outputs FP32 or BF16.  A token

@@ -78,23 +78,28 @@ def test_entry_points_check_sizes_before_launching():
     assert scores(dtype=2) and scores(t=0.0) and scores(t=float("nan"))
     assert scores(k=11) and scores(V=1000, ld=1000, k=129) and scores(k=-1)
 
-    def distill(dtype=0, rows=4, V=10, ld=10, K=2, t=1.0):
-        return lib.dabsn_distill_fwd(dtype, rows, V, ld, NULL, K, NULL, f(t), 1, *([NULL] * 4))
+    def distill(dtype=0, teacher=0, rows=4, V=10, ld=10, K=2, t=1.0, x=16, dx=None, ldd=10,
+                result=None):
+        return lib.dabsn_distill_fwd(dtype, rows, V, ld, x, teacher, K, NULL, NULL, -100, f(t), 1,
+                                     NULL, NULL, result, dx, ldd, NULL)
 
     assert distill(rows=0) == 0
     assert distill(K=0) and distill(K=257) and distill(dtype=7) and distill(t=float("inf"))
-    assert lib.dabsn_distill_prep(0, 4, 0, 2, NULL, NULL, f(1.0), -100, NULL, NULL)
+    assert distill(teacher=2) and distill(V=0) and distill(ld=9) and distill(rows=2 ** 31)
+    assert distill(dx=16) and b"result" in lib.dabsn_last_error()
+    assert distill(dx=8, result=16) and b"phase" in lib.dabsn_last_error()
+    assert distill(dx=32, result=16, ldd=9) and distill(dx=32, result=16, ldd=11)
+
     def reverse(ld=10, ldd=10, x=0, dx=0, unless_one=0, stride=0):
-        return lib.dabsn_distill_bwd(0, 4, 10, ld, x, 2, NULL, f(1.0), NULL, 1, NULL, stride,
+        return lib.dabsn_distill_bwd(0, 4, 10, ld, x, 2, NULL, f(1.0), 1, NULL, stride,
                                      unless_one, dx, ldd, NULL)
 
     assert reverse(ld=9) and reverse(ldd=9) and reverse(ldd=11) and reverse(x=16, dx=4)
     assert reverse(unless_one=1, stride=1)
-    assert lib.dabsn_distill_grad(0, 4, 10, 10, 16, 2, NULL, f(1.0), 1, NULL, NULL, NULL, 8, 10,
-                                  NULL)
-    assert b"phase" in lib.dabsn_last_error()
     assert lib.dabsn_token_scores_bwd(0, 4, 10, 10, 16, NULL, -100, f(1.0), *([NULL] * 4), 4, 10,
                                       NULL)
+    assert lib.dabsn_distill_workspace(100, 5) >= 100 * 5 * 12
+    assert lib.dabsn_distill_workspace(-1, 5) == 0
 
     def lookup(w=0, o=0, N=4, V=10, D=8, ldw=8):
         return lib.dabsn_embedding_fwd(w, o, N, V, D, NULL, NULL, ldw, f(1.0), NULL, NULL)
