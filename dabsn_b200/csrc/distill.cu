@@ -10,8 +10,11 @@
 // entries; a row without any (or with -inf teacher logits throughout) has no
 // loss, no gradient and no part in the mean.  The lists are small: one warp a
 // row turns them into probabilities once (distill_prep), merges an id that is
-// listed twice, and counts the rows.  What costs is the sweep over the student's logits
-// (row_softmax.cuh), one CTA per row.
+// listed twice, and counts the rows: 32768 lists of 64 in 17 us (8 us of
+// traffic; what it waits for is a list's chain of short steps).  What costs is
+// the sweep over the student's logits (row_softmax.cuh), one CTA per row: the
+// loss alone, of 32768 BF16 rows of 32000 with a twentieth ignored, in 315 us,
+// 6.3 TB/s.
 #include <algorithm>
 
 #include "../../include/dabsn_b200.h"

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_fwd_kernel(
 // input; one launch counts its digits, the next places its elements after
 // those of smaller digits and of earlier blocks.
 // ---------------------------------------------------------------------------
-constexpr int RS_ITEMS = 4;
+constexpr int RS_ITEMS = 4;  // 131072 tokens in 18 us; 20 us with 8, 27 us with 16
 constexpr int RS_UNIT = EM_THREADS * RS_ITEMS;  // elements ranked at a time
 constexpr int RS_MAX_BLOCKS = 256;
 constexpr int RS_DIGITS = 256;
@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(EM_THREADS) sort_place_kernel(
 }
 
 // The whole sort of up to RS_SMALL tokens in one CTA and one launch, passes
-// through shared memory: 4099 tokens of 1009 in 6 us, against 13 us in the four
-// launches of two passes.
+// through shared memory: 4099 tokens of 1009 in 12 us, the device time of the
+// four launches of two passes without the gaps between them.
 constexpr int RS_SMALL_THREADS = 1024;
 constexpr int RS_SMALL_ITEMS = 8;
 constexpr int RS_SMALL = RS_SMALL_THREADS * RS_SMALL_ITEMS;
@@ -407,6 +407,10 @@ __device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
 // longer one, which covers a chunk whole, leaves an FP32 partial sum in each
 // chunk it touches, and the join adds those up in order.
 // ---------------------------------------------------------------------------
+// 131072 Zipf tokens of 32000, width 2048, BF16 gradients into an FP32 table:
+// 147 us for the runs and the absent rows, 27 us for the join (122 us of traffic
+// at the copy rate), 18 us for the sort; one CTA per table row took 7000 us.
+// (chunks of 128 positions: 190 us together).
 struct GradPlan {
   int chunk, chunks;   // sorted positions in a chunk, number of chunks
   int units;           // of the columns

@@ -8,12 +8,22 @@
 //   for the gradients g of log_prob and h of entropy.
 //
 // Forward: one CTA per row, one pass over the logits for the maximum, the sum
-// of exponentials and the sum that the entropy needs (row_softmax.cuh).  The
-// alternatives come out of the same pass: every thread knows the maximum of
+// of exponentials and the sum that the entropy needs (row_softmax.cuh).  What
+// bounds it is HBM, with the exponential unit at three quarters: 16384 BF16 rows
+// of 32000 (a tenth of them ignored) in 160 us, 5.9 TB/s.  A row whose token is
+// ignore_index is not read.
+//
+// The alternatives come out of the same pass: every thread knows the maximum of
 // the part of the row it read, the k-th largest of those maxima bounds the
 // row's k-th largest logit from below, and only the parts whose maximum
-// reaches that bound (about k of THREADS) are read again, out of L2.
-// A row whose token is ignore_index is not read.
+// reaches that bound (about k of 256) are read again, out of L2.  20 of 16384
+// rows of 32000: 232 us.  The selection adds two fifths to a row's instructions
+// in short steps between barriers, so it wants many rows on an SM: 256 threads a
+// row and eight CTAs an SM took 232 us, six 240 us, 128 threads a row 253 us, and
+// the selection left to one warp of the CTA 411 us.
+//
+// Reverse: one sweep that reads the logits and writes their gradient, 6.8 TB/s
+// at the same size (294 us).
 #include <algorithm>
 
 #include "../../include/dabsn_b200.h"
@@ -27,6 +37,10 @@ using namespace rowsm;
 typedef unsigned long long u64;
 
 constexpr int TS_THREADS = 256;
+// Where a call has no more rows than SMs, rows of more than 16 KB go to 512
+// threads each: one BF16 row of 128000 with 20 alternatives in 17 us (23 us with
+// 256), one FP32 row of 32000 in 6.3 us (8.5 us); at 592 rows 256 threads are
+// ahead (12.0 us against 14.1 us for BF16 rows of 32000).
 constexpr int TS_FEW_THREADS = 512;
 constexpr int TS_FEW_ROWS = 148;
 constexpr int TS_FEW_BYTES = 16384;
@@ -56,7 +70,7 @@ struct TopkShared {
   unsigned keys[THREADS];
   short hot[THREADS];
   u64 found[TS_CAP];
-  int n_found, n_equal, n_hot;
+  int n_found, n_hot;
   unsigned bound;
   int warp_count[THREADS / 32];
 };
@@ -385,7 +399,8 @@ __global__ void __launch_bounds__(THREADS, 2048 / THREADS) token_scores_top_kern
                                       log_prob, entropy, stats, top_values, top_ids, status);
 }
 
-// Rows short enough for one warp: eight a CTA, no barriers.
+// Rows short enough for one warp: eight a CTA, no barriers.  2048 FP32 rows of 64
+// in 3.4 us forward and 3.2 us back, against 7.4 and 7.2 us with a CTA a row.
 constexpr int TS_WARP_BYTES = 2048;
 
 template <typename T>
