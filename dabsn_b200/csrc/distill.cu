@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     }
     const T* row = logits + (size_t)r * ld;
     const Stats all =
-        block_merge<DT_THREADS>(sweep<T, DT_THREADS, false>(row, V, threadIdx.x, c), part, c);
+        block_merge<DT_THREADS>(sweep<T, DT_THREADS, false, true>(row, V, threadIdx.x, c), part, c);
     const float m = finite_max(all.mx);
     if (threadIdx.x < 32) {
       const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K,
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
     return;
   }
   const Stats all = block_merge<DF_LONG_THREADS>(
-      sweep<T, DF_LONG_THREADS, false>(row, V, t, c), part, c);
+      sweep<T, DF_LONG_THREADS, false, false>(row, V, t, c), part, c);
   const float m = finite_max(all.mx);
   const bool empty = all.s == 0.f;
   const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);

@@ -97,7 +97,7 @@ struct Raw {
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (W > 1) {
       static_assert(W * sizeof(T) == 16, "16 bytes");
-      *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(p));
+      *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(p));  // read once
     } else {
       v[0] = __ldg(p);
     }
@@ -409,8 +409,8 @@ __device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
 // ---------------------------------------------------------------------------
 // 131072 Zipf tokens of 32000, width 2048, BF16 gradients into an FP32 table:
 // 147 us for the runs and the absent rows, 27 us for the join (122 us of traffic
-// at the copy rate), 18 us for the sort; one CTA per table row took 7000 us.
-// (chunks of 128 positions: 190 us together).
+// at the copy rate; chunks of 128 positions: 190 us together), 18 us for the
+// sort.  One CTA per table row took 7000 us.
 struct GradPlan {
   int chunk, chunks;   // sorted positions in a chunk, number of chunks
   int units;           // of the columns

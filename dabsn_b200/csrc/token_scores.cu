@@ -10,20 +10,20 @@
 // Forward: one CTA per row, one pass over the logits for the maximum, the sum
 // of exponentials and the sum that the entropy needs (row_softmax.cuh).  What
 // bounds it is HBM, with the exponential unit at three quarters: 16384 BF16 rows
-// of 32000 (a tenth of them ignored) in 160 us, 5.9 TB/s.  A row whose token is
+// of 32000 (a tenth of them ignored) in 155 us, 6.1 TB/s.  A row whose token is
 // ignore_index is not read.
 //
 // The alternatives come out of the same pass: every thread knows the maximum of
 // the part of the row it read, the k-th largest of those maxima bounds the
 // row's k-th largest logit from below, and only the parts whose maximum
 // reaches that bound (about k of 256) are read again, out of L2.  20 of 16384
-// rows of 32000: 232 us.  The selection adds two fifths to a row's instructions
+// rows of 32000: 233 us.  The selection adds two fifths to a row's instructions
 // in short steps between barriers, so it wants many rows on an SM: 256 threads a
 // row and eight CTAs an SM took 232 us, six 240 us, 128 threads a row 253 us, and
 // the selection left to one warp of the CTA 411 us.
 //
 // Reverse: one sweep that reads the logits and writes their gradient, 6.8 TB/s
-// at the same size (294 us).
+// at the same size (294 to 299 us).
 #include <algorithm>
 
 #include "../../include/dabsn_b200.h"
@@ -350,7 +350,7 @@ __device__ __forceinline__ void token_scores_rows(
       continue;
     }
     const T* row = logits + (size_t)r * ld;
-    const Stats own = sweep<T, THREADS, true>(row, V, threadIdx.x, c);
+    const Stats own = sweep<T, THREADS, true, !TOP>(row, V, threadIdx.x, c);
     if (TOP) offer_part<T, THREADS>(top, row, V, own.mx);
     const Stats all = block_merge<THREADS>(own, part, c);
     if (threadIdx.x == 0)
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_warp_kernel(
   const long long t = tokens[r];
   Stats all;
   const T* row = logits + (size_t)r * ld;
-  if (t != ignore_index) all = warp_merge(sweep<T, 32, true>(row, V, lane, c), c);
+  if (t != ignore_index) all = warp_merge(sweep<T, 32, true, true>(row, V, lane, c), c);
   if (lane == 0)
     write_scores(all, row, t, V, t == ignore_index, inv_t, log_prob + r, entropy + r,
                  stats ? stats + r : nullptr, status);
