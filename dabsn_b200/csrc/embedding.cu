@@ -106,10 +106,11 @@ struct Raw {
 };
 
 // ---------------------------------------------------------------------------
-// Lookup: each CTA copies a group of rows, a thread per unit.  One unit in
-// flight a thread and eight CTAs an SM: 131072 Zipf rows of 2048, FP32 to BF16,
-// in 128 us (100 us of traffic at the copy rate); two or four in flight at fewer
-// CTAs took 158 us.
+// Lookup: each CTA copies a group of rows, a thread per unit.  131072 Zipf rows
+// of 2048, FP32 to BF16, in 121 us (100 us of traffic at the copy rate) with one
+// unit in flight a thread, eight CTAs an SM and eight units a thread; 127 us with
+// four units a thread, 178 us with one, and 158 us with two or four in flight at
+// four CTAs an SM.
 // ---------------------------------------------------------------------------
 template <typename TW, typename TO, int W>
 __global__ void __launch_bounds__(EM_THREADS) embedding_fwd_kernel(
@@ -408,9 +409,8 @@ __device__ __forceinline__ int lower_bound(const int* key, int N, int v) {
 // chunk it touches, and the join adds those up in order.
 // ---------------------------------------------------------------------------
 // 131072 Zipf tokens of 32000, width 2048, BF16 gradients into an FP32 table:
-// 147 us for the runs and the absent rows, 27 us for the join (122 us of traffic
-// at the copy rate; chunks of 128 positions: 190 us together), 18 us for the
-// sort.  One CTA per table row took 7000 us.
+// 141 us for the runs and the absent rows, 17 us for the join (122 us of traffic
+// at the copy rate), 18 us for the sort.  One CTA per table row took 7000 us.
 struct GradPlan {
   int chunk, chunks;   // sorted positions in a chunk, number of chunks
   int units;           // of the columns
@@ -423,7 +423,8 @@ struct GradPlan {
 constexpr int GR_CHUNK_MAX = 64;
 constexpr int GR_ZERO_ROWS = 32;
 constexpr int GR_JOIN_UNITS = 32;
-constexpr int GR_JOIN_CHUNKS = 4;
+constexpr int GR_JOIN_CHUNKS = 8;
+constexpr int GR_JOIN_AHEAD = 4;  // partial sums in flight a thread
 constexpr int GR_POSITIONS = 2048;  // of the chunks of a CTA, at most
 
 GradPlan grad_plan(int64_t N, int64_t V, int units) {
@@ -590,14 +591,20 @@ __global__ void __launch_bounds__(EM_THREADS) embedding_join_kernel(
     float sum[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) sum[k] = 0.f;
-    if (in) {
-#pragma unroll 8
-      for (int j = slice; j <= n; j += SLICES) {
-        float v[W];
-        load_w<W, float>(
-            partial + (((size_t)(chunk + j) * 2 + (j == 0 ? 1 : 0)) * g.units + u) * W, v);
+    for (int j0 = slice; in && j0 <= n; j0 += GR_JOIN_AHEAD * SLICES) {
+      float v[GR_JOIN_AHEAD][W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) sum[k] += v[k];
+      for (int a = 0; a < GR_JOIN_AHEAD; ++a) {
+        const int j = j0 + a * SLICES;
+        if (j <= n)
+          load_w<W, float>(
+              partial + (((size_t)(chunk + j) * 2 + (j == 0 ? 1 : 0)) * g.units + u) * W, v[a]);
+      }
+#pragma unroll
+      for (int a = 0; a < GR_JOIN_AHEAD; ++a) {
+        if (j0 + a * SLICES > n) break;
+#pragma unroll
+        for (int k = 0; k < W; ++k) sum[k] += v[a][k];
       }
     }
 #pragma unroll
@@ -636,9 +643,9 @@ int launch_lookup(int64_t N, int64_t V, int64_t D, const int64_t* tokens, const 
                   int64_t ldw, float scale, void* out, cudaStream_t st) {
   const bool vec = D % 8 == 0 && ldw % 8 == 0 && aligned16(weight) && aligned16(out);
   const int units = (int)(vec ? D / 8 : D);
-  // four units a thread where that still fills the SMs, else one row a CTA
-  const bool fills = N * units >= (int64_t)148 * 8 * 4 * EM_THREADS;
-  const int group = fills ? std::max(1, 4 * EM_THREADS / units)
+  // eight units a thread where that still fills the SMs, else one
+  const bool fills = N * units >= (int64_t)148 * 8 * 8 * EM_THREADS;
+  const int group = fills ? std::max(1, 8 * EM_THREADS / units)
                           : std::max(1, EM_THREADS / units);
   const unsigned grid = (unsigned)((N + group - 1) / group);
   if (vec)
