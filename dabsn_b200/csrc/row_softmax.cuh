@@ -49,8 +49,8 @@ __device__ __forceinline__ float scaled_gap(float x, float m, float c) {
 // arrive at 11.6 elements a clock and SM at the memory's rate, which leaves 11
 // issue slots an element and keeps the exponential unit (16 a clock) busy for
 // 73 % of the time; with scalar arithmetic and a rescaling per vector the sweep
-// of token_scores took 194 us where it takes 160.  (Moving a quarter of the
-// exponentials to a polynomial on the FMA pipes changed nothing: 178 us.)
+// of token_scores took 194 us where it takes 155.  (A quarter of the exponentials
+// as a polynomial on the FMA pipes: 179 us where it took 170.)
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) {
   f32x2 r;
