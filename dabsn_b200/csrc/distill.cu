@@ -32,7 +32,8 @@ constexpr int DT_PREP_THREADS = 512;
 constexpr int DT_STATUS_BAD_TOKEN = 8;
 
 // Entry of a row's list after preparation: id (-1: absent), q, and q summed
-// over the entries with the same id (at the first of them; 0 at the others).
+// over the entries with the same id (at the first of them; 0 at the others; NaN
+// among the teacher's logits makes both NaN, and with them loss and gradient).
 struct Entries {
   int* id;
   float2* q;
@@ -258,8 +259,8 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
       continue;
     }
     const T* row = logits + (size_t)r * ld;
-    const Stats all =
-        block_merge<DT_THREADS>(sweep<T, DT_THREADS, false, true>(row, V, threadIdx.x, c), part, c);
+    const Stats all = block_merge<DT_THREADS>(
+        sweep<T, DT_THREADS, false, true>(row, V, threadIdx.x, c), part, c);
     const float m = finite_max(all.mx);
     if (threadIdx.x < 32) {
       const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K,
@@ -281,8 +282,8 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, const float* __restrict__ weight, long long wstride, bool unless_one,
-    T* __restrict__ dlogits, long long ldd) {
+    int mean_blocks, float temperature, const float* __restrict__ weight, long long wstride,
+    bool unless_one, T* __restrict__ dlogits, long long ldd) {
   if (unless_one && *weight == 1.f) return;
   const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
   const float scale = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     for (int k = threadIdx.x; k < K; k += DT_THREADS) {
       const int id = list.id[r * K + k];
       const float q = list.q[r * K + k].y;
-      if (id >= 0 && q > 0.f)
+      if (id >= 0 && !(q <= 0.f))
         drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), ms.x, c, A, 0.f)));
     }
   }
@@ -368,7 +369,7 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
   for (int k = lane; k < K && !empty; k += 32) {
     const int id = list.id[r * K + k];
     const float q = list.q[r * K + k].y;
-    if (id >= 0 && q > 0.f)
+    if (id >= 0 && !(q <= 0.f))
       drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
   }
 }
@@ -556,7 +557,7 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
       load_edges(pn, sn);
     }
     __syncthreads();  // listed elements are rounded once, with their own term
-    if (id >= 0 && q.y > 0.f && !empty)
+    if (id >= 0 && !(q.y <= 0.f) && !empty)
       drow[id] = from_f<T>(fmaf(-w, q.y, grad_value<false>(x, m, c, A, 0.f)));
     if (t == 0) {
       l = 0.f;
@@ -608,7 +609,7 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
   for (int k = t; k < K && !empty; k += DF_LONG_THREADS) {
     const int id = list.id[r * K + k];
     const float q = list.q[r * K + k].y;
-    if (id >= 0 && q > 0.f)
+    if (id >= 0 && !(q <= 0.f))
       drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
   }
 }

@@ -330,6 +330,62 @@ def test_distillation(lib, rows, V, K, kind, pad, offset, dtype):
     _near(dx, grad * w.double()[:, None], gtol * w.double().abs()[:, None] * 1.01 + 1e-37)
 
 
+@pytest.mark.parametrize("rows,V", [(4, 60), (4, 9000), (450, 9000)])
+def test_distillation_of_non_finite_numbers(lib, rows, V):
+    """Each row by itself: NaN or +inf of the teacher, NaN of the student, all
+    logits of the student masked, one listed token masked."""
+    x = _logits(rows, V, F32, 1)
+    ids = torch.arange(6, device="cuda").repeat(rows, 1)
+    tl = torch.randn(rows, 6, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    tl[0, 2] = math.nan
+    tl[1, 3] = math.inf
+    x[2, V - 1] = math.nan
+    x[3] = -math.inf
+    if rows > 4:
+        x[4, 5] = -math.inf
+    leaf = x.detach().requires_grad_()
+    loss = lib.distillation_loss(leaf, ids, tl, reduction="none")
+    assert loss[:3].isnan().all() and loss[3] == math.inf
+    total = lib.distillation_loss(leaf, ids, tl, reduction="sum")
+    for grad in (torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0],
+                 torch.autograd.grad(total, leaf)[0]):
+        assert grad[0, :6].isnan().any() and grad[1, :6].isnan().any()
+        assert grad[2].isnan().all()
+        assert float(grad[3].abs().max()) == 0.0
+        if rows > 4:
+            assert loss[4] == math.inf and torch.isfinite(grad[4:]).all()
+            assert torch.isfinite(loss[5:]).all()
+
+
+def test_refusals(lib):
+    x, t = _logits(3, 200, F32, 1), _tokens(3, 200, 1)
+    ids, tl = _teacher(3, 200, 4, 1)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        lib.token_log_probs(x.half(), t)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        lib.distillation_loss(x.double(), ids, tl)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        lib.distillation_loss(x, ids, tl.half())
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        lib.embedding(t.clamp(min=0), torch.zeros(200, 8, device="cuda"), dtype=torch.float16)
+    with pytest.raises(TypeError, match="int64 or int32"):
+        lib.token_log_probs(x, t.float())
+    with pytest.raises(TypeError, match="int64 or int32"):
+        lib.embedding(t.short(), torch.zeros(200, 8, device="cuda"))
+    with pytest.raises(ValueError, match="top_k"):
+        lib.token_log_probs(x, t, top_k=129)
+    with pytest.raises(ValueError, match="top_k"):
+        lib.token_log_probs(x[:, :7], t.clamp(max=6), top_k=8)
+    with pytest.raises(ValueError, match="entries"):
+        lib.distillation_loss(x, ids.repeat(1, 65), tl.repeat(1, 65))
+    with pytest.raises(ValueError, match="temperature"):
+        lib.distillation_loss(x, ids, tl, temperature=0.0)
+    with pytest.raises(ValueError, match="same device"):
+        lib.token_log_probs(x, t.cpu())
+    with pytest.raises(ValueError, match="same device"):
+        lib.embedding(t.cpu(), torch.zeros(200, 8, device="cuda"))
+
+
 def test_distillation_of_nothing(lib):
     x = _logits(3, 40, BF16, 1).requires_grad_()
     ids = torch.full((3, 2), -100, device="cuda")
