@@ -126,11 +126,11 @@ _SIGNATURES = {
         _i32),
     "dabsn_distill_workspace": ([_i64, _i64], ctypes.c_size_t),
     "dabsn_distill_fwd": (
-        [_i32, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, ctypes.c_float, _i32]
-        + [_vp] * 4 + [_i64, _vp], _i32),
+        [_i32, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, ctypes.c_float, ctypes.c_float,
+         _i32] + [_vp] * 4 + [_i64, _vp], _i32),
     "dabsn_distill_bwd": (
-        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, _i32, _vp, _i64, _i32, _vp, _i64,
-         _vp], _i32),
+        [_i32, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float, ctypes.c_float, _i32, _vp, _i64,
+         _i32, _vp, _i64, _vp], _i32),
     "dabsn_capture_id": ([_vp], ctypes.c_uint64),
     "dabsn_embedding_fwd": (
         [_i32, _i32, _i64, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _vp, _vp], _i32),

@@ -695,11 +695,12 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     """Log-probabilities of given tokens under ``softmax(logits / temperature)``.
 
     ``logits`` [..., V] (CUDA, FP32 or BF16; any row stride), ``tokens`` [...]
-    (int64 or int32), ``temperature`` in [1e-6, 1e6].  Returns a :class:`TokenLogProbs`: ``log_prob`` and
-    ``entropy`` [...] in FP32, and the ``top_k`` (0 to 128) most likely tokens
-    of every row as ``top_log_probs`` / ``top_tokens`` [..., top_k] (None for
-    0), most likely first, equal logits by the lower id.  ``log_prob`` and ``entropy``
-    are differentiable in the logits; the alternatives are not.
+    (int64 or int32), ``temperature`` in [1e-6, 1e6].  Returns a
+    :class:`TokenLogProbs`: ``log_prob`` and ``entropy`` [...] in FP32, and the
+    ``top_k`` (0 to 128) most likely tokens of every row as ``top_log_probs`` /
+    ``top_tokens`` [..., top_k] (None for 0), most likely first, equal logits by
+    the lower id.  ``log_prob`` and ``entropy`` are differentiable in the
+    logits; the alternatives are not.
 
     A row whose token is ``ignore_index`` is not read: log-probability and
     entropy 0, alternatives -inf with id -1, no gradient.  A row whose logits
@@ -736,42 +737,47 @@ class _Distillation(torch.autograd.Function):
     one captured in another graph than the forward, starts from the logits."""
 
     @staticmethod
-    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, ignore_index,
+    def forward(ctx, logits, teacher_tokens, teacher_logits, temperature, weight, ignore_index,
                 reduction):
         loss, ws, ctx.ready = ops.distill_forward(logits, teacher_tokens, teacher_logits,
-                                                  temperature, ignore_index, reduction,
+                                                  temperature, weight, ignore_index, reduction,
                                                   reduction != "none")
         ctx.save_for_backward(logits, ws)
-        ctx.meta = (teacher_tokens.shape[1], temperature, reduction == "mean",
-                    ops.capture_id(logits.device))
+        ctx.meta = (teacher_tokens.shape[1], temperature, weight, reduction == "mean")
+        ctx.capture = ops.capture_id(logits.device)
         return loss
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, grad):
         logits, ws = ctx.saved_tensors
-        entries, temperature, mean, capture = ctx.meta
         ready, ctx.ready = ctx.ready, None
-        if ready is not None and capture != ops.capture_id(logits.device):
+        if ready is not None and ctx.capture != ops.capture_id(logits.device):
             ready = None
-        dl = ops.distill_backward(logits, ws, entries, temperature, mean, grad, ready)
-        return dl, None, None, None, None, None
+        dl = ops.distill_backward(logits, ws, *ctx.meta, grad, ready)
+        return dl, None, None, None, None, None, None
 
 
 def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor, *,
-                      temperature: float = 1.0, ignore_index: int = -100,
+                      temperature: float = 1.0, weight: float = 1.0, ignore_index: int = -100,
                       reduction: str = "mean") -> Tensor:
     """Distillation from a teacher's top logits:
-    ``temperature^2 * KL(q || softmax(logits / temperature))`` with ``q`` the
-    softmax of ``teacher_logits / temperature`` over the entries a row lists.
+    ``weight * temperature^2 * KL(q || softmax(logits / temperature))`` with
+    ``q`` the softmax of ``teacher_logits / temperature`` over the entries a row
+    lists.
 
     ``logits`` [..., V] (CUDA, FP32 or BF16; any row stride),
     ``teacher_tokens`` [..., K] ids (int64 or int32, 1 to 256 a row) and
     ``teacher_logits`` [..., K] (FP32 or BF16; logits or log-probabilities:
-    only their differences count); ``temperature`` in [1e-6, 1e6].  Entries whose id is ``ignore_index`` are
-    absent; an id listed twice counts with both its entries.  ``reduction`` is
+    only their differences count); ``temperature`` in [1e-6, 1e6].  Entries
+    whose id is ``ignore_index`` are absent; an id listed twice counts with both
+    its entries.  ``reduction`` is
     "mean" (over the rows that list anything; 0 if none does), "sum" or "none".
     The loss is FP32; the gradient goes to ``logits`` alone, in their dtype.
+    It is computed with the loss, for an upstream gradient of 1; another one
+    costs a second pass over the logits, which a factor known beforehand (its
+    share in a sum of losses, one over the number of accumulated steps) avoids
+    as ``weight``.
 
     A row that lists nothing, or whose teacher logits are all -inf, has loss 0
     and no gradient, and its logits are not read.  A listed token whose logit
@@ -798,10 +804,10 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     ignore_index = int(ignore_index)
     if _differentiates(rows):
         loss = _Distillation.apply(rows, teacher_tokens, teacher_logits.detach(), temperature,
-                                   ignore_index, reduction)
+                                   float(weight), ignore_index, reduction)
     else:
         loss = ops.distill_forward(rows, teacher_tokens, teacher_logits, temperature,
-                                   ignore_index, reduction)[0]
+                                   float(weight), ignore_index, reduction)[0]
     return loss.reshape(shape) if reduction == "none" and len(shape) != 1 else loss
 
 

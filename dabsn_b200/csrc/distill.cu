@@ -4,7 +4,7 @@
 //   p = softmax(logits / T) over the vocabulary,
 //   loss_r = T^2 sum_k q_k (log q_k - log p_id_k),
 //   dlogits_j = w_r T (p_j - sum over the entries with id_k = j of q_k)
-// for the weight w_r with which the row's loss enters the result.
+// for the factor w_r with which the row's loss enters the result.
 //
 // An entry whose id is ignore_index is absent, so rows may list fewer than K
 // entries; a row without any (or with -inf teacher logits throughout) has no
@@ -244,12 +244,19 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(long long rows,
   }
 }
 
+// What the divergence and its gradient in the logits are multiplied by.
+struct Scaling {
+  float temperature, weight;
+  __device__ __forceinline__ float loss() const { return temperature * temperature * weight; }
+  __device__ __forceinline__ float gradient() const { return temperature * weight; }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    float temperature, float* __restrict__ loss) {
+    Scaling by, float* __restrict__ loss) {
   __shared__ float part[DT_THREADS / 32][3];
-  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
+  const float inv_t = 1.f / by.temperature, c = kLog2e * inv_t;
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     if (!list.live[r]) {
       if (threadIdx.x == 0) {
@@ -267,7 +274,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
                                                 threadIdx.x, m, inv_t, logf(all.s),
                                                 all.s == 0.f));
       if (threadIdx.x == 0) {
-        loss[r] = temperature * temperature * l;
+        loss[r] = by.loss() * l;
         list.stats[r] = make_float2(m, all.s);
       }
     }
@@ -275,18 +282,18 @@ __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
   }
 }
 
-// `unless_one`: dlogits holds the gradient for weight 1 already, and a weight of
-// 1 (the usual one: nothing behind a mean but backward()) leaves it as it is.
-// Any other weight starts from the logits again, so that every element is
-// rounded once.
+// `unless_one`: dlogits holds the gradient for an upstream gradient of 1 already,
+// and that (the usual one: nothing behind a mean but backward()) leaves it as it
+// is.  Any other starts from the logits again, so that every element is rounded
+// once.
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, const float* __restrict__ weight, long long wstride,
-    bool unless_one, T* __restrict__ dlogits, long long ldd) {
-  if (unless_one && *weight == 1.f) return;
-  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
-  const float scale = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
+    int mean_blocks, Scaling by, const float* __restrict__ upstream,
+    long long ustride, bool unless_one, T* __restrict__ dlogits, long long ldd) {
+  if (unless_one && *upstream == 1.f) return;
+  const float inv_t = 1.f / by.temperature, c = kLog2e * inv_t;
+  const float scale = by.gradient() * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
   for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = logits + (size_t)r * ld;
     T* drow = dlogits + (size_t)r * ldd;
@@ -295,7 +302,7 @@ __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
       zero_row<T, DT_THREADS>(drow, V, threadIdx.x);
       continue;
     }
-    const float w = scale * weight[r * wstride];
+    const float w = scale * upstream[r * ustride];
     const float A = w / ms.y;
     grad_sweep<T, DT_THREADS, false>(row, drow, V, threadIdx.x, ms.x, c, A, 0.f);
     __syncthreads();  // listed elements are rounded once, with their own term
@@ -319,10 +326,10 @@ constexpr int warp_row() {
 
 template <typename T, bool GRAD>
 __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* row, int K,
-                                                 const Entries& list, float temperature, float w,
+                                                 const Entries& list, Scaling by, float w,
                                                  float* loss, T* drow) {
   const int lane = threadIdx.x & 31;
-  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
+  const float inv_t = 1.f / by.temperature, c = kLog2e * inv_t;
   if (!list.live[r]) {
     if (GRAD) zero_row<T, 32>(drow, V, lane);
     if (lane == 0) {
@@ -352,7 +359,7 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
   const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K, lane, m,
                                             inv_t, logf(st.s), empty));
   if (lane == 0) {
-    loss[r] = temperature * temperature * l;
+    loss[r] = by.loss() * l;
     list.stats[r] = make_float2(m, st.s);
   }
   if (!GRAD) return;
@@ -377,13 +384,13 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(DT_THREADS) distill_warp_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, T* __restrict__ dlogits,
+    int mean_blocks, Scaling by, float* __restrict__ loss, T* __restrict__ dlogits,
     long long ldd) {
   const long long r = (long long)blockIdx.x * (DT_THREADS / 32) + (threadIdx.x >> 5);
   const float w =
-      GRAD ? temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f) : 0.f;
+      GRAD ? by.gradient() * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f) : 0.f;
   if (r < rows)
-    distill_warp_row<T, GRAD>(r, V, logits + (size_t)r * ld, K, list, temperature, w, loss,
+    distill_warp_row<T, GRAD>(r, V, logits + (size_t)r * ld, K, list, by, w, loss,
                               GRAD ? dlogits + (size_t)r * ldd : nullptr);
 }
 
@@ -431,15 +438,15 @@ __device__ __forceinline__ void cp_async_wait_for(int pending) {
 template <typename T>
 __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, T* __restrict__ dlogits,
+    int mean_blocks, Scaling by, float* __restrict__ loss, T* __restrict__ dlogits,
     long long ldd) {
   extern __shared__ uint4 slots[];  // [vectors of a thread][DF_THREADS]
   __shared__ float part[DF_THREADS / 32][3];
   __shared__ float loss_part[DF_THREADS / 32];
   const int t = threadIdx.x;
   const long long stride = gridDim.x;
-  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
-  const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
+  const float inv_t = 1.f / by.temperature, c = kLog2e * inv_t;
+  const float w = by.gradient() * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
   // Vectors of a row at most (rows of other alignments have one less).  Copies
   // are committed in groups of four vectors a thread, as many for every row, so
   // that the statistics start on the first while the last are under way.
@@ -562,7 +569,7 @@ __global__ void __launch_bounds__(DF_THREADS, 3) distill_grad_kernel(
     if (t == 0) {
       l = 0.f;
       for (int i = 0; i < DF_THREADS / 32; ++i) l += loss_part[i];
-      loss[r] = temperature * temperature * l;
+      loss[r] = by.loss() * l;
       list.stats[r] = make_float2(m, st.s);
     }
     r = rn;
@@ -574,11 +581,11 @@ constexpr int DF_LONG_THREADS = 1024;
 template <typename T>
 __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
-    int mean_blocks, float temperature, float* __restrict__ loss, T* __restrict__ dlogits,
+    int mean_blocks, Scaling by, float* __restrict__ loss, T* __restrict__ dlogits,
     long long ldd) {
   __shared__ float part[DF_LONG_THREADS / 32][3];
   const int t = threadIdx.x;
-  const float inv_t = 1.f / temperature, c = kLog2e * inv_t;
+  const float inv_t = 1.f / by.temperature, c = kLog2e * inv_t;
   const long long r = blockIdx.x;
   const T* row = logits + (size_t)r * ld;
   T* drow = dlogits + (size_t)r * ldd;
@@ -594,14 +601,14 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
       sweep<T, DF_LONG_THREADS, false, false>(row, V, t, c), part, c);
   const float m = finite_max(all.mx);
   const bool empty = all.s == 0.f;
-  const float w = temperature * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
+  const float w = by.gradient() * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
   const float A = empty ? 0.f : w / all.s;
   grad_sweep<T, DF_LONG_THREADS, false>(row, drow, V, t, m, c, A, 0.f);
   if (t < 32) {
     const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K, t, m,
                                               inv_t, logf(all.s), empty));
     if (t == 0) {
-      loss[r] = temperature * temperature * l;
+      loss[r] = by.loss() * l;
       list.stats[r] = make_float2(m, all.s);
     }
   }
@@ -647,26 +654,26 @@ namespace {
 
 template <typename T>
 int fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
-        float temperature, float* row_loss, cudaStream_t st) {
+        Scaling by, float* row_loss, cudaStream_t st) {
   if (V <= warp_row<T>()) {
     const int64_t grid = (rows + DT_THREADS / 32 - 1) / (DT_THREADS / 32);
     distill_warp_kernel<T, false><<<(unsigned)grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, (int)K, e, 0, temperature, row_loss, nullptr, 0);
+        rows, (int)V, ld, (const T*)logits, (int)K, e, 0, by, row_loss, nullptr, 0);
   } else {
     distill_fwd_kernel<T><<<row_grid(rows), DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, (int)K, e, temperature, row_loss);
+        rows, (int)V, ld, (const T*)logits, (int)K, e, by, row_loss);
   }
   return launch_status("distill_fwd");
 }
 
 template <typename T>
 int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, const Entries& e,
-         float temperature, int mean_blocks, float* row_loss, void* dlogits, int64_t ldd,
+         Scaling by, int mean_blocks, float* row_loss, void* dlogits, int64_t ldd,
          cudaStream_t st) {
   if (V <= warp_row<T>()) {
     const int64_t grid = (rows + DT_THREADS / 32 - 1) / (DT_THREADS / 32);
     distill_warp_kernel<T, true><<<(unsigned)grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
+        rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, by, row_loss,
         (T*)dlogits, ldd);
     return launch_status("distill_grad");
   }
@@ -674,7 +681,7 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
   const int64_t smem = (V * (int64_t)sizeof(T) + unit - 1) / unit * unit;
   if (smem > DF_ROW_BYTES || rows <= 2 * 148) {
     distill_long_kernel<T><<<row_grid(rows), DF_LONG_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
+        rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, by, row_loss,
         (T*)dlogits, ldd);
     return launch_status("distill_grad");
   }
@@ -682,7 +689,7 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
     return DABSN_ERR_LAUNCH;
   const int64_t grid = std::min<int64_t>(rows, 3 * 148);
   distill_grad_kernel<T><<<(unsigned)grid, DF_THREADS, smem, st>>>(
-      rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, temperature, row_loss,
+      rows, (int)V, ld, (const T*)logits, (int)K, e, mean_blocks, by, row_loss,
       (T*)dlogits, ldd);
   return launch_status("distill_grad");
 }
@@ -697,7 +704,7 @@ extern "C" size_t dabsn_distill_workspace(int64_t rows, int64_t K) {
 extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
                                  const void* logits, int teacher_dtype, int64_t K,
                                  const int64_t* teacher_tokens, const void* teacher_logits,
-                                 int64_t ignore_index, float temperature, int mean,
+                                 int64_t ignore_index, float temperature, float weight, int mean,
                                  void* workspace, float* row_loss, float* result, void* dlogits,
                                  int64_t ldd, void* stream) {
   int bad = check_distill("distill_fwd", dtype, rows, V, ld, K, temperature);
@@ -729,13 +736,13 @@ extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
   if (status) return status;
   const int mb = mean ? prep_blocks(rows) : 0;
   const bool bf = dtype == DABSN_BF16;
+  const Scaling by = {temperature, weight};
   if (dlogits)
-    status = bf ? grad<bf16>(rows, V, ld, logits, K, e, temperature, mb, row_loss, dlogits, ldd, st)
-                : grad<float>(rows, V, ld, logits, K, e, temperature, mb, row_loss, dlogits, ldd,
-                              st);
+    status = bf ? grad<bf16>(rows, V, ld, logits, K, e, by, mb, row_loss, dlogits, ldd, st)
+                : grad<float>(rows, V, ld, logits, K, e, by, mb, row_loss, dlogits, ldd, st);
   else
-    status = bf ? fwd<bf16>(rows, V, ld, logits, K, e, temperature, row_loss, st)
-                : fwd<float>(rows, V, ld, logits, K, e, temperature, row_loss, st);
+    status = bf ? fwd<bf16>(rows, V, ld, logits, K, e, by, row_loss, st)
+                : fwd<float>(rows, V, ld, logits, K, e, by, row_loss, st);
   if (status || !result) return status;
   distill_reduce_kernel<<<1, 1024, 0, st>>>(rows, row_loss, e.counts, mb, result);
   return launch_status("distill_reduce");
@@ -743,13 +750,14 @@ extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
 
 extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
                                  const void* logits, int64_t K, const void* workspace,
-                                 float temperature, int mean, const float* weight, int64_t weight_stride, int unless_one,
+                                 float temperature, float weight, int mean,
+                                 const float* upstream, int64_t upstream_stride, int unless_one,
                                  void* dlogits, int64_t ldd, void* stream) {
   int bad = check_distill("distill_bwd", dtype, rows, V, ld, K, temperature);
   if (!bad) bad = check_gradient_rows("distill_bwd", dtype, rows, V, ld, logits, ldd, dlogits);
   if (bad) return bad;
-  if (unless_one && weight_stride != 0) {
-    set_error("distill_bwd: unless_one takes one weight for all rows");
+  if (unless_one && upstream_stride != 0) {
+    set_error("distill_bwd: unless_one takes one upstream gradient for all rows");
     return DABSN_ERR_UNSUPPORTED;
   }
   if (rows == 0) return DABSN_OK;
@@ -759,11 +767,14 @@ extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
   // a launch that mostly finds nothing to do stays one wave of CTAs
   const unsigned grid =
       unless_one ? (unsigned)std::min<int64_t>(rows, 148 * 8) : row_grid(rows);
+  const Scaling by = {temperature, weight};
   if (dtype == DABSN_BF16)
     distill_bwd_kernel<bf16><<<grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const bf16*)logits, (int)K, e, mb, temperature, weight, weight_stride, unless_one != 0, (bf16*)dlogits, ldd);
+        rows, (int)V, ld, (const bf16*)logits, (int)K, e, mb, by, upstream, upstream_stride,
+        unless_one != 0, (bf16*)dlogits, ldd);
   else
     distill_bwd_kernel<float><<<grid, DT_THREADS, 0, st>>>(
-        rows, (int)V, ld, (const float*)logits, (int)K, e, mb, temperature, weight, weight_stride, unless_one != 0, (float*)dlogits, ldd);
+        rows, (int)V, ld, (const float*)logits, (int)K, e, mb, by, upstream, upstream_stride,
+        unless_one != 0, (float*)dlogits, ldd);
   return launch_status("distill_bwd");
 }

@@ -961,7 +961,7 @@ def token_scores_backward(logits: Tensor, tokens: Tensor, temperature: float, ig
 
 
 def distill_forward(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tensor,
-                    temperature: float, ignore_index: int, reduction: str,
+                    temperature: float, weight: float, ignore_index: int, reduction: str,
                     gradient: bool = False):
     """Student's logits [rows, V] against a teacher's lists [rows, K].  Returns
     (loss, workspace for :func:`distill_backward`, dlogits or None): FP32 row
@@ -990,24 +990,25 @@ def distill_forward(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tens
             dl, ldd = _gradient_rows(logits, ld)
     _run("distill_grad" if gradient else "distill_fwd", dev, lib.dabsn_distill_fwd, code, rows, V,
          ld, logits.data_ptr(), teacher, K, ids.data_ptr(), tl.data_ptr(), ignore_index,
-         temperature, reduction == "mean", ws.data_ptr(), row_loss.data_ptr(), _addr(result),
+         temperature, weight, reduction == "mean", ws.data_ptr(), row_loss.data_ptr(), _addr(result),
          _addr(dl), ldd, launches=2 if result is None else 3)
     return (row_loss if result is None else result), ws, dl
 
 
 def distill_backward(logits: Tensor, workspace: Tensor, entries: int, temperature: float,
-                     mean: bool, weight: Tensor, ready: Tensor | None = None) -> Tensor:
-    """dlogits [rows, V] for row weights ``weight`` ([rows], or [] for all
-    rows), divided by the number of rows with a loss if ``mean``.  ``ready``
-    holds the gradient for weight 1; it is returned, and written again where
-    the (one) weight is another."""
-    dev = _same_cuda(logits, workspace, weight)
+                     weight: float, mean: bool, upstream: Tensor,
+                     ready: Tensor | None = None) -> Tensor:
+    """dlogits [rows, V] for the gradients ``upstream`` of the row losses
+    ([rows], or [] for all rows), divided by the number of rows with a loss if
+    ``mean``.  ``ready`` holds the gradient for an upstream one of 1; it is
+    returned, and written again where that is another."""
+    dev = _same_cuda(logits, workspace, upstream)
     rows, V, ld = _logit_rows(logits)
-    w = _dense_f32(weight)
+    up = _dense_f32(upstream)
     dl, ldd = _gradient_rows(logits, ld) if ready is None else (ready, _logit_rows(ready)[2])
     _run("distill_bwd", dev, N.load().dabsn_distill_bwd, act_code(logits.dtype), rows, V, ld,
-         logits.data_ptr(), entries, workspace.data_ptr(), temperature, mean, w.data_ptr(),
-         w.dim() > 0, ready is not None, dl.data_ptr(), ldd)
+         logits.data_ptr(), entries, workspace.data_ptr(), temperature, weight, mean,
+         up.data_ptr(), up.dim() > 0, ready is not None, dl.data_ptr(), ldd)
     return dl
 
 

@@ -507,7 +507,7 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
                            const float* stats, const float* entropy, const float* g_log_prob,
                            const float* g_entropy, void* dlogits, int64_t ldd, void* stream);
 
-/* Distillation from a teacher's top logits: temperature^2 KL(q || softmax(
+/* Distillation from a teacher's top logits: weight temperature^2 KL(q || softmax(
  * logits / temperature)), q the softmax of the teacher's logits over the
  * entries that a row lists (1 <= K <= 256; entries of ignore_index are absent).
  *   teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K]; an id outside
@@ -517,20 +517,20 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  *   (may be null): the gradient of result, with one read of the logits from
  *   memory: [rows, V] in the logits' dtype, rows `ldd` elements apart and at the
  *   16-byte phase of the logits rows.
- *   bwd, with the fwd's workspace: dlogits for row weights weight[r *
- *   weight_stride], divided by the same number if `mean`; `unless_one` (one
- *   weight for all rows): dlogits holds the gradient for weight 1 already.
+ *   bwd, with the fwd's workspace: dlogits for upstream gradients upstream[r *
+ *   upstream_stride] of the row losses, divided by the same number if `mean`;
+ *   `unless_one` (one for all rows): dlogits holds the gradient for 1 already.
  *   `workspace` holds dabsn_distill_workspace(rows, K) bytes, 8-byte aligned. */
 size_t dabsn_distill_workspace(int64_t rows, int64_t K);
 int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int teacher_dtype, int64_t K, const int64_t* teacher_tokens,
                       const void* teacher_logits, int64_t ignore_index, float temperature,
-                      int mean, void* workspace, float* row_loss, float* result, void* dlogits,
+                      float weight, int mean, void* workspace, float* row_loss, float* result, void* dlogits,
                       int64_t ldd, void* stream);
 int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
-                      int64_t K, const void* workspace, float temperature, int mean,
-                      const float* weight, int64_t weight_stride, int unless_one, void* dlogits,
-                      int64_t ldd, void* stream);
+                      int64_t K, const void* workspace, float temperature, float weight,
+                      int mean, const float* upstream, int64_t upstream_stride, int unless_one,
+                      void* dlogits, int64_t ldd, void* stream);
 
 /* Scaled embedding lookup: out [N, D] = scale * weight[tokens], weight [V, D]
  * with rows `ldw` elements apart; tables and outputs FP32 or BF16.  A token

@@ -323,9 +323,19 @@ def test_distillation(lib, rows, V, K, kind, pad, offset, dtype):
         _near(half, grad * share * -0.3, gtol * share * 0.3 * 1.01 + 1e-37)
         (again,) = torch.autograd.grad(got, leaf)
         assert torch.equal(again, dx)
+    # a factor known beforehand: a power of two changes no digit
+    leaf = x.detach().requires_grad_()
+    got4 = lib.distillation_loss(leaf, ids, tl, temperature=T, weight=0.25, reduction="sum")
+    assert torch.equal(got4, got.detach() * 0.25)
+    for up in (1.0, 0.5):
+        (dx4,) = torch.autograd.grad(got4, leaf, torch.tensor(up, device="cuda"),
+                                     retain_graph=True)
+        _near(dx4, grad * 0.25 * up, gtol * 0.25 * up + 1e-37)
     leaf = x.detach().requires_grad_()
     w = torch.randn(rows, generator=torch.Generator().manual_seed(5))
     got = lib.distillation_loss(leaf, ids, tl, temperature=T, reduction="none")
+    assert torch.equal(lib.distillation_loss(x, ids, tl, temperature=T, weight=2.0,
+                                             reduction="none"), got.detach() * 2.0)
     (dx,) = torch.autograd.grad(got, leaf, w.cuda())
     _near(dx, grad * w.double()[:, None], gtol * w.double().abs()[:, None] * 1.01 + 1e-37)
 
@@ -509,8 +519,8 @@ def test_gradients_against_differences(lib):
             if (t[r] > -math.inf).any():
                 q = torch.softmax(t[r], -1)
                 keep = q > 0
-                total = total + 2.25 * (q[keep] * (torch.log(q[keep])
-                                                   - logp[r, ids.cpu()[r].clamp(min=0)[keep]])).sum()
+                lp = logp[r, ids.cpu()[r].clamp(min=0)[keep]]
+                total = total + 2.25 * (q[keep] * (torch.log(q[keep]) - lp)).sum()
         return total
 
     (a,) = torch.autograd.grad(out.log_prob.sum() + 0.3 * out.entropy.sum(), leaf)

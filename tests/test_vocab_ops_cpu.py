@@ -80,7 +80,7 @@ def test_entry_points_check_sizes_before_launching():
 
     def distill(dtype=0, teacher=0, rows=4, V=10, ld=10, K=2, t=1.0, x=16, dx=None, ldd=10,
                 result=None):
-        return lib.dabsn_distill_fwd(dtype, rows, V, ld, x, teacher, K, NULL, NULL, -100, f(t), 1,
+        return lib.dabsn_distill_fwd(dtype, rows, V, ld, x, teacher, K, NULL, NULL, -100, f(t), f(1.0), 1,
                                      NULL, NULL, result, dx, ldd, NULL)
 
     assert distill(rows=0) == 0
@@ -91,7 +91,7 @@ def test_entry_points_check_sizes_before_launching():
     assert distill(dx=32, result=16, ldd=9) and distill(dx=32, result=16, ldd=11)
 
     def reverse(ld=10, ldd=10, x=0, dx=0, unless_one=0, stride=0):
-        return lib.dabsn_distill_bwd(0, 4, 10, ld, x, 2, NULL, f(1.0), 1, NULL, stride,
+        return lib.dabsn_distill_bwd(0, 4, 10, ld, x, 2, NULL, f(1.0), f(1.0), 1, NULL, stride,
                                      unless_one, dx, ldd, NULL)
 
     assert reverse(ld=9) and reverse(ldd=9) and reverse(ldd=11) and reverse(x=16, dx=4)
