@@ -37,13 +37,17 @@ using namespace rowsm;
 typedef unsigned long long u64;
 
 constexpr int TS_THREADS = 256;
-// Where a call has no more rows than SMs, rows of more than 16 KB go to 512
-// threads each: one BF16 row of 128000 with 20 alternatives in 17 us (23 us with
-// 256), one FP32 row of 32000 in 6.3 us (8.5 us); at 592 rows 256 threads are
-// ahead (12.0 us against 14.1 us for BF16 rows of 32000).
+// Up to three rows an SM, long rows go to 512 threads each: those of more than
+// 24 KB, or with alternatives, whose selection takes longer among more threads, of
+// more than 96 KB.  148 rows, 256 threads and 512: BF16 of 32000 in 7.5 and 6.2
+// us, with 20 alternatives in 11.3 and 11.7; FP32 of 32000 in 10.3 and 8.2, 14.9
+// and 13.1; FP32 of 128000 in 28.8 and 19.9, 44.9 and 31.5.  At 444 rows the two
+// are level for BF16 rows of 32000 (10.0 and 10.2 us), and FP32 rows of 128000
+// with alternatives take 69.5 and 58.8 us.
 constexpr int TS_FEW_THREADS = 512;
-constexpr int TS_FEW_ROWS = 148;
-constexpr int TS_FEW_BYTES = 16384;
+constexpr int TS_FEW_ROWS = 444;
+constexpr int TS_FEW_BYTES = 24 * 1024;
+constexpr int TS_FEW_TOP_BYTES = 96 * 1024;
 constexpr int TS_MAX_K = 128;
 constexpr int TS_CAP = 1024;  // candidates of a row
 constexpr int STATUS_BAD_TOKEN = 8;
@@ -202,23 +206,33 @@ __device__ __forceinline__ void visit_row(const T* p, int n, float low, Visit vi
   if (t < r.tail && to_f<T>(p[r.tail0 + t]) >= low) visit(to_f<T>(p[r.tail0 + t]), r.tail0 + t);
 }
 
-// More logits reach the bound than are kept: a flat row, a masked one with
-// fewer than k logits left, one built against the bound.  With the k-th largest
-// key of the threads (or, where too many lie above that too, of the row): what
-// lies above it, and of the logits equal to it the lowest indices, in order.
+// More logits reach the bound than are kept (a flat row, one built against the
+// bound), or fewer than k threads have any left in a masked row.  With the k-th
+// largest key of the threads (or, where too many lie above that too, of the row;
+// -inf for the masked row): what lies above it, and of the logits equal to it the
+// lowest indices, in order.
 template <typename T, int THREADS>
-__device__ __noinline__ void select_top_slow(TopkShared<THREADS>& sh, const T* p, int n, int k) {
+__device__ __noinline__ void select_top_slow(TopkShared<THREADS>& sh, const T* p, int n, int k,
+                                             bool masked) {
   const int t = threadIdx.x;
-  if (t < 32) find_bound<T, THREADS>(sh, k, true);
-  if (t == 0) sh.n_found = 0;
-  __syncthreads();
-  unsigned bound = sh.bound;
+  unsigned bound = order_key(-INFINITY);
   auto above = [&](float x, int index) {
     const unsigned key = order_key(x);
     if (key > bound && *(volatile int*)&sh.n_found <= TS_CAP) keep(sh, key, index);
   };
-  // strictly above, so the next number is where the visit starts
-  visit_row<T, THREADS>(p, n, bound == 0u ? -INFINITY : key_value(bound + 1u), above);
+  if (t == 0) sh.n_found = sh.n_hot = 0;
+  if (masked) {
+    __syncthreads();
+    if (sh.keys[t] > bound) sh.hot[atomicAdd(&sh.n_hot, 1)] = (short)t;
+    __syncthreads();
+    visit_parts<T, THREADS>(sh, p, n, sh.n_hot, -FLT_MAX, above);
+  } else {
+    if (t < 32) find_bound<T, THREADS>(sh, k, true);
+    __syncthreads();
+    bound = sh.bound;
+    // strictly above, so the next number is where the visit starts
+    visit_row<T, THREADS>(p, n, bound == 0u ? -INFINITY : key_value(bound + 1u), above);
+  }
   __syncthreads();
   if (sh.n_found > TS_CAP) {
     bound = 0;
@@ -281,7 +295,8 @@ __device__ __forceinline__ void select_top(TopkShared<THREADS>& sh, const T* p, 
   const unsigned bound = sh.bound;
   // Below the key of -inf the bound admits masked logits: the other way takes
   // those in order.
-  if (bound > order_key(-INFINITY)) {
+  const bool masked = bound <= order_key(-INFINITY);
+  if (!masked) {
     visit_parts<T, THREADS>(sh, p, n, sh.n_hot, key_value(bound), [&](float x, int index) {
       if (*(volatile int*)&sh.n_found <= TS_CAP) keep(sh, order_key(x), index);
     });
@@ -289,7 +304,7 @@ __device__ __forceinline__ void select_top(TopkShared<THREADS>& sh, const T* p, 
     if (sh.n_found <= TS_CAP) return;
   }
   __syncthreads();
-  select_top_slow<T, THREADS>(sh, p, n, k);
+  select_top_slow<T, THREADS>(sh, p, n, k, masked);
 }
 
 // Calls put(rank, candidate) for the k best candidates.
@@ -510,11 +525,12 @@ int launch_fwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
                cudaStream_t st) {
   const float inv_t = 1.f / temperature;
   int* status = device_status();
-  if (k == 0 && V * sizeof(T) <= TS_WARP_BYTES)
+  if (k == 0 && V * (int64_t)sizeof(T) <= TS_WARP_BYTES)
     token_scores_warp_kernel<T><<<warp_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, log_prob, entropy,
         (float2*)stats, status);
-  else if (rows <= TS_FEW_ROWS && V * sizeof(T) > TS_FEW_BYTES)
+  else if (rows <= TS_FEW_ROWS &&
+           V * (int64_t)sizeof(T) > (k > 0 ? TS_FEW_TOP_BYTES : TS_FEW_BYTES))
     launch_rows<T, TS_FEW_THREADS>(rows, V, ld, logits, tokens, ignore_index, inv_t, k,
                                    log_prob, entropy, stats, top_values, top_ids, status, st);
   else
@@ -529,7 +545,7 @@ int launch_bwd(int64_t rows, int64_t V, int64_t ld, const void* logits, const in
                const float* g_log_prob, const float* g_entropy, void* dlogits, int64_t ldd,
                cudaStream_t st) {
   const float inv_t = 1.f / temperature;
-  if (V * sizeof(T) <= TS_WARP_BYTES)
+  if (V * (int64_t)sizeof(T) <= TS_WARP_BYTES)
     token_scores_bwd_kernel<T, 32, HAS_B><<<warp_grid(rows), TS_THREADS, 0, st>>>(
         rows, (int)V, ld, (const T*)logits, tokens, ignore_index, inv_t, (const float2*)stats,
         entropy, g_log_prob, g_entropy, (T*)dlogits, ldd);
