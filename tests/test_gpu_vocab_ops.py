@@ -166,6 +166,23 @@ def _near(got, want, tol, inf_below=None):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,pad,offset", [(60, 1, 3), (300, 0, 0), (5000, 3, 1), (40001, 0, 0)])
+def test_token_log_probs_few_left(lib, V, pad, offset, dtype):
+    """0, 1, ... logits left by a mask, around the number asked for: those
+    first, then the masked ids in order; the same of one shared value."""
+    k = 20
+    x = _logits(2 * k + 4, V, dtype, V, kind="flat", pad=pad, offset=offset)
+    g = torch.Generator().manual_seed(V)
+    for r in range(2 * k + 4):
+        left = torch.randperm(V, generator=g)[: r // 2].cuda()
+        x[r] = -math.inf if r % 2 else -7.0
+        x[r, left] = torch.randn(len(left), generator=g).to(dtype).cuda()
+    out = lib.token_log_probs(x, _tokens(2 * k + 4, V, 1, ignored=False), top_k=k)
+    order = torch.sort(x.float().cpu(), dim=-1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(out.top_tokens.cpu(), order)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_token_log_probs_top_k_range(lib, dtype):
     for V, k in ((128, 128), (130, 1), (5000, 128), (40000, 128), (60, 60)):
         x = _logits(3, V, dtype, k, kind="ties" if V == 5000 else "normal")
