@@ -787,13 +787,12 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean, sum or none, got {reduction!r}")
     shape = logits.shape[:-1]
-    for name, t in (("teacher_tokens", teacher_tokens), ("teacher_logits", teacher_logits)):
-        if t.dim() != logits.dim() or t.shape[:-1] != shape:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
-                             f"{(*shape, 'entries')}")
-    if teacher_tokens.shape != teacher_logits.shape:
-        raise ValueError("teacher_tokens and teacher_logits differ in shape: "
-                         f"{tuple(teacher_tokens.shape)} and {tuple(teacher_logits.shape)}")
+    if teacher_tokens.dim() == 0 or teacher_tokens.shape[:-1] != shape:
+        raise ValueError(f"teacher_tokens has shape {tuple(teacher_tokens.shape)}, expected "
+                         f"{(*shape, 'entries')}")
+    if teacher_logits.shape != teacher_tokens.shape:
+        raise ValueError(f"teacher_logits has shape {tuple(teacher_logits.shape)}, "
+                         f"teacher_tokens {tuple(teacher_tokens.shape)}: they differ")
     entries = teacher_tokens.shape[-1]
     if entries == 0:
         raise ValueError("a teacher's list holds at least one entry")
@@ -801,9 +800,11 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     if teacher_tokens.dim() != 2:
         teacher_tokens = teacher_tokens.reshape(-1, entries)
         teacher_logits = teacher_logits.reshape(-1, entries)
+    if teacher_logits.requires_grad:
+        teacher_logits = teacher_logits.detach()
     ignore_index = int(ignore_index)
     if _differentiates(rows):
-        loss = _Distillation.apply(rows, teacher_tokens, teacher_logits.detach(), temperature,
+        loss = _Distillation.apply(rows, teacher_tokens, teacher_logits, temperature,
                                    float(weight), ignore_index, reduction)
     else:
         loss = ops.distill_forward(rows, teacher_tokens, teacher_logits, temperature,

@@ -39,6 +39,7 @@ struct Entries {
   float2* q;
   float2* stats;  // [rows] maximum and sum of exponentials of the student's row
   int* live;      // [rows] 1 where the row has a loss
+  float* loss;    // [rows] losses, where the caller has no place for them
   int* counts;    // [blocks] live rows of each preparation block
 };
 
@@ -54,7 +55,8 @@ Entries entries_of(void* ws, int64_t rows, int64_t K) {
   e.stats = e.q + rows * K;
   e.id = (int*)(e.stats + rows);
   e.live = e.id + rows * K;
-  e.counts = e.live + rows;
+  e.loss = (float*)(e.live + rows);
+  e.counts = (int*)(e.loss + rows);
   return e;
 }
 
@@ -701,7 +703,7 @@ int grad(int64_t rows, int64_t V, int64_t ld, const void* logits, int64_t K, con
 
 extern "C" size_t dabsn_distill_workspace(int64_t rows, int64_t K) {
   if (rows < 0 || K < 1) return 0;
-  return (size_t)rows * K * 12 + (size_t)rows * 12 + (size_t)prep_blocks(rows) * 4;
+  return (size_t)rows * K * 12 + (size_t)rows * 16 + (size_t)prep_blocks(rows) * 4;
 }
 
 extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
@@ -729,6 +731,7 @@ extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
     return result ? launch_status("distill_fwd") : DABSN_OK;
   }
   const Entries e = entries_of(workspace, rows, K);
+  if (!row_loss) row_loss = e.loss;
   if (teacher_dtype == DABSN_BF16)
     launch_prep<bf16>(rows, V, K, teacher_tokens, teacher_logits, 1.f / temperature,
                       ignore_index, e, st);

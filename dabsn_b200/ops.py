@@ -982,15 +982,17 @@ def distill_forward(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tens
         temperature)
     lib = N.load()
     ws = torch.empty(lib.dabsn_distill_workspace(rows, K), device=dev, dtype=torch.uint8)
-    row_loss = torch.empty(rows, device=dev, dtype=torch.float32)
-    result, dl, ldd = None, None, 0
-    if reduction != "none":
+    row_loss = result = dl = None
+    ldd = 0
+    if reduction == "none":
+        row_loss = torch.empty(rows, device=dev, dtype=torch.float32)
+    else:
         result = torch.empty((), device=dev, dtype=torch.float32)
         if gradient:
             dl, ldd = _gradient_rows(logits, ld)
     _run("distill_grad" if gradient else "distill_fwd", dev, lib.dabsn_distill_fwd, code, rows, V,
          ld, logits.data_ptr(), teacher, K, ids.data_ptr(), tl.data_ptr(), ignore_index,
-         temperature, weight, reduction == "mean", ws.data_ptr(), row_loss.data_ptr(), _addr(result),
+         temperature, weight, reduction == "mean", ws.data_ptr(), _addr(row_loss), _addr(result),
          _addr(dl), ldd, launches=2 if result is None else 3)
     return (row_loss if result is None else result), ws, dl
 

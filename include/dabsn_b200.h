@@ -512,9 +512,9 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  * entries that a row lists (1 <= K <= 256; entries of ignore_index are absent).
  *   teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K]; an id outside
  *   [0, V) gives a NaN loss and status 8.
- *   fwd: row_loss FP32 [rows]; result FP32 [1] (may be null): the sum of the row
- *   losses, divided by the number of rows that list anything if `mean`; dlogits
- *   (may be null): the gradient of result, with one read of the logits from
+ *   fwd: row_loss FP32 [rows] (may be null); result FP32 [1] (may be null): the
+ *   sum of the row losses, divided by the number of rows that list anything if
+ *   `mean`; dlogits (may be null): the gradient of result, with one read of the logits from
  *   memory: [rows, V] in the logits' dtype, rows `ldd` elements apart and at the
  *   16-byte phase of the logits rows.
  *   bwd, with the fwd's workspace: dlogits for upstream gradients upstream[r *
