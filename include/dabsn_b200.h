@@ -514,9 +514,9 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  *   [0, V) gives a NaN loss and status 8.
  *   fwd: row_loss FP32 [rows] (may be null); result FP32 [1] (may be null): the
  *   sum of the row losses, divided by the number of rows that list anything if
- *   `mean`; dlogits (may be null): the gradient of result, with one read of the logits from
- *   memory: [rows, V] in the logits' dtype, rows `ldd` elements apart and at the
- *   16-byte phase of the logits rows.
+ *   `mean`; dlogits (may be null): the gradient of result, with one read of the
+ *   logits from memory: [rows, V] in the logits' dtype, rows `ldd` elements apart
+ *   and at the 16-byte phase of the logits rows.
  *   bwd, with the fwd's workspace: dlogits for upstream gradients upstream[r *
  *   upstream_stride] of the row losses, divided by the same number if `mean`;
  *   `unless_one` (one for all rows): dlogits holds the gradient for 1 already.
