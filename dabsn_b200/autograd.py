@@ -770,8 +770,9 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     ``teacher_tokens`` [..., K] ids (int64 or int32, 1 to 256 a row) and
     ``teacher_logits`` [..., K] (FP32 or BF16; logits or log-probabilities:
     only their differences count); ``temperature`` in [1e-6, 1e6].  Entries
-    whose id is ``ignore_index`` are absent; an id listed twice counts with both
-    its entries.  ``reduction`` is
+    whose id is ``ignore_index`` are absent, and so are entries of id -1 with a
+    logit of -inf, which :func:`token_log_probs` gives for a row it ignored; an
+    id listed twice counts with both its entries.  ``reduction`` is
     "mean" (over the rows that list anything; 0 if none does), "sum" or "none".
     The loss is FP32; the gradient goes to ``logits`` alone, in their dtype.
     It is computed with the loss, for an upstream gradient of 1; another one

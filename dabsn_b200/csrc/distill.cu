@@ -7,7 +7,8 @@
 // for the factor w_r with which the row's loss enters the result.
 //
 // An entry whose id is ignore_index is absent, so rows may list fewer than K
-// entries; a row without any (or with -inf teacher logits throughout) has no
+// entries, and so is one of id -1 with a logit of -inf, which is how token_scores
+// leaves the alternatives of a row it ignored; a row without any (or with -inf teacher logits throughout) has no
 // loss, no gradient and no part in the mean.  The lists are small: one warp a
 // row turns them into probabilities once (distill_prep), merges an id that is
 // listed twice, and counts the rows: 32768 lists of 64 in 17 us (8 us of
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
       if (k < K) {
         const long long t = ids[r * K + k];
         const float x = to_f<T>(logits[r * K + k]);
-        if (t != ignore_index) {
+        if (t != ignore_index && !(t == -1 && x == -INFINITY)) {
           if (t >= 0 && t < V) {
             id[i] = (int)t;
             q[i] = x;

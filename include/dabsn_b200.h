@@ -509,7 +509,8 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
 
 /* Distillation from a teacher's top logits: weight temperature^2 KL(q || softmax(
  * logits / temperature)), q the softmax of the teacher's logits over the
- * entries that a row lists (1 <= K <= 256; entries of ignore_index are absent).
+ * entries that a row lists (1 <= K <= 256; entries of ignore_index, and those of
+ * id -1 with a logit of -inf, are absent).
  *   teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K]; an id outside
  *   [0, V) gives a NaN loss and status 8.
  *   fwd: row_loss FP32 [rows] (may be null); result FP32 [1] (may be null): the
