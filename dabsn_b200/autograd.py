@@ -783,7 +783,8 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     A row that lists nothing, or whose teacher logits are all -inf, has loss 0
     and no gradient, and its logits are not read.  A listed token whose logit
     is -inf makes the loss +inf; NaN or +inf among a row's teacher logits makes its
-    loss, and the gradient of the listed tokens, NaN.  An id outside [0, V) makes the loss NaN and
+    loss, and the gradient of the listed tokens, NaN.  An id outside [0, V) makes
+    the row's loss and, unless its upstream gradient is 0, its gradient NaN and
     is raised at the next synchronisation (device status 8)."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean, sum or none, got {reduction!r}")

@@ -31,15 +31,19 @@ constexpr int DT_THREADS = 256;
 constexpr int DT_MAX_K = 256;
 constexpr int DT_PREP_THREADS = 512;
 constexpr int DT_STATUS_BAD_TOKEN = 8;
+constexpr int DT_BAD_LIST = 2;  // of Entries::live
 
 // Entry of a row's list after preparation: id (-1: absent), q, and q summed
 // over the entries with the same id (at the first of them; 0 at the others; NaN
 // among the teacher's logits makes both NaN, and with them loss and gradient).
+// A list that names an id outside the vocabulary has no right gradient: its loss
+// is NaN and so is its whole row of the gradient, unless the factor with which
+// the row enters is 0.
 struct Entries {
   int* id;
   float2* q;
   float2* stats;  // [rows] maximum and sum of exponentials of the student's row
-  int* live;      // [rows] 1 where the row has a loss
+  int* live;      // [rows] 0 no loss, 1 a loss, 2 a NaN loss for an id outside
   float* loss;    // [rows] losses, where the caller has no place for them
   int* counts;    // [blocks] live rows of each preparation block
 };
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(DT_PREP_THREADS) distill_prep_kernel(
         out.q[r * K + k] = make_float2(mine, (later >> i) & 1u ? 0.f : all[i]);
       }
     }
-    if (lane == 0) out.live[r] = live;
+    if (lane == 0) out.live[r] = bad ? DT_BAD_LIST : live;
   }
   if (lane == 0) live_rows[warp] = counted;
   __syncthreads();
@@ -254,6 +258,18 @@ struct Scaling {
   __device__ __forceinline__ float gradient() const { return temperature * weight; }
 };
 
+// A of grad_value for a row with the factor w and the sum of exponentials s: p_j w
+// is 2^d_j A.  A row with every logit masked (s == 0) has no gradient.
+__device__ __forceinline__ float gradient_factor(int live, float w, float s) {
+  if (live == DT_BAD_LIST && w != 0.f) return __int_as_float(0x7fc00000);
+  return s == 0.f ? 0.f : w / s;
+}
+
+// Whether a listed entry changes its element: it has a probability or is NaN.
+__device__ __forceinline__ bool entry_counts(int id, float q, bool empty) {
+  return id >= 0 && !(q <= 0.f) && !empty;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(DT_THREADS) distill_fwd_kernel(
     long long rows, int V, long long ld, const T* __restrict__ logits, int K, Entries list,
@@ -301,18 +317,19 @@ __global__ void __launch_bounds__(DT_THREADS) distill_bwd_kernel(
     const T* row = logits + (size_t)r * ld;
     T* drow = dlogits + (size_t)r * ldd;
     const float2 ms = list.stats[r];
-    if (!list.live[r] || ms.y == 0.f) {
+    const int live = list.live[r];
+    if (!live) {
       zero_row<T, DT_THREADS>(drow, V, threadIdx.x);
       continue;
     }
     const float w = scale * upstream[r * ustride];
-    const float A = w / ms.y;
+    const float A = gradient_factor(live, w, ms.y);
     grad_sweep<T, DT_THREADS, false>(row, drow, V, threadIdx.x, ms.x, c, A, 0.f);
     __syncthreads();  // listed elements are rounded once, with their own term
     for (int k = threadIdx.x; k < K; k += DT_THREADS) {
       const int id = list.id[r * K + k];
       const float q = list.q[r * K + k].y;
-      if (id >= 0 && !(q <= 0.f))
+      if (entry_counts(id, q, ms.y == 0.f))
         drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), ms.x, c, A, 0.f)));
     }
   }
@@ -333,7 +350,8 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
                                                  float* loss, T* drow) {
   const int lane = threadIdx.x & 31;
   const float inv_t = 1.f / by.temperature, c = kLog2e * inv_t;
-  if (!list.live[r]) {
+  const int live = list.live[r];
+  if (!live) {
     if (GRAD) zero_row<T, 32>(drow, V, lane);
     if (lane == 0) {
       loss[r] = 0.f;
@@ -366,7 +384,7 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
     list.stats[r] = make_float2(m, st.s);
   }
   if (!GRAD) return;
-  const float A = empty ? 0.f : w / st.s;
+  const float A = gradient_factor(live, w, st.s);
   const f32x2 m2 = pair(-m, -m), c2 = pair(c, c), A2 = pair(A, A);
   uint4* dv = reinterpret_cast<uint4*>(drow + s.head);
 #pragma unroll
@@ -376,10 +394,10 @@ __device__ __forceinline__ void distill_warp_row(long long r, int V, const T* ro
   if (lane < s.head) drow[lane] = from_f<T>(grad_value<false>(head, m, c, A, 0.f));
   if (lane < s.tail) drow[s.tail0 + lane] = from_f<T>(grad_value<false>(tail, m, c, A, 0.f));
   __syncwarp();  // listed elements are rounded once, with their own term
-  for (int k = lane; k < K && !empty; k += 32) {
+  for (int k = lane; k < K; k += 32) {
     const int id = list.id[r * K + k];
     const float q = list.q[r * K + k].y;
-    if (id >= 0 && !(q <= 0.f))
+    if (entry_counts(id, q, empty))
       drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
   }
 }
@@ -495,6 +513,7 @@ __global__ void __launch_bounds__(DF_THREADS, 2) distill_grad_kernel(
   while (r < rows) {
     const T* row = logits + (size_t)r * ld;
     const RowShape s = row_shape(row, V);
+    const int live = list.live[r];
     int id = -1;
     float2 q = make_float2(0.f, 0.f);
     float x = 0.f;
@@ -532,7 +551,7 @@ __global__ void __launch_bounds__(DF_THREADS, 2) distill_grad_kernel(
     if ((t & 31) == 0) loss_part[t >> 5] = l;
 
     // gradient, and the next row's copies
-    const float A = empty ? 0.f : w / st.s;
+    const float A = gradient_factor(live, w, st.s);
     const long long rn = next_live(r + stride);
     const T* pn = logits + (size_t)(rn < rows ? rn : r) * ld;
     RowShape sn = row_shape(pn, V);
@@ -570,7 +589,7 @@ __global__ void __launch_bounds__(DF_THREADS, 2) distill_grad_kernel(
       load_edges(pn, sn);
     }
     __syncthreads();  // listed elements are rounded once, with their own term
-    if (id >= 0 && !(q.y <= 0.f) && !empty)
+    if (entry_counts(id, q.y, empty))
       drow[id] = from_f<T>(fmaf(-w, q.y, grad_value<false>(x, m, c, A, 0.f)));
     if (t == 0) {
       l = 0.f;
@@ -595,7 +614,8 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
   const long long r = blockIdx.x;
   const T* row = logits + (size_t)r * ld;
   T* drow = dlogits + (size_t)r * ldd;
-  if (!list.live[r]) {
+  const int live = list.live[r];
+  if (!live) {
     zero_row<T, DF_LONG_THREADS>(drow, V, t);
     if (t == 0) {
       loss[r] = 0.f;
@@ -608,7 +628,7 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
   const float m = finite_max(all.mx);
   const bool empty = all.s == 0.f;
   const float w = by.gradient() * (mean_blocks ? mean_scale(list.counts, mean_blocks) : 1.f);
-  const float A = empty ? 0.f : w / all.s;
+  const float A = gradient_factor(live, w, all.s);
   grad_sweep<T, DF_LONG_THREADS, false>(row, drow, V, t, m, c, A, 0.f);
   if (t < 32) {
     const float l = warp_sum(list_loss<T, 32>(row, list.id + r * K, list.q + r * K, K, t, m,
@@ -619,10 +639,10 @@ __global__ void __launch_bounds__(DF_LONG_THREADS, 2) distill_long_kernel(
     }
   }
   __syncthreads();  // listed elements are rounded once, with their own term
-  for (int k = t; k < K && !empty; k += DF_LONG_THREADS) {
+  for (int k = t; k < K; k += DF_LONG_THREADS) {
     const int id = list.id[r * K + k];
     const float q = list.q[r * K + k].y;
-    if (id >= 0 && !(q <= 0.f))
+    if (entry_counts(id, q, empty))
       drow[id] = from_f<T>(fmaf(-w, q, grad_value<false>(to_f<T>(row[id]), m, c, A, 0.f)));
   }
 }

@@ -512,7 +512,8 @@ int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const
  * entries that a row lists (1 <= K <= 256; entries of ignore_index, and those of
  * id -1 with a logit of -inf, are absent).
  *   teacher_tokens int64 and teacher_logits FP32/BF16 [rows, K]; an id outside
- *   [0, V) gives a NaN loss and status 8.
+ *   [0, V) gives a NaN loss, a NaN row of the gradient (unless the factor with
+ *   which the row enters is 0) and status 8.
  *   fwd: row_loss FP32 [rows] (may be null); result FP32 [1] (may be null): the
  *   sum of the row losses, divided by the number of rows that list anything if
  *   `mean`; dlogits (may be null): the gradient of result, with one read of the

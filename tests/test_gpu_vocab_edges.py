@@ -63,3 +63,50 @@ def test_an_id_of_minus_one_with_a_logit_is_outside(lib):
     loss = lib.distillation_loss(x, ids, tl, reduction="none")
     assert loss.isnan().tolist() == [False, True, True]
     assert _native.device_status(reset=True) == 8
+
+
+# ---------------------------------------------------------------------------
+# Ids outside the vocabulary
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,V", [(6, 60), (6, 9000), (450, 9000), (6, 40001)])
+def test_gradients_of_lists_with_a_bad_id(lib, rows, V, dtype):
+    """A list that names a token outside [0, V) has a NaN loss and a NaN
+    gradient, also where no id of it is valid and where the student's row is
+    masked throughout; the other rows are as if it were not there."""
+    from dabsn_b200 import _native
+
+    x = _logits(rows, V, dtype, 3)
+    x[3] = -math.inf
+    ids = torch.arange(4, device="cuda").repeat(rows, 1)
+    tl = torch.randn(rows, 4, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    ids[0, 2] = V
+    ids[1] = -5
+    ids[3, 0] = V + 7
+    bad = torch.tensor([0, 1, 3], device="cuda")
+    rest = torch.tensor([r for r in range(rows) if r not in (0, 1, 3)], device="cuda")
+    leaf = x.detach().requires_grad_()
+    up = torch.linspace(0.5, 2.0, rows, device="cuda")
+    none = lib.distillation_loss(leaf, ids, tl, reduction="none")
+    total = lib.distillation_loss(leaf, ids, tl, reduction="sum")
+    assert none[bad].isnan().all() and not none[rest].isnan().any() and total.isnan()
+    grads = [torch.autograd.grad(none, leaf, up)[0],
+             torch.autograd.grad(total, leaf, retain_graph=True)[0],
+             torch.autograd.grad(total, leaf, torch.tensor(0.5, device="cuda"))[0]]
+    good = ids.clone()
+    good[bad] = -100
+    a = lib.distillation_loss(leaf, good, tl, reduction="none")
+    b = lib.distillation_loss(leaf, good, tl, reduction="sum")
+    want = [torch.autograd.grad(a, leaf, up)[0],
+            torch.autograd.grad(b, leaf, retain_graph=True)[0],
+            torch.autograd.grad(b, leaf, torch.tensor(0.5, device="cuda"))[0]]
+    for got, ref in zip(grads, want):
+        assert got[bad].isnan().all()
+        assert torch.equal(got[rest], ref[rest])
+    # an upstream gradient of zero takes the row out
+    up0 = up.clone()
+    up0[bad] = 0.0
+    none = lib.distillation_loss(leaf, ids, tl, reduction="none")
+    (dx,) = torch.autograd.grad(none, leaf, up0)
+    assert float(dx[bad].abs().max()) == 0.0 and torch.equal(dx[rest], want[0][rest])
+    assert _native.device_status(reset=True) == 8
