@@ -266,8 +266,9 @@ __device__ __forceinline__ float gradient_factor(int live, float w, float s) {
 }
 
 // Whether a listed entry changes its element: it has a probability or is NaN.
+// In a row with every logit masked NaN alone reaches the gradient.
 __device__ __forceinline__ bool entry_counts(int id, float q, bool empty) {
-  return id >= 0 && !(q <= 0.f) && !empty;
+  return id >= 0 && !(q <= 0.f) && (!empty || q != q);
 }
 
 template <typename T>

@@ -110,3 +110,24 @@ def test_gradients_of_lists_with_a_bad_id(lib, rows, V, dtype):
     (dx,) = torch.autograd.grad(none, leaf, up0)
     assert float(dx[bad].abs().max()) == 0.0 and torch.equal(dx[rest], want[0][rest])
     assert _native.device_status(reset=True) == 8
+
+
+def test_nan_of_a_teacher_with_a_masked_student(lib):
+    """NaN among the teacher's logits makes the listed tokens' gradient NaN,
+    whatever the student's row holds."""
+    for rows, V in ((4, 60), (4, 9000), (450, 9000)):
+        x = _logits(rows, V, F32, 1)
+        x[1] = -math.inf
+        ids = torch.arange(6, device="cuda").repeat(rows, 1)
+        tl = torch.zeros(rows, 6, device="cuda")
+        tl[1, 2] = math.nan
+        leaf = x.detach().requires_grad_()
+        loss = lib.distillation_loss(leaf, ids, tl, reduction="none")
+        total = lib.distillation_loss(leaf, ids, tl, reduction="sum")
+        assert loss.isnan().tolist() == [r == 1 for r in range(rows)]
+        for grad in (torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0],
+                     torch.autograd.grad(total, leaf, retain_graph=True)[0],
+                     torch.autograd.grad(total, leaf, torch.tensor(2.0, device="cuda"))[0]):
+            assert grad[1, :6].isnan().all() and float(grad[1, 6:].abs().max()) == 0.0
+            rest = [r for r in range(rows) if r != 1]
+            assert not grad[rest].isnan().any()
