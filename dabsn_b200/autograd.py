@@ -707,8 +707,9 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     are all -inf has log-probability -inf, entropy 0, no gradient, and its
     first ids as alternatives.  NaN or +inf among the logits makes the row's
     numbers NaN (its alternatives' ids are then valid but unspecified).  A
-    token outside [0, V) makes its log-probability NaN and is raised at the
-    next synchronisation (device status 8)."""
+    token outside [0, V) makes its log-probability and, unless the upstream
+    gradient is 0, that one's gradient NaN and is raised at the next
+    synchronisation (device status 8)."""
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens has shape {tuple(tokens.shape)}, expected "
                          f"{tuple(logits.shape[:-1])}")

@@ -454,16 +454,20 @@ __global__ void __launch_bounds__(TS_THREADS) token_scores_bwd_kernel(
     T* drow = dlogits + (size_t)r * ldd;
     const long long t = tokens[r];
     const float2 ms = stats[r];
-    if (t == ignore_index || ms.y == 0.f) {
+    const float g = g_log_prob ? g_log_prob[r] * inv_t : 0.f;
+    // the log-probability of a token outside the vocabulary is NaN, and so is
+    // its gradient
+    const bool undefined = t != ignore_index && (t < 0 || t >= V) && g != 0.f;
+    if (t == ignore_index || (ms.y == 0.f && !undefined)) {
       // padding, or a row with every logit masked: nothing to learn
       zero_row<T, THREADS>(drow, V, lane);
       continue;
     }
-    const float g = g_log_prob ? g_log_prob[r] * inv_t : 0.f;
     const float h = HAS_B ? g_entropy[r] * inv_t : 0.f;
     // p_j (log p_j + entropy) = 2^d_j (d_j ln2 - log s + entropy) / s
     const float B = HAS_B ? -h * kLn2 / ms.y : 0.f;
-    const float A = -(HAS_B ? fmaf(h, entropy[r] - logf(ms.y), g) : g) / ms.y;
+    const float A = undefined ? __int_as_float(0x7fc00000)
+                              : -(HAS_B ? fmaf(h, entropy[r] - logf(ms.y), g) : g) / ms.y;
     grad_sweep<T, THREADS, HAS_B>(row, drow, V, lane, ms.x, c, A, B);
     if (t >= 0 && t < V) {
       // the token's element is rounded once, with its own term

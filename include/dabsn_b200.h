@@ -497,7 +497,8 @@ uint64_t dabsn_capture_id(void* stream);
  * Reverse: dlogits [rows, V] in the logits' dtype, rows `ldd` elements apart
  * and at the 16-byte phase of the logits rows, for gradients of log_prob and
  * entropy (FP32 [rows], either may be null).
- * A token outside [0, V) gives NaN and device status 8. */
+ * A token outside [0, V) gives a NaN log_prob, a NaN row of the gradient where
+ * g_log_prob is not 0, and device status 8. */
 int dabsn_token_scores_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                            const int64_t* tokens, int64_t ignore_index, float temperature,
                            int64_t top_k, float* log_prob, float* entropy, float* stats,

@@ -112,6 +112,38 @@ def test_gradients_of_lists_with_a_bad_id(lib, rows, V, dtype):
     assert _native.device_status(reset=True) == 8
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [60, 9000])
+def test_gradients_of_a_bad_token(lib, V, dtype):
+    """Its log-probability is NaN and so is that gradient; its entropy does not
+    depend on the token."""
+    from dabsn_b200 import _native
+
+    x = _logits(5, V, dtype, 4)
+    x[4] = -math.inf
+    tokens = torch.tensor([3, V, -7, 5, V + 1], device="cuda")
+    bad = [1, 2, 4]
+    leaf = x.detach().requires_grad_()
+    out = lib.token_log_probs(leaf, tokens, temperature=0.9)
+    up = torch.linspace(0.5, 1.5, 5, device="cuda")
+    fine = lib.token_log_probs(leaf, tokens.clamp(0, V - 1), temperature=0.9)
+    (g,) = torch.autograd.grad(out.log_prob, leaf, up, retain_graph=True)
+    (want,) = torch.autograd.grad(fine.log_prob, leaf, up, retain_graph=True)
+    assert out.log_prob.isnan().tolist() == [False, True, True, False, True]
+    assert g[bad].isnan().all() and torch.equal(g[[0, 3]], want[[0, 3]])
+    (h,) = torch.autograd.grad(out.entropy, leaf, up, retain_graph=True)
+    (hwant,) = torch.autograd.grad(fine.entropy, leaf, up, retain_graph=True)
+    assert torch.equal(h, hwant)
+    (both,) = torch.autograd.grad([out.log_prob, out.entropy], leaf, [up, up], retain_graph=True)
+    assert both[bad].isnan().all() and not both[[0, 3]].isnan().any()
+    # an upstream gradient of zero takes the log-probability out
+    up0 = up.clone()
+    up0[bad] = 0.0
+    (some,) = torch.autograd.grad([out.log_prob, out.entropy], leaf, [up0, up])
+    assert torch.equal(some[bad], hwant[bad])
+    assert _native.device_status(reset=True) == 8
+
+
 def test_nan_of_a_teacher_with_a_masked_student(lib):
     """NaN among the teacher's logits makes the listed tokens' gradient NaN,
     whatever the student's row holds."""
