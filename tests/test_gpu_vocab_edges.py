@@ -163,3 +163,71 @@ def test_nan_of_a_teacher_with_a_masked_student(lib):
             assert grad[1, :6].isnan().all() and float(grad[1, 6:].abs().max()) == 0.0
             rest = [r for r in range(rows) if r != 1]
             assert not grad[rest].isnan().any()
+
+
+# ---------------------------------------------------------------------------
+# Loops that only large calls go round
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,pad,offset", [(4099, 5, 3), (4104, 0, 0), (2057, 1, 1)])
+def test_distillation_of_many_rows_with_gaps(lib, V, pad, offset, dtype):
+    """A CTA of the one-pass gradient takes every 444th row: rows without a loss
+    between two that have one, several in a row, and at either end."""
+    rows, K, T = 2011, 7, 1.5
+    x = _logits(rows, V, dtype, V, pad=pad, offset=offset)
+    gen = torch.Generator().manual_seed(V)
+    ids = torch.randint(0, V, (rows, K), generator=gen)
+    tl = torch.randn(rows, K, generator=gen) * 2.0
+    ids[::3] = -100
+    for first in (5, 17, 200, 443):
+        ids[first::444] = -100  # nothing at all for this CTA
+    for first in (7, 100):
+        ids[first + 444] = ids[first + 888] = -100  # two in a row, between others
+    ids[0], ids[444], ids[1332] = 1, 2, 3
+    ids, tl = ids.cuda(), tl.cuda()
+    loss, size, grad, gsize, live, C = _distill_reference(x, ids, tl, T)
+    n = int(live.sum())
+    assert 0 < n < rows
+    ltol = U * C * size * 2
+    gtol = _half_step(dtype) * grad.abs() + 2 * U * C[:, None] * gsize + 1e-37
+    plain = lib.distillation_loss(x, ids, tl, temperature=T, reduction="none")
+    _near(plain, loss, ltol)
+    leaf = x.detach().requires_grad_()
+    got = lib.distillation_loss(leaf, ids, tl, temperature=T)
+    _near(got, loss.sum() / n, (ltol.sum() + U * size.sum()) / n + U * loss.sum().abs() / n)
+    (dx,) = torch.autograd.grad(got, leaf, retain_graph=True)
+    _near(dx, grad / n, gtol / n + 1e-37)
+    # the reverse from the logits, over the same rows
+    (half,) = torch.autograd.grad(got, leaf, torch.tensor(0.5, device="cuda"))
+    _near(half, grad / n * 0.5, gtol / n * 0.51 + 1e-37)
+
+
+@pytest.mark.parametrize("N,V", [(600011, 37), (600011, 900), (262145, 70001), (786432, 70001)])
+def test_embedding_gradient_of_many_tokens(lib, N, V):
+    """More tokens than 256 sort blocks rank in one step, one to three digits;
+    sums of small whole numbers are exact."""
+    g = torch.Generator().manual_seed(N + V)
+    tokens = (torch.rand(N, generator=g) ** 3 * V).long().clamp(max=V - 1)
+    go = torch.randint(-4, 5, (N, 8), generator=g).float()
+    w = torch.zeros(V, 8, device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(lib.embedding(tokens.cuda(), w), w, go.cuda())
+    assert torch.equal(dw.cpu(), torch.zeros(V, 8).index_add_(0, tokens, go))
+
+
+@pytest.mark.parametrize("D", [515, 1029, 2056])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_embedding_runs_over_column_tiles(lib, D, dtype):
+    """Tokens whose positions cover whole pieces of the sums, in tables wider
+    than a tile of columns; whole numbers, exact."""
+    runs = [63, 1, 9000, 64, 65, 127, 129, 192, 2, 1, 62, 300, 33, 33, 1000]
+    for many in (1, 4):  # below and above 32768 positions
+        sizes = runs * many
+        V = 2 * len(sizes) + 1
+        g = torch.Generator().manual_seed(D)
+        tokens = torch.cat([torch.full((n,), 2 * i + 1) for i, n in enumerate(sizes)])
+        tokens = tokens[torch.randperm(len(tokens), generator=g)]
+        go = torch.randint(-4, 5, (len(tokens), D), generator=g).float()
+        w = torch.zeros(V, D, device="cuda", requires_grad=True)
+        out = lib.embedding(tokens.cuda(), w, dtype=dtype)
+        (dw,) = torch.autograd.grad(out, w, go.cuda().to(dtype))
+        assert torch.equal(dw.cpu(), torch.zeros(V, D).index_add_(0, tokens, go))
