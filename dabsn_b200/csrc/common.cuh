@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace dabsn {
 
 // ---------------------------------------------------------------------------
@@ -115,6 +117,9 @@ void set_error(const char* fmt, ...);
 bool kernel_prepared(const void* kernel, int smem_bytes);
 int current_device();
 int launch_status(const char* what);
+// DABSN_OK, or an error that says so where one of the pointers is null (a tensor
+// without memory of its own: a wrapper subclass, a functionalized tensor).
+int check_pointers(const char* what, std::initializer_list<const void*> pointers);
 }  // namespace dabsn
 
 // ---------------------------------------------------------------------------

@@ -752,6 +752,8 @@ extern "C" int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld,
     if (result) cudaMemsetAsync(result, 0, sizeof(float), st);
     return result ? launch_status("distill_fwd") : DABSN_OK;
   }
+  bad = check_pointers("distill_fwd", {logits, teacher_tokens, teacher_logits, workspace});
+  if (bad) return bad;
   const Entries e = entries_of(workspace, rows, K);
   if (!row_loss) row_loss = e.loss;
   if (teacher_dtype == DABSN_BF16)
@@ -789,6 +791,8 @@ extern "C" int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld,
     return DABSN_ERR_UNSUPPORTED;
   }
   if (rows == 0) return DABSN_OK;
+  bad = check_pointers("distill_bwd", {logits, workspace, upstream, dlogits});
+  if (bad) return bad;
   const Entries e = entries_of(const_cast<void*>(workspace), rows, K);
   cudaStream_t st = (cudaStream_t)stream;
   const int mb = mean ? prep_blocks(rows) : 0;

@@ -720,7 +720,7 @@ using namespace dabsn;
 extern "C" int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, int64_t V,
                                    int64_t D, const int64_t* tokens, const void* weight,
                                    int64_t ldw, float scale, void* out, void* stream) {
-  const int bad = check_embedding("embedding_fwd", weight_dtype, out_dtype, N, V, D);
+  int bad = check_embedding("embedding_fwd", weight_dtype, out_dtype, N, V, D);
   if (bad) return bad;
   if (ldw < D) {
     set_error("embedding_fwd: row stride %lld below the width %lld", (long long)ldw,
@@ -728,6 +728,8 @@ extern "C" int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, i
     return DABSN_ERR_SHAPE;
   }
   if (N == 0) return DABSN_OK;
+  bad = check_pointers("embedding_fwd", {tokens, weight, out});
+  if (bad) return bad;
   cudaStream_t st = (cudaStream_t)stream;
   if (weight_dtype == DABSN_BF16)
     return out_dtype == DABSN_BF16
@@ -747,12 +749,15 @@ extern "C" int dabsn_embedding_bwd(int out_dtype, int weight_dtype, int64_t N, i
                                    int64_t D, const int64_t* tokens, int64_t padding_idx,
                                    const void* dout, float scale, void* dweight, void* workspace,
                                    size_t workspace_bytes, void* stream) {
-  const int bad = check_embedding("embedding_bwd", weight_dtype, out_dtype, N, V, D);
+  int bad = check_embedding("embedding_bwd", weight_dtype, out_dtype, N, V, D);
   if (bad) return bad;
   if (workspace_bytes < dabsn_embedding_bwd_workspace(N, V, D)) {
     set_error("embedding_bwd: workspace of %zu bytes is too small", workspace_bytes);
     return DABSN_ERR_UNSUPPORTED;
   }
+  bad = check_pointers("embedding_bwd", {dweight, workspace});
+  if (!bad && N > 0) bad = check_pointers("embedding_bwd", {tokens, dout});
+  if (bad) return bad;
   cudaStream_t st = (cudaStream_t)stream;
   const SortPlan plan = sort_plan(N, V);
   const SortSpace s = sort_space(workspace, N);

@@ -78,6 +78,15 @@ int launch_status(const char* what) {
   return DABSN_OK;
 }
 
+int check_pointers(const char* what, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (p == nullptr) {
+      set_error("%s: null pointer (a tensor without memory of its own)", what);
+      return DABSN_ERR_UNSUPPORTED;
+    }
+  return DABSN_OK;
+}
+
 }  // namespace dabsn
 
 __device__ int g_dabsn_status[1];

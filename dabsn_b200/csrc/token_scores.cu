@@ -578,6 +578,9 @@ extern "C" int dabsn_token_scores_fwd(int dtype, int64_t rows, int64_t V, int64_
     return DABSN_ERR_UNSUPPORTED;
   }
   if (rows == 0) return DABSN_OK;
+  int null = check_pointers("token_scores_fwd", {logits, tokens, log_prob, entropy});
+  if (!null && top_k > 0) null = check_pointers("token_scores_fwd", {top_values, top_ids});
+  if (null) return null;
   cudaStream_t st = (cudaStream_t)stream;
   return dtype == DABSN_BF16
              ? launch_fwd<bf16>(rows, V, ld, logits, tokens, ignore_index, temperature, top_k,
@@ -597,6 +600,8 @@ extern "C" int dabsn_token_scores_bwd(int dtype, int64_t rows, int64_t V, int64_
     bad = check_gradient_rows("token_scores_bwd", dtype, rows, V, ld, logits, ldd, dlogits);
   if (bad) return bad;
   if (rows == 0) return DABSN_OK;
+  bad = check_pointers("token_scores_bwd", {logits, tokens, stats, entropy, dlogits});
+  if (bad) return bad;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == DABSN_BF16)
     return g_entropy ? launch_bwd<bf16, true>(rows, V, ld, logits, tokens, ignore_index,

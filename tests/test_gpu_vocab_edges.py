@@ -231,3 +231,17 @@ def test_embedding_runs_over_column_tiles(lib, D, dtype):
         out = lib.embedding(tokens.cuda(), w, dtype=dtype)
         (dw,) = torch.autograd.grad(out, w, go.cuda().to(dtype))
         assert torch.equal(dw.cpu(), torch.zeros(V, D).index_add_(0, tokens, go))
+
+
+# ---------------------------------------------------------------------------
+# Tensors that are not what a kernel can read
+# ---------------------------------------------------------------------------
+def test_tensors_without_memory_are_refused(lib):
+    """Under functionalize a tensor's data pointer is null."""
+    x = _logits(4, 50, F32, 1)
+    t = torch.arange(4, device="cuda")
+    for call in (lambda z: lib.token_log_probs(z, t).log_prob,
+                 lambda z: lib.distillation_loss(z, t[:, None], torch.zeros(4, 1, device="cuda")),
+                 lambda z: lib.embedding(t, z)):
+        with pytest.raises(RuntimeError, match="null pointer"):
+            torch.func.functionalize(call)(x)
