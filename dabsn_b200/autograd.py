@@ -19,6 +19,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native, ops
@@ -631,6 +632,16 @@ class TokenLogProbs(NamedTuple):
     top_tokens: Tensor | None
 
 
+def _refuse_transforms(*tensors: Tensor | None) -> None:
+    """Refuses forward-mode derivatives: the kernels write plain memory, so a
+    tangent would vanish and read as zero."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(
+                    "dabsn_b200: forward-mode derivatives are not implemented")
+
+
 def _once_differentiable(backward):
     """``torch.autograd.function.once_differentiable`` where a graph of the
     reverse is being recorded; without one there is nothing to guard, and the
@@ -638,6 +649,7 @@ def _once_differentiable(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        _refuse_transforms(*grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -713,6 +725,7 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens has shape {tuple(tokens.shape)}, expected "
                          f"{tuple(logits.shape[:-1])}")
+    _refuse_transforms(logits)
     shape, top_k = tokens.shape, int(top_k)
     rows = _as_rows(logits)
     flat = tokens if tokens.dim() == 1 else tokens.reshape(-1)
@@ -799,6 +812,7 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     entries = teacher_tokens.shape[-1]
     if entries == 0:
         raise ValueError("a teacher's list holds at least one entry")
+    _refuse_transforms(logits, teacher_logits)
     rows = _as_rows(logits)
     if teacher_tokens.dim() != 2:
         teacher_tokens = teacher_tokens.reshape(-1, entries)
@@ -852,6 +866,7 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0,
             raise ValueError(f"padding_idx {padding_idx} lies outside the table of "
                              f"{weight.shape[0]} rows")
         padding_idx = int(padding_idx) % weight.shape[0]
+    _refuse_transforms(weight)
     args = (weight, tokens, float(scale), padding_idx, dtype or weight.dtype)
     return (_Embedding.apply(*args) if _differentiates(weight) else
             ops.embedding_forward(tokens, weight, args[2], args[4]))

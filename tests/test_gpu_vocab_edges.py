@@ -245,3 +245,26 @@ def test_tensors_without_memory_are_refused(lib):
                  lambda z: lib.embedding(t, z)):
         with pytest.raises(RuntimeError, match="null pointer"):
             torch.func.functionalize(call)(x)
+
+
+# ---------------------------------------------------------------------------
+# Tracing and forward mode, with the kernels themselves
+# ---------------------------------------------------------------------------
+def _calls(lib):
+    t = torch.tensor([4, 0, 49, 7], device="cuda")
+    ids = torch.tensor([[1, 2], [3, 4], [5, 6], [0, 49]], device="cuda")
+    tl = torch.linspace(-1, 1, 8, device="cuda").view(4, 2)
+    return (lambda z: lib.token_log_probs(z, t, top_k=2).log_prob + 0,
+            lambda z: lib.distillation_loss(z, ids, tl) + 0,
+            lambda z: lib.embedding(t % 4, z) + 0)
+
+
+def test_forward_mode_is_refused(lib):
+    x = _logits(4, 50, F32, 1)
+    for call in _calls(lib):
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))

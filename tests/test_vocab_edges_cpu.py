@@ -5,7 +5,12 @@ from __future__ import annotations
 
 import ctypes
 
-from dabsn_b200 import _native
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import dabsn_b200
+from dabsn_b200 import _native, ops
 
 NULL = ctypes.c_void_p(0)
 
@@ -53,3 +58,99 @@ def test_null_pointers_are_refused():
         assert call(x=16, dx=None) == 4 and b"null pointer" in lib.dabsn_last_error()
     assert scores(k=2, values=None, ids=1) == 4 and scores(k=2, values=1, ids=None) == 4
     assert b"null pointer" in lib.dabsn_last_error()
+
+
+# ---------------------------------------------------------------------------
+# Forward-mode derivatives and tracing
+# ---------------------------------------------------------------------------
+def _written(values):
+    """A result as the kernels give one: allocated by torch, written through
+    its address."""
+    out = torch.empty(values.shape, dtype=values.dtype)
+    values = values.detach().contiguous()
+    ctypes.memmove(out.data_ptr(), values.data_ptr(), values.numel() * values.element_size())
+    return out
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The operators with their kernels replaced by the same sums on the CPU."""
+    off = torch._C._DisableTorchDispatch  # a kernel's work is out of torch's sight
+
+    def quiet(f):
+        def run(*args, **kw):
+            state = torch._C._get_tracing_state()
+            torch._C._set_tracing_state(None)
+            try:
+                with off(), torch.no_grad():
+                    values = f(*args, **kw)
+            finally:
+                torch._C._set_tracing_state(state)
+            return values
+
+        return run
+
+    def scores(logits, tokens, top_k, temperature, ignore_index, with_stats=True):
+        logp = quiet(lambda: torch.log_softmax(logits / temperature, -1))()
+        lp = _written(quiet(lambda: logp.gather(1, tokens[:, None])[:, 0].contiguous())())
+        ent = _written(quiet(lambda: -(logp.exp() * logp).sum(-1))())
+        return lp, ent, None, None, torch.zeros(len(tokens), 2)
+
+    def distill(logits, ids, tl, temperature, weight, ignore_index, reduction, gradient=False):
+        q = quiet(lambda: torch.softmax(tl / temperature, -1))()
+        logp = quiet(lambda: torch.log_softmax(logits / temperature, -1))()
+        loss = quiet(lambda: (q * (q.log() - logp.gather(1, ids))).sum(-1).mean())()
+        return _written(loss), torch.zeros(1), torch.zeros_like(logits) if gradient else None
+
+    def lookup(tokens, weight, scale, dtype):
+        return _written(quiet(lambda: (weight[tokens] * scale).to(dtype))())
+
+    monkeypatch.setattr(ops, "token_scores_forward", scores)
+    monkeypatch.setattr(ops, "distill_forward", distill)
+    monkeypatch.setattr(ops, "embedding_forward", lookup)
+    monkeypatch.setattr(ops, "capture_id", lambda device: 0)
+    monkeypatch.setattr(ops, "embedding_backward", lambda t, g, *a: _written(
+        quiet(lambda: torch.zeros(5, 3).index_add_(0, t, g))()))
+    ids = torch.tensor([[1, 2], [0, 1], [2, 1]])
+    t = torch.tensor([1, 0, 2])
+    tl = torch.tensor([[0.0, 1.0], [2.0, 1.0], [0.5, 0.5]])
+    return {
+        "token_log_probs": lambda x: dabsn_b200.token_log_probs(x[:3], t).log_prob,
+        "distillation_loss": lambda x: dabsn_b200.distillation_loss(x[:3], ids, tl),
+        "embedding": lambda x: dabsn_b200.embedding(t, x),
+    }
+
+
+NAMES = ["token_log_probs", "distillation_loss", "embedding"]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(host, name, grad):
+    x = torch.randn(5, 3).requires_grad_(grad)
+    want = host[name](x)
+    with forward_ad.dual_level():
+        assert torch.equal(host[name](x), want)  # no tangent: as without
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            host[name](dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            host[name](dual)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(host[name], (x.detach(),), (torch.ones_like(x),))
+
+
+def test_forward_mode_of_the_teacher_and_of_a_reverse_is_refused(host):
+    x = torch.randn(3, 4)
+    ids, tl = torch.tensor([[1], [0], [2]]), torch.zeros(3, 1)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            dabsn_b200.distillation_loss(x, ids, forward_ad.make_dual(tl, torch.ones_like(tl)))
+    w = torch.randn(5, 3, requires_grad=True)
+    out = host["embedding"](w)
+    (g,) = torch.autograd.grad(out, w, torch.ones_like(out), retain_graph=True)
+    assert g.sum(-1).tolist() == [3.0, 3.0, 3.0, 0.0, 0.0]
+    with forward_ad.dual_level():
+        up = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, w, up)
