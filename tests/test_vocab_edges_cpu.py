@@ -8,6 +8,7 @@ import ctypes
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import dabsn_b200
 from dabsn_b200 import _native, ops
@@ -154,3 +155,20 @@ def test_forward_mode_of_the_teacher_and_of_a_reverse_is_refused(host):
         up = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(out, w, up)
+
+
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_make_fx_is_refused(host, name, grad, pre_dispatch):
+    x = torch.randn(5, 3).requires_grad_(grad)
+    with pytest.raises(RuntimeError, match="make_fx"):
+        make_fx(host[name], pre_dispatch=pre_dispatch)(x)
+    host[name](x)
+
+
+def test_make_fx_of_a_reverse_is_refused(host):
+    w = torch.randn(5, 3, requires_grad=True)
+    out = host["embedding"](w)
+    with pytest.raises(RuntimeError, match="make_fx"):
+        make_fx(lambda g: torch.autograd.grad(out, w, g)[0])(torch.ones_like(out))
