@@ -663,10 +663,11 @@ def _once_differentiable(backward):
 
 
 def _differentiates(t: Tensor) -> bool:
-    """Whether a call has to record its reverse; without one the operators
-    below run their forward directly (a node costs a single token's call more
-    than its kernel)."""
-    return t.requires_grad and torch.is_grad_enabled()
+    """Whether a call goes through its autograd function: to record its reverse,
+    or as the operation that ``torch.jit.trace`` records.  Otherwise the
+    operators below run their forward directly (a node costs a single token's
+    call more than its kernel)."""
+    return t.requires_grad and torch.is_grad_enabled() or torch._C._is_tracing()
 
 
 class _TokenScores(torch.autograd.Function):
@@ -762,7 +763,7 @@ class _Distillation(torch.autograd.Function):
                 reduction):
         loss, ws, ctx.ready = ops.distill_forward(logits, teacher_tokens, teacher_logits,
                                                   temperature, weight, ignore_index, reduction,
-                                                  reduction != "none")
+                                                  ctx.needs_input_grad[0] and reduction != "none")
         ctx.save_for_backward(logits, ws)
         ctx.meta = (teacher_tokens.shape[1], temperature, weight, reduction == "mean")
         ctx.capture = ops.capture_id(logits.device)

@@ -259,6 +259,20 @@ def _calls(lib):
             lambda z: lib.embedding(t % 4, z) + 0)
 
 
+def test_traced_and_compiled_calls_compute(lib):
+    x, y = _logits(4, 50, F32, 1), _logits(4, 50, F32, 2)
+    for call in _calls(lib):
+        traced = torch.jit.trace(call, (x,))
+        assert torch.equal(traced(y), call(y)) and torch.equal(traced(x), call(x))
+        torch._dynamo.reset()
+        compiled = torch.compile(call, backend="eager")
+        assert torch.equal(compiled(y), call(y))
+        a, b = y.clone().requires_grad_(), y.clone().requires_grad_()
+        (got,) = torch.autograd.grad(compiled(a).sum(), a)
+        (want,) = torch.autograd.grad(call(b).sum(), b)
+        assert torch.equal(got, want)
+
+
 def test_forward_mode_is_refused(lib):
     x = _logits(4, 50, F32, 1)
     for call in _calls(lib):

@@ -157,6 +157,16 @@ def test_forward_mode_of_the_teacher_and_of_a_reverse_is_refused(host):
             torch.autograd.grad(out, w, up)
 
 
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", NAMES)
+def test_a_traced_call_computes(host, name, grad):
+    """torch.jit.trace records the operator, not the allocation of its result."""
+    traced = torch.jit.trace(host[name], (torch.randn(5, 3).requires_grad_(grad),))
+    for seed in range(3):
+        x = torch.randn(5, 3, generator=torch.Generator().manual_seed(seed))
+        assert torch.equal(traced(x).detach(), host[name](x))
+
+
 @pytest.mark.parametrize("pre_dispatch", [False, True])
 @pytest.mark.parametrize("grad", [False, True])
 @pytest.mark.parametrize("name", NAMES)
