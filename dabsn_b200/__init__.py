@@ -14,11 +14,14 @@ are a C-ABI shared library (``include/dabsn_b200.h``) loaded with ctypes;
 ``token_log_probs``, ``distillation_loss`` and ``embedding`` are differentiable
 functions of torch tensors that need neither the reference nor ``install``:
 scoring and distillation over a model's logits, and its token embedding.
+``raise_on_device_status`` raises what their kernels (and the others) could only
+record on the device, an id outside the vocabulary for instance.
 """
 
 from __future__ import annotations
 
-from .autograd import TokenLogProbs, distillation_loss, embedding, token_log_probs
+from .autograd import (TokenLogProbs, distillation_loss, embedding, raise_on_device_status,
+                       token_log_probs)
 from .backend import b200_status, enable, enable_b200, install, native_available, status
 
 __all__ = [
@@ -30,6 +33,7 @@ __all__ = [
     "enable_b200",
     "install",
     "native_available",
+    "raise_on_device_status",
     "status",
     "token_log_probs",
 ]

@@ -218,8 +218,8 @@ DEVICE_CODES = {
 
 
 def raise_on_device_status() -> None:
-    """Raise when an earlier launch recorded an error in the device's status
-    word.
+    """Raise when an earlier launch recorded an error in the current device's
+    status word.
 
     Every device-side wait of this library is bounded; one that gives up
     records a code there and ends its launch early, so that launch's outputs
@@ -227,7 +227,9 @@ def raise_on_device_status() -> None:
     vocabulary the same way (the reference raises on it).  The word is read
     (and cleared) here, at host points where the step synchronises anyway
     (the admitted bank's width read), so the error reaches the caller instead
-    of passing silently.  Reading it synchronises the device."""
+    of passing silently.  Reading it waits for the default stream and the
+    streams that block it, not for torch's side streams:
+    ``dabsn_b200.raise_on_device_status`` waits for the device."""
     code = device_status(reset=True)
     if code != 0:
         what = DEVICE_CODES.get(code, f"device status code {code}")

@@ -622,6 +622,17 @@ def make_ce_from_logits(original):
     return chunked_cross_entropy_from_logits
 
 
+def raise_on_device_status(device: torch.device | int | None = None) -> None:
+    """Waits for the device (the current one by default) and raises a
+    ``RuntimeError`` if a kernel recorded an error there since the last time: an
+    id outside the vocabulary, a bounded wait that gave up.  The outputs of that
+    launch are then invalid.  The operators do not wait for the device, so a
+    program calls this where such an error has to stop it."""
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        _native.raise_on_device_status()
+
+
 class TokenLogProbs(NamedTuple):
     """What :func:`token_log_probs` returns: FP32 numbers shaped like the
     tokens, and the alternatives with one more axis (int64 ids), None where
@@ -728,8 +739,8 @@ def token_log_probs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatu
     first ids as alternatives.  NaN or +inf among the logits makes the row's
     numbers NaN (its alternatives' ids are then valid but unspecified).  A
     token outside [0, V) makes its log-probability and, unless the upstream
-    gradient is 0, that one's gradient NaN and is raised at the next
-    synchronisation (device status 8)."""
+    gradient is 0, that one's gradient NaN and records device status 8, which
+    ``dabsn_b200.raise_on_device_status()`` raises; no call here waits for it."""
     if tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens has shape {tuple(tokens.shape)}, expected "
                          f"{tuple(logits.shape[:-1])}")
@@ -807,7 +818,8 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     is -inf makes the loss +inf; NaN or +inf among a row's teacher logits makes its
     loss, and the gradient of the listed tokens, NaN.  An id outside [0, V) makes
     the row's loss and, unless its upstream gradient is 0, its gradient NaN and
-    is raised at the next synchronisation (device status 8)."""
+    records device status 8, which ``dabsn_b200.raise_on_device_status()``
+    raises; no call here waits for it."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean, sum or none, got {reduction!r}")
     shape = logits.shape[:-1]
@@ -865,8 +877,8 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0,
     tokens sorted by id, in order of position, so it is the same every time.
     Tokens equal to ``padding_idx`` (negative: from the end, as in
     ``torch.nn.functional.embedding``) take no part in it.  A token outside
-    [0, V) gives a NaN row and is raised at the next synchronisation (device
-    status 8)."""
+    [0, V) gives a NaN row and records device status 8, which
+    ``dabsn_b200.raise_on_device_status()`` raises; no call here waits for it."""
     if weight.dim() != 2:
         raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
     if padding_idx is not None:

@@ -282,3 +282,23 @@ def test_forward_mode_is_refused(lib):
                 call(dual)
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
+def test_the_status_of_another_stream_is_raised(lib):
+    """raise_on_device_status waits for work that is still queued on a stream of
+    its own."""
+    w = torch.randn(5, 16, device="cuda")
+    bad, good = torch.tensor([1, 5], device="cuda"), torch.tensor([1, 4], device="cuda")
+    lib.embedding(good, w)
+    lib.raise_on_device_status()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        lib.embedding(bad, w)
+    with pytest.raises(RuntimeError, match="outside"):
+        lib.raise_on_device_status()
+    lib.raise_on_device_status()
+    lib.embedding(bad, w)
+    with pytest.raises(RuntimeError, match="outside"):
+        lib.raise_on_device_status(0)

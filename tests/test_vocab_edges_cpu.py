@@ -3,6 +3,7 @@ way on the host; no GPU is needed."""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import pytest
@@ -182,3 +183,21 @@ def test_make_fx_of_a_reverse_is_refused(host):
     out = host["embedding"](w)
     with pytest.raises(RuntimeError, match="make_fx"):
         make_fx(lambda g: torch.autograd.grad(out, w, g)[0])(torch.ones_like(out))
+
+
+# ---------------------------------------------------------------------------
+# What the kernels can only record
+# ---------------------------------------------------------------------------
+def test_the_device_status_can_be_raised(monkeypatch):
+    codes, waits = [8, 0], []
+    monkeypatch.setattr(_native, "device_status", lambda reset=False: codes.pop(0))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: waits.append(1))
+    monkeypatch.setattr(torch.cuda, "device", contextlib.nullcontext)
+    with pytest.raises(RuntimeError, match="outside"):
+        dabsn_b200.raise_on_device_status()
+    dabsn_b200.raise_on_device_status()
+    assert len(waits) == 2
+    for name in NAMES:
+        text = getattr(dabsn_b200, name).__doc__
+        assert "dabsn_b200.raise_on_device_status()" in text
+        assert "next synchronisation" not in " ".join(text.split())
