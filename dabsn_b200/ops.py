@@ -940,7 +940,8 @@ def token_scores_forward(logits: Tensor, tokens: Tensor, top_k: int, temperature
     top_ids = torch.empty((rows, k), device=dev, dtype=torch.int64) if k else None
     _run("token_scores_fwd", dev, N.load().dabsn_token_scores_fwd, code, rows, V, ld,
          logits.data_ptr(), tokens.data_ptr(), ignore_index, temperature, k, log_prob.data_ptr(),
-         entropy.data_ptr(), _addr(stats), _addr(top_values), _addr(top_ids))
+         entropy.data_ptr(), _addr(stats), _addr(top_values), _addr(top_ids),
+         launches=1 if rows else 0)
     return log_prob, entropy, top_values, top_ids, stats
 
 
@@ -956,7 +957,8 @@ def token_scores_backward(logits: Tensor, tokens: Tensor, temperature: float, ig
     dl, ldd = _gradient_rows(logits, ld)
     _run("token_scores_bwd", dev, N.load().dabsn_token_scores_bwd, act_code(logits.dtype), rows,
          V, ld, logits.data_ptr(), tokens.data_ptr(), ignore_index, _temperature(temperature),
-         stats.data_ptr(), entropy.data_ptr(), _addr(g), _addr(h), dl.data_ptr(), ldd)
+         stats.data_ptr(), entropy.data_ptr(), _addr(g), _addr(h), dl.data_ptr(), ldd,
+         launches=1 if rows else 0)
     return dl
 
 
@@ -993,7 +995,7 @@ def distill_forward(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Tens
     _run("distill_grad" if gradient else "distill_fwd", dev, lib.dabsn_distill_fwd, code, rows, V,
          ld, logits.data_ptr(), teacher, K, ids.data_ptr(), tl.data_ptr(), ignore_index,
          temperature, weight, reduction == "mean", ws.data_ptr(), _addr(row_loss), _addr(result),
-         _addr(dl), ldd, launches=2 if result is None else 3)
+         _addr(dl), ldd, launches=0 if rows == 0 else 2 if result is None else 3)
     return (row_loss if result is None else result), ws, dl
 
 
@@ -1010,7 +1012,8 @@ def distill_backward(logits: Tensor, workspace: Tensor, entries: int, temperatur
     dl, ldd = _gradient_rows(logits, ld) if ready is None else (ready, _logit_rows(ready)[2])
     _run("distill_bwd", dev, N.load().dabsn_distill_bwd, act_code(logits.dtype), rows, V, ld,
          logits.data_ptr(), entries, workspace.data_ptr(), temperature, weight, mean,
-         up.data_ptr(), up.dim() > 0, ready is not None, dl.data_ptr(), ldd)
+         up.data_ptr(), up.dim() > 0, ready is not None, dl.data_ptr(), ldd,
+         launches=1 if rows else 0)
     return dl
 
 
@@ -1036,8 +1039,17 @@ def embedding_forward(tokens: Tensor, weight: Tensor, scale: float, dtype: torch
     out = torch.empty((*tokens.shape, D), device=dev, dtype=dtype)
     _run("embedding_fwd", dev, N.load().dabsn_embedding_fwd, act_code(w.dtype), act_code(dtype),
          ids.numel(), V, D, ids.data_ptr(), w.data_ptr(), w.stride(0) if V > 1 else D, scale,
-         out.data_ptr())
+         out.data_ptr(), launches=1 if ids.numel() else 0)
     return out
+
+
+def _embedding_launches(n: int, vocab: int) -> int:
+    """Launches of the table's gradient of n tokens (embedding.cu): the sort, one
+    up to 8192 tokens and two for each digit of the ids 0 to vocab above, the
+    sums, and the join where there are more than two chunks of positions."""
+    if n <= 8192:
+        return (n > 0) + 1 + (n > 2 * 32)
+    return 2 * ((vocab.bit_length() + 7) // 8) + 2
 
 
 def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: float,
@@ -1054,7 +1066,7 @@ def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: floa
     ws = torch.empty(need, device=dev, dtype=torch.uint8)
     _run("embedding_bwd", dev, lib.dabsn_embedding_bwd, act_code(g.dtype), act_code(dtype), n,
          vocab, D, ids.data_ptr(), -1 if padding_idx is None else padding_idx, g.data_ptr(),
-         scale, dw.data_ptr(), ws.data_ptr(), need, launches=3 if n <= 8192 else 6)
+         scale, dw.data_ptr(), ws.data_ptr(), need, launches=_embedding_launches(n, vocab))
     return dw
 
 

@@ -302,3 +302,69 @@ def test_the_status_of_another_stream_is_raised(lib):
     lib.embedding(bad, w)
     with pytest.raises(RuntimeError, match="outside"):
         lib.raise_on_device_status(0)
+
+
+# ---------------------------------------------------------------------------
+# Counted launches
+# ---------------------------------------------------------------------------
+def _kernels_of(call):
+    """Kernels in a graph of the call, and how many the library counted."""
+    from cuda.bindings import runtime as rt
+
+    from dabsn_b200 import ops
+
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    before = ops.LAUNCH_COUNT["n"]
+    with torch.cuda.graph(graph):
+        call()
+    counted = ops.LAUNCH_COUNT["n"] - before
+    raw = rt.cudaGraph_t(graph.raw_cuda_graph())
+    err, _, total = rt.cudaGraphGetNodes(raw, 0)
+    assert err == rt.cudaError_t.cudaSuccess
+    if total == 0:
+        return 0, counted
+    err, nodes, total = rt.cudaGraphGetNodes(raw, total)
+    assert err == rt.cudaError_t.cudaSuccess
+    kinds = [rt.cudaGraphNodeGetType(node)[1] for node in nodes[:total]]
+    return sum(k == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for k in kinds), counted
+
+
+@pytest.mark.parametrize("n,V", [(0, 9), (1, 9), (64, 9), (65, 9), (96, 9), (97, 300),
+                                 (8192, 300), (8193, 9), (8193, 255), (8193, 256), (8193, 65535),
+                                 (40000, 65536), (40000, 1009)])
+def test_launches_of_the_embedding(lib, n, V):
+    from dabsn_b200 import ops
+
+    t = torch.zeros(n, dtype=torch.int64, device="cuda")
+    w = torch.zeros(V, 8, device="cuda")
+    g = torch.zeros(n, 8, device="cuda")
+    for call in (lambda: ops.embedding_forward(t, w, 1.0, F32),
+                 lambda: ops.embedding_backward(t, g, V, 1.0, None, F32)):
+        call()
+        kernels, counted = _kernels_of(call)
+        assert kernels == counted
+
+
+@pytest.mark.parametrize("rows", [0, 3])
+def test_launches_of_scores_and_distillation(lib, rows):
+    from dabsn_b200 import ops
+
+    x, t = _logits(rows, 40, F32, 1), torch.zeros(rows, dtype=torch.int64, device="cuda")
+    ids, tl = t[:, None].contiguous(), torch.zeros(rows, 1, device="cuda")
+    for k in (0, 3):
+        lp, h, _, _, stats = ops.token_scores_forward(x, t, k, 1.0, -100)
+        kernels, counted = _kernels_of(lambda: ops.token_scores_forward(x, t, k, 1.0, -100))
+        assert kernels == counted
+        kernels, counted = _kernels_of(
+            lambda: ops.token_scores_backward(x, t, 1.0, -100, stats, h, lp, h))
+        assert kernels == counted
+    for reduction in ("none", "sum"):
+        def forward(reduction=reduction):
+            return ops.distill_forward(x, ids, tl, 1.0, 1.0, -100, reduction, reduction == "sum")
+
+        loss, ws, _ = forward()
+        kernels, counted = _kernels_of(forward)
+        assert kernels == counted
+        kernels, counted = _kernels_of(
+            lambda: ops.distill_backward(x, ws, 1, 1.0, 1.0, False, loss))
+        assert kernels == counted
