@@ -83,8 +83,11 @@ __device__ __forceinline__ void store_w(T* p, const float (&v)[W]) {
   } else if constexpr (W == 4 && sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   } else if constexpr (W == 4) {
-    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
-    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(h);
+    uint2 u;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+    h[0] = __floats2bfloat162_rn(v[0], v[1]);
+    h[1] = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = u;
   } else {
     p[0] = from_f<T>(v[0]);
   }
@@ -93,7 +96,7 @@ __device__ __forceinline__ void store_w(T* p, const float (&v)[W]) {
 // A 16-byte vector (or one element) as it was loaded, and as FP32.
 template <int W, typename T>
 struct Raw {
-  T v[W];
+  alignas(W * sizeof(T)) T v[W];
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (W > 1) {
       static_assert(W * sizeof(T) == 16, "16 bytes");
@@ -104,6 +107,8 @@ struct Raw {
   }
   __device__ __forceinline__ float at(int i) const { return to_f<T>(v[i]); }
 };
+static_assert(alignof(Raw<4, float>) == 16 && alignof(Raw<8, bf16>) == 16,
+              "written as one vector, wherever the compiler keeps it");
 
 // ---------------------------------------------------------------------------
 // Lookup: each CTA copies a group of rows, a thread per unit.  131072 Zipf rows
