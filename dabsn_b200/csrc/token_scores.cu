@@ -577,6 +577,11 @@ extern "C" int dabsn_token_scores_fwd(int dtype, int64_t rows, int64_t V, int64_
               TS_MAX_K);
     return DABSN_ERR_UNSUPPORTED;
   }
+  // the selection's scans of a row step past its end by up to a CTA's threads
+  if (top_k > 0 && V > INT32_MAX - TS_FEW_THREADS) {
+    set_error("token_scores_fwd: V=%lld is too long for alternatives", (long long)V);
+    return DABSN_ERR_SHAPE;
+  }
   if (rows == 0) return DABSN_OK;
   int null = check_pointers("token_scores_fwd", {logits, tokens, log_prob, entropy});
   if (!null && top_k > 0) null = check_pointers("token_scores_fwd", {top_values, top_ids});

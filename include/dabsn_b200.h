@@ -490,7 +490,8 @@ uint64_t dabsn_capture_id(void* stream);
 /* Log-probabilities of given tokens, with entropy and top alternatives.
  *   logits [rows, V] FP32/BF16, rows contiguous and `ld` elements apart, any
  *   alignment; tokens [rows] int64 (rows of ignore_index are not read);
- *   temperature in [1e-6, 1e6]; 0 <= top_k <= min(128, V).
+ *   temperature in [1e-6, 1e6]; 0 <= top_k <= min(128, V); V < 2^31 - 512 with
+ *   alternatives, else V < 2^31 - 1.
  *   log_prob, entropy [rows] FP32; stats FP32 [rows, 2] (maximum, sum of
  *   exponentials; for the reverse, may be null); top_values FP32 and top_ids
  *   int64 [rows, top_k], most likely first, equal logits by the lower id.

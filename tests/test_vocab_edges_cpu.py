@@ -201,3 +201,18 @@ def test_the_device_status_can_be_raised(monkeypatch):
         text = getattr(dabsn_b200, name).__doc__
         assert "dabsn_b200.raise_on_device_status()" in text
         assert "next synchronisation" not in " ".join(text.split())
+
+
+def test_rows_too_long_for_alternatives_are_refused():
+    """The scans for alternatives step 512 elements at a time through 32-bit
+    indices, which a row of nearly 2^31 would carry past the largest."""
+    lib = _native.load()
+
+    def scores(V, k):
+        return lib.dabsn_token_scores_fwd(0, 0, V, V, None, None, -100, ctypes.c_float(1.0), k,
+                                          *([None] * 6))
+
+    assert scores(2 ** 31 - 2, 1) and b"alternatives" in lib.dabsn_last_error()
+    assert scores(2 ** 31 - 512, 1) and scores(2 ** 31 - 513, 1) == 0
+    assert scores(2 ** 31 - 2, 0) == 0
+    assert 2 ** 31 - 513 + 512 < 2 ** 31  # the largest index that the scans form
