@@ -1018,10 +1018,13 @@ def distill_backward(logits: Tensor, workspace: Tensor, entries: int, temperatur
 
 
 def capture_id(device: torch.device) -> int:
-    """Identity of the CUDA graph capture that the current stream is in (0: none)."""
-    if not torch.cuda.is_current_stream_capturing():
+    """Identity of the CUDA graph capture that ``device``'s current stream is in
+    (0: none)."""
+    if (torch.cuda.current_device() == device.index
+            and not torch.cuda.is_current_stream_capturing()):
         return 0
-    return N.load().dabsn_capture_id(torch._C._cuda_getCurrentRawStream(device.index))
+    with torch.cuda.device(device):
+        return N.load().dabsn_capture_id(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def embedding_forward(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) -> Tensor:

@@ -216,3 +216,19 @@ def test_rows_too_long_for_alternatives_are_refused():
     assert scores(2 ** 31 - 512, 1) and scores(2 ** 31 - 513, 1) == 0
     assert scores(2 ** 31 - 2, 0) == 0
     assert 2 ** 31 - 513 + 512 < 2 ** 31  # the largest index that the scans form
+
+
+def test_the_capture_is_that_of_the_logits_device(monkeypatch):
+    """A call on another device than the current one asks that device's stream."""
+    class Lib:
+        @staticmethod
+        def dabsn_capture_id(stream):
+            return {10: 0, 11: 7}[stream]
+
+    monkeypatch.setattr(_native, "load", lambda: Lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "device", contextlib.nullcontext)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 10 + i, raising=False)
+    assert ops.capture_id(torch.device("cuda", 0)) == 0
+    assert ops.capture_id(torch.device("cuda", 1)) == 7
