@@ -874,7 +874,8 @@ def embedding(tokens: Tensor, weight: Tensor, *, scale: float = 1.0,
     the table's by default), rounded once.
 
     The table's gradient is dense, in the table's dtype: FP32 sums over the
-    tokens sorted by id, in order of position, so it is the same every time.
+    tokens sorted by id and position, in a fixed order, so it is the same every
+    time.
     Tokens equal to ``padding_idx`` (negative: from the end, as in
     ``torch.nn.functional.embedding``) take no part in it.  A token outside
     [0, V) gives a NaN row and records device status 8, which

@@ -6,10 +6,11 @@
 // Both are bound by memory: the lookup writes N x D and reads the rows used,
 // the gradient reads N x D and writes the whole table (zeros where no token
 // points).  The gradient's sums run over the tokens sorted by id, positions
-// ascending inside an id, so no atomics are needed and the result does not
-// depend on scheduling: a stable radix sort of (id, position), digits of at
-// most eight bits, then one sum per run of equal ids in FP32, rounded once to
-// the table's type.
+// ascending inside an id, so no atomics are needed: a stable radix sort of (id,
+// position), digits of at most eight bits, then one sum per run of equal ids in
+// FP32, rounded once to the table's type.  A long run is summed in pieces, which
+// are added up in an order of their own; the tokens alone fix it, so the result is
+// the same every time.
 //
 // Tokens outside [0, V) give NaN rows and status 8, and take no part in the
 // gradient; nor do tokens equal to the padding id.
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(EM_THREADS) sort_place_kernel(
   for (long long unit = first; unit < last; unit += RS_UNIT) {
     for (int w = 0; w < RS_WARPS; ++w) offset[w][t] = 0;
     __syncthreads();
-    // a warp ranks 512 consecutive elements, 32 at a time, in order
+    // a warp ranks 32 * RS_ITEMS consecutive elements, 32 at a time, in order
     int k[RS_ITEMS], rank[RS_ITEMS];
 #pragma unroll
     for (int j = 0; j < RS_ITEMS; ++j) {
@@ -453,6 +454,11 @@ GradPlan grad_plan(int64_t N, int64_t V, int units) {
   g.units = units;
   g.tiles = (units + EM_THREADS - 1) / EM_THREADS;
   g.wide = (units + g.tiles - 1) / g.tiles;
+  // Longer chunks leave fewer partial sums, shorter ones more groups for a small
+  // call.  Runs and join with 32 and 64, Zipf tokens: 32000 x 2048 BF16, 61 and 69
+  // us for 8192 tokens, 65 and 67 for 16384, 80 and 76 for 32768, 169 and 161 for
+  // 131072; 32000 x 512 FP32, 25 and 35, 28 and 37, 35 and 38, 80 and 70; 1009 x
+  // 515 FP32, 21 and 28, 30 and 35, 48 and 46, 154 and 131.
   g.chunk = N >= 32768 ? GR_CHUNK_MAX : 32;
   g.groups = std::min(EM_THREADS / g.wide, GR_POSITIONS / GR_CHUNK_MAX);
   g.chunks = (int)((N + g.chunk - 1) / g.chunk);

@@ -39,11 +39,18 @@ typedef unsigned long long u64;
 constexpr int TS_THREADS = 256;
 // Up to three rows an SM, long rows go to 512 threads each: those of more than
 // 24 KB, or with alternatives, whose selection takes longer among more threads, of
-// more than 96 KB.  148 rows, 256 threads and 512: BF16 of 32000 in 7.5 and 6.2
-// us, with 20 alternatives in 11.3 and 11.7; FP32 of 32000 in 10.3 and 8.2, 14.9
-// and 13.1; FP32 of 128000 in 28.8 and 19.9, 44.9 and 31.5.  At 444 rows the two
-// are level for BF16 rows of 32000 (10.0 and 10.2 us), and FP32 rows of 128000
-// with alternatives take 69.5 and 58.8 us.
+// more than 96 KB.  Device us with 256 threads a row and with 512:
+//   rows                         8        148        444        592
+//   BF16 x 8000 (16 KB)     4.0  3.2   4.7  4.1   6.2  5.7   6.6  7.9
+//   FP32 x 8000 (32 KB)     4.6  4.0   5.7  5.2   7.1  7.2   7.9  9.9
+//   BF16 x 32000            6.2  4.9   7.3  6.2  10.2 10.1  11.6 13.7
+//   FP32 x 128000          25.9 15.8  28.6 19.8  42.9 41.4  53.9 60.1
+// and with 20 alternatives:
+//   BF16 x 32000 (64 KB)   10.3 10.5  11.8 12.2  15.1 16.2  17.4 19.1
+//   FP32 x 32000 (128 KB)  13.0 11.7  15.4 14.0  22.7 21.8  27.5 26.3
+//   BF16 x 128000          23.1 17.8  25.8 20.8  41.7 36.6  48.6 45.3
+//   FP32 x 128000          33.0 22.2  43.9 32.1  69.9 59.8  87.5 77.8
+// (888 rows: 67.2 and 74.6 for BF16 x 128000, 37.0 and 41.1 for FP32 x 32000.)
 constexpr int TS_FEW_THREADS = 512;
 constexpr int TS_FEW_ROWS = 444;
 constexpr int TS_FEW_BYTES = 24 * 1024;

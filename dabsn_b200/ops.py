@@ -1039,10 +1039,11 @@ def embedding_forward(tokens: Tensor, weight: Tensor, scale: float, dtype: torch
     w = weight
     if w.stride(1) != 1 or w.stride(0) < D:
         w = w.contiguous()
+    n = ids.numel()
     out = torch.empty((*tokens.shape, D), device=dev, dtype=dtype)
     _run("embedding_fwd", dev, N.load().dabsn_embedding_fwd, act_code(w.dtype), act_code(dtype),
-         ids.numel(), V, D, ids.data_ptr(), w.data_ptr(), w.stride(0) if V > 1 else D, scale,
-         out.data_ptr(), launches=1 if ids.numel() else 0)
+         n, V, D, ids.data_ptr(), w.data_ptr(), w.stride(0) if V > 1 else D, scale,
+         out.data_ptr(), launches=1 if n else 0)
     return out
 
 
@@ -1058,7 +1059,8 @@ def _embedding_launches(n: int, vocab: int) -> int:
 def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: float,
                        padding_idx: int | None, dtype: torch.dtype) -> Tensor:
     """The table's gradient [vocab, D] in ``dtype`` from grad_out [..., D]: sums
-    over equal tokens in FP32, in order of position (no atomics)."""
+    over equal tokens in FP32, in an order that the tokens alone fix (no
+    atomics)."""
     dev = _same_cuda(grad_out, tokens)
     ids = _int_rows(tokens, grad_out.shape[:-1], "tokens")
     n, D = ids.numel(), grad_out.shape[-1]

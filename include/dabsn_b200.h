@@ -529,8 +529,8 @@ size_t dabsn_distill_workspace(int64_t rows, int64_t K);
 int dabsn_distill_fwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int teacher_dtype, int64_t K, const int64_t* teacher_tokens,
                       const void* teacher_logits, int64_t ignore_index, float temperature,
-                      float weight, int mean, void* workspace, float* row_loss, float* result, void* dlogits,
-                      int64_t ldd, void* stream);
+                      float weight, int mean, void* workspace, float* row_loss, float* result,
+                      void* dlogits, int64_t ldd, void* stream);
 int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void* logits,
                       int64_t K, const void* workspace, float temperature, float weight,
                       int mean, const float* upstream, int64_t upstream_stride, int unless_one,
@@ -540,7 +540,7 @@ int dabsn_distill_bwd(int dtype, int64_t rows, int64_t V, int64_t ld, const void
  * with rows `ldw` elements apart; tables and outputs FP32 or BF16.  A token
  * outside [0, V) gives a NaN row and device status 8.
  * Reverse: dweight [V, D] contiguous = scale * sums of dout [N, D] over equal
- * tokens, in order of position (FP32, no atomics); tokens outside [0, V) and
+ * tokens, in an order that the tokens alone fix (FP32, no atomics); tokens outside [0, V) and
  * tokens equal to padding_idx (-1: none) take no part.  `workspace` holds at
  * least dabsn_embedding_bwd_workspace bytes, 16-byte aligned. */
 int dabsn_embedding_fwd(int weight_dtype, int out_dtype, int64_t N, int64_t V, int64_t D,
