@@ -648,14 +648,15 @@ def _refuse_transforms(*tensors: Tensor | None) -> None:
     """Refuses what would lose a kernel's work without an error: forward-mode
     derivatives (the kernels write plain memory, so a tangent would vanish and
     read as zero) and ``make_fx`` (it would record the allocation of the results
-    and not what writes them).  Outside of both this reads two variables: a
-    single token's call takes 11.5 us."""
+    and not what writes them).  Outside of both this reads two variables, the
+    second one another thread's as well: a single token's call takes 11.5 us."""
     if forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(
                     "dabsn_b200: forward-mode derivatives are not implemented")
-    if proxy_tensor._CURRENT_MAKE_FX_TRACER is not None:
+    if (proxy_tensor._CURRENT_MAKE_FX_TRACER is not None
+            and proxy_tensor.get_proxy_mode() is not None):
         raise RuntimeError("dabsn_b200: make_fx cannot trace kernels that are not dispatcher "
                            "operators")
 

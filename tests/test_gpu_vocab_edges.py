@@ -368,3 +368,17 @@ def test_launches_of_scores_and_distillation(lib, rows):
         kernels, counted = _kernels_of(
             lambda: ops.distill_backward(x, ws, 1, 1.0, 1.0, False, loss))
         assert kernels == counted
+
+
+def test_make_fx_is_refused(lib):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = _logits(4, 50, F32, 1)
+    for call in _calls(lib):
+        for pre_dispatch in (False, True):
+            with pytest.raises(RuntimeError, match="make_fx"):
+                make_fx(call, pre_dispatch=pre_dispatch)(x)
+        leaf = x.clone().requires_grad_()
+        out = call(leaf)
+        with pytest.raises(RuntimeError, match="make_fx"):  # on the engine's thread
+            make_fx(lambda g: torch.autograd.grad(out, leaf, g)[0])(torch.ones_like(out))

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -232,3 +233,20 @@ def test_the_capture_is_that_of_the_logits_device(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 10 + i, raising=False)
     assert ops.capture_id(torch.device("cuda", 0)) == 0
     assert ops.capture_id(torch.device("cuda", 1)) == 7
+
+
+def test_make_fx_in_another_thread_refuses_nothing_here(host):
+    """Only the thread that traces is refused."""
+    x, seen = torch.randn(5, 3), []
+
+    def other():
+        seen.append(host["embedding"](x))
+
+    def traced(z):
+        thread = threading.Thread(target=other)
+        thread.start()
+        thread.join()
+        return z + 1
+
+    make_fx(traced)(x)
+    assert len(seen) == 1 and torch.equal(seen[0], host["embedding"](x))
