@@ -915,10 +915,16 @@ def _int_rows(t: Tensor, shape, what: str) -> Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _dense(t: Tensor) -> Tensor:
+    """Contiguous, and as it stands in memory: the imaginary part of a conjugate is a
+    view whose sign is still to be turned."""
+    return t if t.is_contiguous() and not t.is_neg() else t.contiguous().resolve_neg()
+
+
 def _dense_f32(t: Tensor | None) -> Tensor | None:
-    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+    if t is None:
         return t
-    return t.to(torch.float32).contiguous()
+    return _dense(t if t.dtype is torch.float32 else t.to(torch.float32))
 
 
 def token_scores_forward(logits: Tensor, tokens: Tensor, top_k: int, temperature: float,
@@ -1064,7 +1070,7 @@ def embedding_backward(tokens: Tensor, grad_out: Tensor, vocab: int, scale: floa
     dev = _same_cuda(grad_out, tokens)
     ids = _int_rows(tokens, grad_out.shape[:-1], "tokens")
     n, D = ids.numel(), grad_out.shape[-1]
-    g = grad_out if grad_out.is_contiguous() else grad_out.contiguous()
+    g = _dense(grad_out)
     dw = torch.empty((vocab, D), device=dev, dtype=dtype)
     lib = N.load()
     need = lib.dabsn_embedding_bwd_workspace(n, vocab, D)

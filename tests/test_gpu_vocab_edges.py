@@ -382,3 +382,25 @@ def test_make_fx_is_refused(lib):
         out = call(leaf)
         with pytest.raises(RuntimeError, match="make_fx"):  # on the engine's thread
             make_fx(lambda g: torch.autograd.grad(out, leaf, g)[0])(torch.ones_like(out))
+
+
+def test_a_gradient_with_a_pending_sign(lib):
+    """An upstream gradient that is the imaginary part of a conjugate: for one
+    number a contiguous view whose sign is still to be turned."""
+    x = _logits(1, 50, F32, 1)
+    t = torch.tensor([4], device="cuda")
+
+    def log_prob(z):
+        return lib.token_log_probs(z, t).log_prob
+
+    def column(z):
+        return lib.embedding(t * 0, z[:, :1])
+
+    for f in (log_prob, column):
+        a = x.clone().requires_grad_()
+        out = f(a)
+        up = torch.complex(torch.zeros_like(out), torch.full_like(out, 2.0)).detach().conj().imag
+        assert up.is_neg() and up.is_contiguous()
+        (want,) = torch.autograd.grad(out, a, torch.full_like(out, -2.0), retain_graph=True)
+        (got,) = torch.autograd.grad(out, a, up)
+        assert torch.equal(got, want) and float(want.abs().max()) > 0

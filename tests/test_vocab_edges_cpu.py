@@ -250,3 +250,19 @@ def test_make_fx_in_another_thread_refuses_nothing_here(host):
 
     make_fx(traced)(x)
     assert len(seen) == 1 and torch.equal(seen[0], host["embedding"](x))
+
+
+def test_upstream_gradients_with_a_pending_sign():
+    """The imaginary part of one conjugate number is a contiguous view with its
+    sign still to be turned."""
+    pending = torch.tensor([1.0 + 2.0j]).conj().imag
+    dense = ops._dense_f32(pending)
+    assert (ctypes.c_float * 1).from_address(dense.data_ptr())[0] == -2.0
+    assert pending.is_neg() and pending.is_contiguous()
+    wide = torch.tensor([[1.0 + 2.0j, 3.0 + 4.0j]]).conj().imag
+    dense = ops._dense(wide)
+    assert list((ctypes.c_float * 2).from_address(dense.data_ptr())) == [-2.0, -4.0]
+    assert ops._dense_f32(None) is None
+    plain = torch.randn(3)
+    assert ops._dense_f32(plain) is plain
+    assert ops._dense_f32(plain.double()).dtype == torch.float32
