@@ -818,10 +818,10 @@ def distillation_loss(logits: Tensor, teacher_tokens: Tensor, teacher_logits: Te
     and no gradient, and its logits are not read.  A listed token whose logit
     is -inf makes the loss +inf, as does one of the type's lowest value at a
     temperature below 1, where its quotient passes FP32; NaN or +inf among a
-    row's teacher logits makes its loss, and the gradient of the listed tokens, NaN.  An id outside [0, V) makes
-    the row's loss and, unless its upstream gradient is 0, its gradient NaN and
-    records device status 8, which ``dabsn_b200.raise_on_device_status()``
-    raises; no call here waits for it."""
+    row's teacher logits makes its loss, and the gradient of the listed tokens,
+    NaN.  An id outside [0, V) makes the row's loss and, unless its upstream
+    gradient is 0, its gradient NaN and records device status 8, which
+    ``dabsn_b200.raise_on_device_status()`` raises; no call here waits for it."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean, sum or none, got {reduction!r}")
     shape = logits.shape[:-1]
